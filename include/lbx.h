@@ -420,6 +420,144 @@ int lbx_kv_move(uint16_t *const *k_caches, uint16_t *const *v_caches, int32_t n_
                 int32_t kv_heads, int32_t max_seq, int32_t head_dim, const int32_t *src,
                 const int32_t *dst, int32_t n, cudaStream_t stream);
 
+/* ---- 8-bit integer product ----------------------------------------------
+ * No reference counterpart (the reference's dense layers, the lm_head among
+ * them, stay bf16): y = s_t * w_scale_n * sum_k c_tk w_nk (+ bias_n), with
+ * the tokens quantised in the call, a scale each, and the weights quantised
+ * beforehand, a scale for each output channel.
+ *
+ * lbx_quant_tokens: for each of m rows of x [m, k] (fp32 or bf16, row stride
+ * x_ld elements) a = max |x|, scale = a * (1/127 in fp32) and
+ * q = rint(x * i), i = 127 / a (0 where a = 0), each operation rounded to
+ * fp32, ties to even; |q| <= 127.  A row holding a NaN or an infinity gets
+ * scale NaN and codes 0.  q rows are q_ld bytes apart (q_ld >= k).  The same
+ * call quantises a weight matrix, its rows being the output channels. */
+int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, int32_t m, int32_t k, int8_t *q,
+                     int64_t q_ld, float *scale, cudaStream_t stream);
+
+typedef struct lbx_int8_args {
+  int32_t m, n, k;        /* tokens, output channels, input features (<= 131072:
+                             127 * 128 * k then fits the int32 sums)           */
+  int32_t x_dtype, y_dtype;
+  int32_t use_pdl;
+  const void *x; int64_t x_ld;        /* [m, k]                                */
+  const int8_t *w; int64_t w_ld;      /* [n, k] row-major; w 16-byte aligned,
+                                         w_ld a multiple of 16 bytes           */
+  const float *w_scale;   /* [n]                                               */
+  const float *bias;      /* [n] or NULL                                       */
+  void *y; int64_t y_ld;  /* [m, n]                                            */
+} lbx_int8_args;
+/* The sums are exact, so a token's bits depend neither on the other tokens of
+ * the call nor on how the work is split.  The workspace must be zero-filled
+ * once when it is allocated (split tiles add their integer partial sums there
+ * and leave it at zero); calls sharing one are ordered on one stream. */
+size_t lbx_linear_int8_workspace_size(int32_t m, int32_t n, int32_t k);
+int lbx_linear_int8(const lbx_int8_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
+
+/* ---- KV cache held in 4 bits ---------------------------------------------
+ * No reference counterpart (its cache is fp32, cpp:1183-1187).  Each head and
+ * slot holds head_dim codes of 4 bits and, for each group of 64 dimensions,
+ * a pair (step, least) in bf16; a value is least + step * code (4.5 bits a
+ * value).  Codes lie in 32-bit words of eight: block b = dimensions
+ * 8b .. 8b+7, dimension 8b + i in bits 4i .. 4i+3, and with g = b / 8,
+ * r = b % 8 block b is word
+ *     keys:   (r % 4) * (head_dim / 32) + 2 * g + r / 4
+ *     values: r * (head_dim / 64) + g
+ * of its row (the orders in which the attention kernel's lanes read them).
+ * head_dim is 64 or 128; max_seq a multiple of 64.  Arrays are
+ * [n_seq, kv_heads, max_seq, head_dim/2] bytes and
+ * [n_seq, kv_heads, max_seq, head_dim/64, 2] bf16, 16-byte aligned. */
+typedef struct lbx_kv4_cache {
+  uint8_t *k_codes; uint16_t *k_params;
+  uint8_t *v_codes; uint16_t *v_params;
+  int32_t n_seq, kv_heads, max_seq, head_dim;
+} lbx_kv4_cache;
+
+/* Rotates (keys), quantises and stores n new tokens of every sequence at slots
+ * start[s] .. start[s] + n - 1.  k_new / v_new: [n_seq * n, kv_heads *
+ * head_dim], rows kv_ld elements apart.  A key is rotated by rope_cs (the
+ * (cos, sin) pairs of lbx_rope_table, one row for each token; NULL: not
+ * rotated) with each product and the difference rounded to fp32.  Per group:
+ * step = bf16((hi - lo) * (1/15)) (0 below the least normal float), least =
+ * bf16(lo), code = clamp(rint((y - least) * (1 / step)), 0, 15), fp32
+ * operations rounded one by one, ties to even.  A group holding a NaN or an
+ * infinity stores NaN for both (its values read as NaN).  start: device
+ * int32 [n_seq], or NULL: max_start for every sequence; max_start bounds them
+ * on the host.  A start outside [0, max_start] writes nothing and records
+ * device error 0x801. */
+typedef struct lbx_kv4_append_args {
+  lbx_kv4_cache cache;
+  int32_t n, max_start, dtype, use_pdl;
+  const int32_t *start;
+  const void *k_new; const void *v_new; int64_t kv_ld;
+  const float *rope_cs;
+} lbx_kv4_append_args;
+int lbx_kv4_append(const lbx_kv4_append_args *a /* host */, cudaStream_t stream);
+
+/* The values of slots start[s] .. start[s] + n - 1 of every sequence, fp32
+ * [n_seq, kv_heads, n, head_dim] each (k or v may be NULL).  A start outside
+ * [0, max_start] reads nothing, gives NaN and records device error 0x802. */
+int lbx_kv4_read(const lbx_kv4_cache *c /* host */, const int32_t *start, int32_t max_start, int32_t n,
+                 float *k, float *v, cudaStream_t stream);
+
+/* Attention of n new tokens of every sequence over its 4-bit cache, the new
+ * tokens' keys and values already stored at slots prefix[s] ..
+ * prefix[s] + n - 1.  q [n_seq * n, heads * head_dim] (rows q_ld elements
+ * apart) is rotated by rope_cs (NULL: not); query i of a sequence sees slots
+ * [0, prefix[s]) and the new slots prefix[s] + j with bit j of its tree mask
+ * set, or j <= i without one.  A query that sees nothing gives zeros.  Stale
+ * slots are never used, whatever they hold.  Query head h reads kv head
+ * h / (heads / kv_heads).  n <= 64 with a tree mask, any n without.  out
+ * [n_seq * n, heads * head_dim] has q's type.  A query's bits depend neither on
+ * the other queries and sequences of the call nor on max_prefix, so a causal
+ * run in one call equals its tokens one at a time.  A prefix outside
+ * [0, max_prefix] gives NaN rows and records device error 0x803. */
+typedef struct lbx_kv4_attn_args {
+  lbx_kv4_cache cache;
+  int32_t n, heads, max_prefix, dtype, use_pdl;
+  float scale;
+  const int32_t *prefix;     /* device int32 [n_seq], or NULL: max_prefix */
+  const void *q; int64_t q_ld;
+  const float *rope_cs;      /* [n_seq * n][head_dim/2] (cos, sin), or NULL */
+  const uint64_t *tree_mask; /* [n_seq * n] or NULL */
+  void *out;
+} lbx_kv4_attn_args;
+/* Workspace: zero-filled once at allocation (it holds self-resetting tickets). */
+size_t lbx_kv4_attn_workspace_size(const lbx_kv4_attn_args *a /* host */);
+int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
+
+/* ---- verification of sampled drafts --------------------------------------
+ * The sampling acceptance of speculative_decoding.py:331-363 from given random
+ * numbers.  For every sequence: p_i = softmax(target_i / T), q_i =
+ * softmax(draft_i / T); draft i is accepted while u_i < min(1, p_i(d_i) /
+ * max(q_i(d_i), 1e-10)); with a accepted drafts the next token is
+ * argmax_v r_v / e_v (the lowest index of equal ones), r = max(p_a - q_a, 0) after
+ * a rejection (p_a where that is all zero) and p_k after none.  With e
+ * exponentially distributed that is a draw from r.  k = 0 draws a token from
+ * target_0: the sampler of the drafts themselves.  draft == NULL: the drafts
+ * were not sampled (greedy or looked up), q_i is 1 at d_i.  T = 0: p and q are 1
+ * at their first maximum.  A logit of -inf or NaN has probability 0; +inf
+ * counts as the maximum, shared equally.  A row without any probability
+ * rejects its draft, and gives the next token -1.  A draft outside the
+ * vocabulary is rejected (device error 0x811), q_i then taken as it is.
+ * n_draft[s] outside [0, k] is clamped (device error 0x812). */
+typedef struct lbx_accept_args {
+  int32_t n_seq, k, vocab, dtype;      /* dtype: of both logits; k <= LBX_ACCEPT_MAX_K */
+  int32_t use_pdl;
+  float temperature;                   /* >= 0; of every sequence when temps == NULL */
+  const float *temps;                  /* device [n_seq] or NULL */
+  const int64_t *tokens; int64_t tokens_ld;             /* [n_seq, k] */
+  const int32_t *n_draft;                               /* device [n_seq] or NULL: k */
+  const void *target; int64_t target_seq, target_row;   /* [n_seq, k+1, vocab] strides in elements */
+  const void *draft; int64_t draft_seq, draft_row;      /* [n_seq, k, vocab] */
+  const float *u; int64_t u_ld;                         /* [n_seq, k] in [0, 1) */
+  const float *e; int64_t e_ld;                         /* [n_seq, vocab], > 0 */
+  int64_t *accepted;                                    /* [n_seq] */
+  int64_t *next;                                        /* [n_seq] */
+} lbx_accept_args;
+#define LBX_ACCEPT_MAX_K 64
+int lbx_accept_sampled(const lbx_accept_args *a /* host */, cudaStream_t stream);
+
 /* ---- diagnostics --------------------------------------------------------- */
 /* Launch floor of a linear call, for benchmarks (no reference counterpart):
  * the call's two stage grids with the same launch shapes, shared memory and

@@ -20,6 +20,7 @@ LBX_EPI_STORE, LBX_EPI_ADD, LBX_EPI_SILU0 = 0, 1, 2
 LBX_EXEC_AUTO, LBX_EXEC_KERNELS, LBX_EXEC_PROGRAM, LBX_EXEC_CLUSTER = 0, 1, 2, 3
 LBX_EXEC_KERNELS_ONE_CTA_V = 4
 LBX_EXEC_TC, LBX_EXEC_NO_TC = 5, 6
+LBX_ACCEPT_MAX_K = 64
 
 
 class Branch(ctypes.Structure):
@@ -80,6 +81,47 @@ class Model(ctypes.Structure):
     ]
 
 
+class Int8Args(ctypes.Structure):
+    _fields_ = [
+        ("m", c_int32), ("n", c_int32), ("k", c_int32), ("x_dtype", c_int32), ("y_dtype", c_int32),
+        ("use_pdl", c_int32), ("x", c_void_p), ("x_ld", c_int64), ("w", c_void_p), ("w_ld", c_int64),
+        ("w_scale", c_void_p), ("bias", c_void_p), ("y", c_void_p), ("y_ld", c_int64),
+    ]
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", c_void_p), ("k_params", c_void_p), ("v_codes", c_void_p), ("v_params", c_void_p),
+        ("n_seq", c_int32), ("kv_heads", c_int32), ("max_seq", c_int32), ("head_dim", c_int32),
+    ]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv4Cache), ("n", c_int32), ("max_start", c_int32), ("dtype", c_int32), ("use_pdl", c_int32),
+        ("start", c_void_p), ("k_new", c_void_p), ("v_new", c_void_p), ("kv_ld", c_int64),
+        ("rope_cs", c_void_p),
+    ]
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv4Cache), ("n", c_int32), ("heads", c_int32), ("max_prefix", c_int32), ("dtype", c_int32),
+        ("use_pdl", c_int32), ("scale", c_float), ("prefix", c_void_p), ("q", c_void_p), ("q_ld", c_int64),
+        ("rope_cs", c_void_p), ("tree_mask", c_void_p), ("out", c_void_p),
+    ]
+
+
+class AcceptArgs(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", c_int32), ("k", c_int32), ("vocab", c_int32), ("dtype", c_int32), ("use_pdl", c_int32),
+        ("temperature", c_float), ("temps", c_void_p), ("tokens", c_void_p), ("tokens_ld", c_int64),
+        ("n_draft", c_void_p), ("target", c_void_p), ("target_seq", c_int64), ("target_row", c_int64),
+        ("draft", c_void_p), ("draft_seq", c_int64), ("draft_row", c_int64), ("u", c_void_p), ("u_ld", c_int64),
+        ("e", c_void_p), ("e_ld", c_int64), ("accepted", c_void_p), ("next", c_void_p),
+    ]
+
+
 _SIGNATURES = {
     "lbx_linear_workspace_size": (c_size_t, [POINTER(Proj), c_int32, c_int32]),
     "lbx_linear": (c_int, [POINTER(Proj), POINTER(LinearArgs), c_void_p, c_size_t, c_void_p]),
@@ -125,6 +167,15 @@ _SIGNATURES = {
                                   c_void_p]),
     "lbx_kv_move": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                             c_void_p, c_int32, c_void_p]),
+    "lbx_quant_tokens": (c_int, [c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                 c_void_p]),
+    "lbx_linear_int8_workspace_size": (c_size_t, [c_int32, c_int32, c_int32]),
+    "lbx_linear_int8": (c_int, [POINTER(Int8Args), c_void_p, c_size_t, c_void_p]),
+    "lbx_kv4_append": (c_int, [POINTER(Kv4AppendArgs), c_void_p]),
+    "lbx_kv4_read": (c_int, [POINTER(Kv4Cache), c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "lbx_kv4_attn_workspace_size": (c_size_t, [POINTER(Kv4AttnArgs)]),
+    "lbx_kv4_attn": (c_int, [POINTER(Kv4AttnArgs), c_void_p, c_size_t, c_void_p]),
+    "lbx_accept_sampled": (c_int, [POINTER(AcceptArgs), c_void_p]),
     "lbx_last_error": (c_int, [c_char_p, c_size_t]),
     "lbx_device_error": (c_int, [POINTER(c_int32), c_void_p]),
     "lbx_clear_device_error": (c_int, [c_void_p]),

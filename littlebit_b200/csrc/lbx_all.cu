@@ -11,5 +11,8 @@
 #include "misc.cu"
 #include "attention.cu"
 #include "lmhead.cu"
+#include "int8.cu"
+#include "kv4.cu"
+#include "sample.cu"
 #include "program.cu"
 #include "forward.cu"

@@ -536,3 +536,336 @@ def accept_greedy_tree(cand: torch.Tensor, node_argmax: torch.Tensor,
     L.check(lib().lbx_accept_greedy_tree(_p(cand), _p(node_argmax), _p(retrieve), L_, D1, _p(out),
                                          _stream(out.device)), "accept_greedy_tree")
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integer product (scales for each token and each channel)
+# ---------------------------------------------------------------------------
+def _rows(name: str, t: torch.Tensor, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tensor:
+    """A 2-D CUDA tensor whose rows are contiguous (any row stride that does not overlap)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (the B200 library has no CPU path)")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} has type {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise RuntimeError(f"{name} must be 2-D with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+class _on:
+    """Makes a tensor's device current for a call where it is not."""
+    __slots__ = ("dev", "prev")
+
+    def __init__(self, dev: torch.device):
+        self.dev, self.prev = dev.index, None
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.dev:
+            self.prev = cur
+            torch.cuda.set_device(self.dev)
+        return ctypes.c_void_p(torch.cuda.current_stream(self.dev).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
+
+
+def _stream_ws(device: torch.device, tag: str, stream: ctypes.c_void_p, nbytes: int) -> torch.Tensor:
+    """Scratch of one operator on one stream (calls on different streams never share it)."""
+    return workspace(device, f"{tag}/{stream.value or 0}").get(nbytes)
+
+
+def _vec(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    _cuda(name, t)
+    if t.dtype != dtype or t.numel() != n or t.device != device:
+        raise RuntimeError(f"{name} must hold {n} {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t
+
+
+def quantize_tokens(x: torch.Tensor):
+    """x [m, k] (float32 or bfloat16) -> (codes int8 [m, k], scale float32 [m]): each
+    row in 8 bits by its absolute maximum.  Rows of the codes start on 16 bytes,
+    as :func:`linear_int8` wants its weights: ``quantize_tokens(weight)`` quantises a
+    weight matrix by output channel."""
+    _rows("x", x)
+    m, k = x.shape
+    ld = -(-k // 16) * 16
+    q = torch.empty(m, ld, dtype=torch.int8, device=x.device)[:, :k]
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    with _on(x.device) as st:
+        L.check(lib().lbx_quant_tokens(_p(x), _dt(x), _ld(x), m, k, _p(q), ld, _p(scale), st), "quantize_tokens")
+    return q, scale
+
+
+def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y[t, n] = s_t * weight_scale[n] * sum_k c_tk * weight[n, k] (+ bias[n]).
+
+    x [m, k] float32 or bfloat16 is quantised by token in the call (c, s of
+    :func:`quantize_tokens`); weight int8 [n, k] has rows on 16 bytes.  The sums
+    are exact integers, so a token's result does not depend on the others.
+    Result type: ``out_dtype``, else x's."""
+    _rows("x", x)
+    _rows("weight", weight, (torch.int8,))
+    (m, k), n = x.shape, weight.shape[0]
+    if weight.shape[1] != k:
+        raise RuntimeError(f"x has {k} features, weight {weight.shape[1]}")
+    dev = x.device
+    if weight.device != dev:
+        raise RuntimeError("x and weight must be on one device")
+    _vec("weight_scale", weight_scale, n, torch.float32, dev)
+    if bias is not None:
+        _vec("bias", bias, n, torch.float32, dev)
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=dev)
+    else:
+        _rows("out", out)
+        if tuple(out.shape) != (m, n) or out.device != dev or (out_dtype is not None and out.dtype != out_dtype):
+            raise RuntimeError(f"out must be [{m}, {n}] on {dev}")
+    a = L.Int8Args(m, n, k, _dt(x), _dt(out), 0, x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight),
+                   weight_scale.data_ptr(), _p(bias), out.data_ptr(), _ld(out))
+    with _on(dev) as st:
+        ws = _stream_ws(dev, "int8", st, int(lib().lbx_linear_int8_workspace_size(m, n, k)))
+        L.check(lib().lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
+    return out
+
+
+class Int8Linear:
+    """A dense layer (an lm_head, say) kept as 8-bit integers with a scale for each
+    output channel: half the bytes of bf16 for every token that reads it."""
+
+    def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        self.weight, self.weight_scale, self.bias = weight, weight_scale, bias
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Linear":
+        """Quantise weight [out, in] (float32 or bfloat16) by output channel."""
+        q, s = quantize_tokens(weight)
+        return cls(q, s, None if bias is None else bias.to(torch.float32).contiguous())
+
+    @property
+    def out_features(self) -> int:
+        return self.weight.shape[0]
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return linear_int8(x, self.weight, self.weight_scale, self.bias, out, out_dtype)
+
+
+# ---------------------------------------------------------------------------
+# KV cache held in 4 bits
+# ---------------------------------------------------------------------------
+KV4_GROUP = 64
+
+
+@dataclass(frozen=True)
+class Kv4Cache:
+    """Keys and values of S sequences in 4 bits: codes uint8 [S, kv_heads, max_seq,
+    head_dim / 2] and, for each group of 64 dimensions, (step, least) bfloat16
+    [S, kv_heads, max_seq, head_dim / 64, 2]; a value is least + step * code.
+    The order of the codes is that of include/lbx.h; :func:`kv4_read` gives the
+    values back."""
+    k_codes: torch.Tensor
+    k_params: torch.Tensor
+    v_codes: torch.Tensor
+    v_params: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_seq: int, kv_heads: int, max_seq: int, head_dim: int, device="cuda") -> "Kv4Cache":
+        """max_seq is rounded up to a multiple of 64."""
+        if head_dim not in (64, 128):
+            raise RuntimeError("head_dim must be 64 or 128")
+        shp = (n_seq, kv_heads, -(-max_seq // 64) * 64)
+        c = [torch.zeros(*shp, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2)]
+        p = [torch.zeros(*shp, head_dim // KV4_GROUP, 2, dtype=torch.bfloat16, device=device) for _ in range(2)]
+        return cls(c[0], p[0], c[1], p[1])
+
+    @property
+    def shape(self):
+        """(n_seq, kv_heads, max_seq, head_dim)"""
+        s = self.k_codes.shape
+        return s[0], s[1], s[2], 2 * s[3]
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_params, self.v_codes, self.v_params))
+
+    def __post_init__(self):
+        kc, kp, vc, vp = self.k_codes, self.k_params, self.v_codes, self.v_params
+        for nm, t, ty in (("k_codes", kc, torch.uint8), ("v_codes", vc, torch.uint8),
+                          ("k_params", kp, torch.bfloat16), ("v_params", vp, torch.bfloat16)):
+            _cuda(nm, t)
+            if t.dtype != ty:
+                raise RuntimeError(f"{nm} must be {ty}")
+            if t.device != kc.device:
+                raise RuntimeError("cache tensors must be on one device")
+        if kc.dim() != 4 or kp.dim() != 5:
+            raise RuntimeError("codes must be 4-D and params 5-D")
+        S, H, T, D2 = kc.shape
+        if vc.shape != kc.shape or vp.shape != kp.shape or tuple(kp.shape) != (S, H, T, 2 * D2 // KV4_GROUP, 2):
+            raise RuntimeError(f"cache shapes do not fit together: {tuple(kc.shape)} {tuple(kp.shape)} "
+                               f"{tuple(vc.shape)} {tuple(vp.shape)}")
+        object.__setattr__(self, "_struct", L.Kv4Cache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(),
+                                                       S, H, T, 2 * D2))
+
+    def struct(self) -> L.Kv4Cache:
+        """The C descriptor (the tensors of a cache are fixed)."""
+        return self._struct
+
+
+def _rope_arg(rope_cs: Optional[torch.Tensor], rows: int, d: int, device) -> Optional[int]:
+    if rope_cs is None:
+        return None
+    return _vec("rope_cs", rope_cs, rows * d, torch.float32, device).data_ptr()
+
+
+def _start_arg(name: str, start, n_seq: int, bound: int, device):
+    """(device pointer or None, host bound) of per-sequence slot counts: an int for all,
+    or a device int32 [n_seq] with its host-side upper bound."""
+    if isinstance(start, torch.Tensor):
+        return _vec(name, start, n_seq, torch.int32, device).data_ptr(), int(bound)
+    return None, int(start)
+
+
+def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start, max_start: Optional[int] = None,
+               rope_cs: Optional[torch.Tensor] = None) -> None:
+    """Rotate (keys, by ``rope_cs`` of :func:`rope_table`), quantise and store n new
+    tokens of every sequence of the cache.
+
+    k_new / v_new [S * n, kv_heads * head_dim], float32 or bfloat16, sequence by
+    sequence.  ``start``: first slot, an int for every sequence, or a device int32
+    [S] bounded by ``max_start``."""
+    c = cache.struct()
+    _rows("k_new", k_new)
+    _rows("v_new", v_new, (k_new.dtype,))
+    dev = cache.k_codes.device
+    if v_new.shape != k_new.shape or k_new.shape[1] != c.kv_heads * c.head_dim or k_new.shape[0] % c.n_seq:
+        raise RuntimeError(f"k_new / v_new must be [{c.n_seq} * n, {c.kv_heads * c.head_dim}], got "
+                           f"{tuple(k_new.shape)} and {tuple(v_new.shape)}")
+    if k_new.device != dev or v_new.device != dev:
+        raise RuntimeError("k_new, v_new and the cache must be on one device")
+    if k_new.shape[0] > 1 and v_new.stride(0) != k_new.stride(0):
+        raise RuntimeError("k_new and v_new must have one row stride")
+    sp, bound = _start_arg("start", start, c.n_seq, max_start if max_start is not None else c.max_seq, dev)
+    a = L.Kv4AppendArgs(c, k_new.shape[0] // c.n_seq, bound, _dt(k_new), 0, sp, k_new.data_ptr(), v_new.data_ptr(),
+                        _ld(k_new), _rope_arg(rope_cs, k_new.shape[0], c.head_dim, dev))
+    with _on(dev) as st:
+        L.check(lib().lbx_kv4_append(ctypes.byref(a), st), "kv4_append")
+
+
+def kv4_read(cache: Kv4Cache, start, max_start: Optional[int], n: int):
+    """The values of n slots of every sequence: (k, v) float32 [S, kv_heads, n, head_dim]."""
+    c = cache.struct()
+    dev = cache.k_codes.device
+    sp, bound = _start_arg("start", start, c.n_seq, max_start if max_start is not None else c.max_seq, dev)
+    k = torch.empty(c.n_seq, c.kv_heads, n, c.head_dim, dtype=torch.float32, device=dev)
+    v = torch.empty_like(k)
+    with _on(dev) as st:
+        L.check(lib().lbx_kv4_read(ctypes.byref(c), sp, bound, n, k.data_ptr(), v.data_ptr(), st), "kv4_read")
+    return k, v
+
+
+def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional[int], heads: int, scale: float,
+                  rope_cs: Optional[torch.Tensor] = None, tree_mask: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of n new tokens of every sequence over its 4-bit cache, which
+    already holds them (:func:`kv4_append`).
+
+    q [S * n, heads * head_dim], float32 or bfloat16, is rotated by ``rope_cs``.
+    ``prefix``: cached slots before the new tokens, an int, or a device int32 [S]
+    bounded by ``max_prefix``.  A query sees its sequence's cached slots and the
+    new ones up to itself, or those of its ``tree_mask`` bits (int64 [S * n], n <= 64).
+    A query that sees nothing gives zeros.  Result: q's shape and type."""
+    c = cache.struct()
+    _rows("q", q)
+    dev = cache.k_codes.device
+    if q.device != dev:
+        raise RuntimeError("q and the cache must be on one device")
+    if q.shape[0] == 0 or q.shape[0] % c.n_seq or q.shape[1] != heads * c.head_dim:
+        raise RuntimeError(f"q must be [{c.n_seq} * n, {heads * c.head_dim}], got {tuple(q.shape)}")
+    pp, bound = _start_arg("prefix", prefix, c.n_seq, max_prefix if max_prefix is not None else c.max_seq, dev)
+    tm = None
+    if tree_mask is not None:
+        tm = _vec("tree_mask", tree_mask, q.shape[0], torch.int64, dev).data_ptr()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _cuda("out", out)
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            raise RuntimeError(f"out must have q's shape, type and device")
+    a = L.Kv4AttnArgs(c, q.shape[0] // c.n_seq, heads, bound, _dt(q), 0, float(scale), pp, q.data_ptr(), _ld(q),
+                      _rope_arg(rope_cs, q.shape[0], c.head_dim, dev), tm, out.data_ptr())
+    with _on(dev) as st:
+        ws = _stream_ws(dev, "kv4", st, max(1, int(lib().lbx_kv4_attn_workspace_size(ctypes.byref(a)))))
+        L.check(lib().lbx_kv4_attn(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "attention_kv4")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# verification of sampled drafts
+# ---------------------------------------------------------------------------
+def accept_sampled(tokens: Optional[torch.Tensor], target_logits: torch.Tensor, draft_logits: Optional[torch.Tensor],
+                   u: Optional[torch.Tensor], e: torch.Tensor, temperature=1.0,
+                   n_draft: Optional[torch.Tensor] = None):
+    """Verify k sampled drafts of each of S sequences (speculative_decoding.py:331-363)
+    from given random numbers -> (accepted int64 [S], next token int64 [S]).
+
+    tokens int64 [S, k]; target_logits [S, k + 1, V] and draft_logits [S, k, V],
+    float32 or bfloat16 (draft_logits None: the drafts were not sampled); u float32
+    [S, k] uniform in [0, 1); e float32 [S, V] exponentially distributed (> 0);
+    temperature a number or a device float32 [S]; n_draft int32 [S]: sequences
+    with fewer drafts.  With k = 0 (tokens, draft_logits and u None or empty) it
+    draws next from softmax(target_logits[:, 0] / temperature)."""
+    t = target_logits
+    if t.dim() != 3 or not t.is_cuda:
+        raise RuntimeError("target_logits must be a CUDA tensor [S, k + 1, V]")
+    S, k1, V = t.shape
+    k, dev, dt = k1 - 1, t.device, _dt(t)
+    if k < 0 or V < 1:
+        raise RuntimeError("target_logits must be [S, k + 1, V] with V >= 1")
+
+    def plane(name, x, shape, dtype):
+        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.device != dev:
+            raise RuntimeError(f"{name} must be a tensor on {dev}")
+        if tuple(x.shape) != shape or x.dtype != dtype:
+            raise RuntimeError(f"{name} must be {shape} {dtype}, got {tuple(x.shape)} {x.dtype}")
+        if x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise RuntimeError(f"{name} must be contiguous along its last dimension")
+        return x
+
+    plane("target_logits", t, (S, k1, V), t.dtype)
+    plane("e", e, (S, V), torch.float32)
+    if k:
+        plane("tokens", tokens, (S, k), torch.int64)
+        plane("u", u, (S, k), torch.float32)
+        if draft_logits is not None:
+            plane("draft_logits", draft_logits, (S, k, V), t.dtype)
+    d = draft_logits if k else None
+    a = L.AcceptArgs()
+    a.n_seq, a.k, a.vocab, a.dtype = S, k, V, dt
+    if isinstance(temperature, torch.Tensor):
+        a.temps = _vec("temperature", temperature, S, torch.float32, dev).data_ptr()
+    else:
+        a.temperature = float(temperature)
+    if k:
+        a.tokens, a.tokens_ld = tokens.data_ptr(), tokens.stride(0)
+        a.u, a.u_ld = u.data_ptr(), u.stride(0)
+        if n_draft is not None:
+            a.n_draft = _vec("n_draft", n_draft, S, torch.int32, dev).data_ptr()
+    a.target, a.target_seq, a.target_row = t.data_ptr(), t.stride(0), t.stride(1)
+    if d is not None:
+        a.draft, a.draft_seq, a.draft_row = d.data_ptr(), d.stride(0), d.stride(1)
+    a.e, a.e_ld = e.data_ptr(), e.stride(0)
+    res = torch.empty(2, S, dtype=torch.int64, device=dev)
+    a.accepted = res.data_ptr()
+    a.next = res.data_ptr() + 8 * S
+    with _on(dev) as st:
+        L.check(lib().lbx_accept_sampled(ctypes.byref(a), st), "accept_sampled")
+    return res[0], res[1]

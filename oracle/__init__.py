@@ -16,4 +16,6 @@ Modules:
   littlebit — rank sizing, _compute_forward, runtime converter (littlebit.py, convert_hf_to_runtime.py)
   decoder   — LittleBit Llama decoder with KV cache, RoPE, tree masks (HF Llama + cpp:1522-2079)
   spec      — greedy speculative loop, tree buffers, posterior  (speculative_decoding.py, tree_utils.py)
+  lowbit    — 8-bit product, 4-bit KV cache and its attention, sampled verification (no reference counterpart, but
+              for the sampling acceptance of speculative_decoding.py:331-363)
 """
