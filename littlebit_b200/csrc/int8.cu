@@ -5,7 +5,10 @@
 //
 // The sums are exact int32 (127 * 128 * 131072 < 2^31), so every split of the
 // work gives the same bits.
-#include "common.cuh"
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "tcgen05.cuh"
 
 namespace lbx {
 
@@ -19,6 +22,8 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
   __shared__ uint32_t red[Q8_THREADS / 32];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();  // (a kernel that starts early may count on all that came before this one)
   // |x| as an integer: the order of the non-negative floats, infinities and
   // NaNs (0x7f800000 and up) above every number
   uint32_t m = 0;
@@ -41,68 +46,347 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
   }
 }
 
-// 64 tokens x 64 channels a CTA, four products at a time (dp4a)
-constexpr int I8_T = 64;
-__global__ void __launch_bounds__(256) linear_int8_kernel(const int8_t *__restrict__ q, int64_t q_ld,
-                                                          const float *__restrict__ s, const int8_t *__restrict__ w,
-                                                          int64_t w_ld, const float *__restrict__ ws,
-                                                          const float *__restrict__ bias, int m, int n, int k,
-                                                          void *__restrict__ y, int64_t y_ld, int ydt) {
-  __shared__ int sx[16][I8_T + 1], sw[16][I8_T + 1];
-  const int n0 = blockIdx.x * I8_T, m0 = blockIdx.y * I8_T;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < k; k0 += 64) {
-    for (int e = tid; e < 16 * I8_T; e += 256) {
-      const int c = e & 15, r = e >> 4, kk = k0 + 4 * c;
-      int a = 0, b = 0;
-      for (int i = 0; i < 4; ++i) {
-        if (kk + i >= k) break;
-        if (m0 + r < m) a |= (int)(uint8_t)q[(int64_t)(m0 + r) * q_ld + kk + i] << (8 * i);
-        if (n0 + r < n) b |= (int)(uint8_t)w[(int64_t)(n0 + r) * w_ld + kk + i] << (8 * i);
-      }
-      sx[c][r] = a;
-      sw[c][r] = b;
+// ---------------------------------------------------------------------------
+// Product on the tensor cores (tcgen05.mma kind::i8, int32 sums in TMEM).
+//
+// A CTA's tile is 128 channels (operand A: the weights) x BN tokens (operand
+// B, BN = 16, or a multiple of 32 up to 256), K in blocks of 128 bytes that TMA
+// lands in 128-byte swizzle; out-of-range rows and bytes arrive as zeros, so odd
+// sizes need no other care.  A lane of the accumulator is a channel, a column a
+// token: each column's store is 128 consecutive results.
+//
+// Tiles are dealt to one persistent CTA an SM: whole rounds of tiles first
+// ("full"), and what does not fill a round (everything, for few tiles) is cut
+// into equal runs of K blocks over the CTAs ("rest"), so that a single token's
+// 250 tiles keep all SMs streaming.  A tile that is cut leaves its parts as
+// int32 in the workspace and the CTA that completes it adds them: the
+// sums are exact, so neither the cut nor the order shows in the result.
+// ---------------------------------------------------------------------------
+constexpr int I8_THREADS = 192;   // warp 0: copies, warp 1: MMA, warps 2-5: results
+constexpr int I8_KB = 128;        // K bytes a block
+constexpr int I8_MAXST = 12;      // stages at most
+constexpr int I8_MAXCTA = 1024;   // ticket words
+constexpr int I8_MINBLK = 4;      // K blocks a CTA takes of the rest, at least
+
+struct I8Params {
+  int m, n, KB;
+  int TN, TM, BN;      // channel tiles, token tiles, tokens a tile
+  int full, T;         // tiles of whole rounds, all tiles
+  int G, Gr;           // CTAs, CTAs that share the rest
+  int64_t rb;          // K blocks of the rest
+  int ST;              // stages
+  uint32_t idesc, tcols;
+  const float *s, *ws, *bias;
+  void *y; int64_t y_ld; int ydt;
+  int32_t *part;       // [CTA][2][BN][128] parts of cut tiles
+  unsigned *ticket;    // [T - full] K blocks arrived, zero between calls
+};
+
+// a CTA's pieces: its run of the rest, then its whole tiles
+struct I8Pieces {
+  int64_t r0, r1;
+  int t, G, full, KB;
+  LBX_DEV I8Pieces(const I8Params &p, int c) : r0(0), r1(0), t(c), G(p.G), full(p.full), KB(p.KB) {
+    if (c < p.Gr) {
+      r0 = p.rb * c / p.Gr;
+      r1 = p.rb * (c + 1) / p.Gr;
     }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sx[c][ty + 16 * i], sw[c][tx + 16 * j], acc[i][j]);
-    }
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int t = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
-      if (t >= m || c >= n) continue;
-      float v = __int2float_rn(acc[i][j]) * s[t] * ws[c];
-      if (bias) v += bias[c];
-      if (ydt == LBX_F32) reinterpret_cast<float *>(y)[(int64_t)t * y_ld + c] = v;
-      else reinterpret_cast<uint16_t *>(y)[(int64_t)t * y_ld + c] = f32_to_bf16(v);
+  LBX_DEV bool next(int &tile, int &k0, int &k1) {
+    if (r0 < r1) {
+      const int64_t q = r0 / KB;
+      tile = full + (int)q;
+      k0 = (int)(r0 - q * KB);
+      k1 = (int)min((int64_t)KB, k0 + (r1 - r0));
+      r0 += k1 - k0;
+      return true;
     }
+    if (t < full) {
+      tile = t;
+      k0 = 0;
+      k1 = KB;
+      t += G;
+      return true;
+    }
+    return false;
+  }
+};
+
+// tile -> (channel tile, token tile): groups of 16 token tiles, so that the
+// tiles of a round share few weight and few token rows (both stay in L2)
+constexpr int I8_GT = 16;
+LBX_DEV void i8_tile(const I8Params &p, int tile, int &tn, int &tm) {
+  const int g = tile / (p.TN * I8_GT), gs = min(I8_GT, p.TM - g * I8_GT), r = tile - g * p.TN * I8_GT;
+  tn = r / gs;
+  tm = g * I8_GT + (r - tn * gs);
 }
 
-struct Int8Ws {
-  size_t q, s, total;
+LBX_DEV void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+LBX_DEV void i8_store(const I8Params &p, int64_t t, int ch, int acc, float wsc, float b, bool has_b) {
+  float v = __int2float_rn(acc) * __ldcg(p.s + t) * wsc;
+  if (has_b) v += b;
+  if (p.ydt == LBX_F32) reinterpret_cast<float *>(p.y)[t * p.y_ld + ch] = v;
+  else reinterpret_cast<uint16_t *>(p.y)[t * p.y_ld + ch] = f32_to_bf16(v);
+}
+
+__global__ void __launch_bounds__(I8_THREADS, 1)
+    linear_int8_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                       const __grid_constant__ I8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *sm = align1024(smem_raw);
+  __shared__ __align__(8) uint64_t full[I8_MAXST], empty[I8_MAXST], tfull[2], tempty[2], drain;
+  __shared__ uint32_t tbase;
+  __shared__ int abort_flag, s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+  const int abytes = 128 * I8_KB, bbytes = p.BN * I8_KB, stage = abytes + bbytes;
+  volatile int *abrt = &abort_flag;
+  if (tid == 0) {
+    for (int i = 0; i < p.ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    abort_flag = 0;
+  }
+  if (warp == 1) tmem_alloc(&tbase, p.tcols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tbase, tbuf = p.tcols / 2;
+
+  if (warp == 0 && lane == 0) {
+    // ---- copies.  The weights do not come from the kernel before this one:
+    // the first stages' are on their way before its codes are waited for.
+    auto load_w = [&](int j, int tile, int kb) {
+      int tn, tm;
+      i8_tile(p, tile, tn, tm);
+      uint8_t *d = sm + (j % p.ST) * stage;
+      mbar_arrive_expect_tx(&full[j % p.ST], (uint32_t)stage);
+      tma_2d(d, &tw, kb * I8_KB, tn * 128, &full[j % p.ST]);
+    };
+    auto load_x = [&](int j, int tile, int kb) {
+      int tn, tm;
+      i8_tile(p, tile, tn, tm);
+      tma_2d(sm + (j % p.ST) * stage + abytes, &tx, kb * I8_KB, tm * p.BN, &full[j % p.ST]);
+    };
+    int tile, k0, k1, j = 0;
+    {
+      I8Pieces pre(p, cta);
+      while (j < p.ST && pre.next(tile, k0, k1))
+        for (int kb = k0; kb < k1 && j < p.ST; ++kb) load_w(j++, tile, kb);
+    }
+    const int npre = j;
+    pdl_wait();
+    I8Pieces it(p, cta);
+    j = 0;
+    bool ok = true;
+    while (ok && it.next(tile, k0, k1)) {
+      for (int kb = k0; kb < k1; ++kb, ++j) {
+        if (j >= npre) {
+          if (!wd_wait(&empty[j % p.ST], (uint32_t)(j / p.ST - 1) & 1u, 0x821, abrt)) {
+            ok = false;
+            break;
+          }
+          load_w(j, tile, kb);
+        }
+        load_x(j, tile, kb);
+      }
+    }
+    if (*abrt) {  // copies in flight land before shared memory is given up
+      int none = 0;
+      for (int i = max(0, j - p.ST); i < j; ++i) wd_wait(&full[i % p.ST], (uint32_t)(i / p.ST) & 1u, 0x822, &none);
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ---- MMA
+    I8Pieces it(p, cta);
+    int tile, k0, k1, j = 0, n = 0;
+    bool ok = true;
+    while (ok && it.next(tile, k0, k1)) {
+      const uint32_t d = tmem + (uint32_t)(n & 1) * tbuf;
+      if (n >= 2 && !wd_wait(&tempty[n & 1], (uint32_t)(n / 2 - 1) & 1u, 0x823, abrt)) break;
+      tc_fence_after();
+      for (int kb = k0; kb < k1; ++kb, ++j) {
+        if (!wd_wait(&full[j % p.ST], (uint32_t)(j / p.ST) & 1u, 0x824, abrt)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = smem_u32(sm + (j % p.ST) * stage), b = a + (uint32_t)abytes;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          umma_i8(d, sw128_desc(a + 32 * q), sw128_desc(b + 32 * q), p.idesc, kb > k0 || q > 0 ? 1u : 0u);
+        umma_commit(&empty[j % p.ST]);
+      }
+      if (ok) umma_commit(&tfull[n & 1]);
+      ++n;
+    }
+    if (*abrt) {  // products in flight end before TMEM is given up
+      int none = 0;
+      umma_commit(&drain);
+      wd_wait(&drain, 0, 0x825, &none);
+    }
+  } else if (warp >= 2) {
+    // ---- results: this warp's lane quarter is warp % 4
+    pdl_wait();
+    const int row = 32 * (warp & 3) + lane;
+    const uint32_t lq = (uint32_t)(32 * (warp & 3)) << 16;
+    I8Pieces it(p, cta);
+    int tile, k0, k1, n = 0;
+    while (it.next(tile, k0, k1)) {
+      // (after a wait that gave up all four warps still go through the same
+      // barriers: the pieces left then pass at once, and the call has failed)
+      wd_wait(&tfull[n & 1], (uint32_t)(n / 2) & 1u, 0x826, abrt);
+      __syncwarp();
+      tc_fence_after();
+      int tn, tm;
+      i8_tile(p, tile, tn, tm);
+      const int ch = tn * 128 + row, t0 = tm * p.BN, nc = min(p.BN, p.m - t0);
+      const bool cok = ch < p.n, whole = k0 == 0 && k1 == p.KB, hb = p.bias != nullptr;
+      const float wsc = cok ? p.ws[ch] : 0.f, bs = cok && hb ? p.bias[ch] : 0.f;
+      int32_t *slot = p.part + ((int64_t)cta * 2 + (k0 > 0 ? 0 : 1)) * 128 * p.BN;
+      const uint32_t ta = tmem + (uint32_t)(n & 1) * tbuf + lq;
+      for (int c0 = 0; c0 < nc; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld<16>(ta + c0, r);
+        tmem_ld_wait();
+        if (whole) {
+          if (cok) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c0 + j < nc) i8_store(p, t0 + c0 + j, ch, (int)r[j], wsc, bs, hb);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < nc) __stcg(slot + (c0 + j) * 128 + row, (int)r[j]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&tempty[n & 1]);
+      ++n;
+      if (whole) continue;
+      // the part is out; the CTA whose part completes the tile adds them all
+      __threadfence();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (tid == 64) {
+        const unsigned old = atomicAdd(p.ticket + (tile - p.full), (unsigned)(k1 - k0));
+        s_last = old + (unsigned)(k1 - k0) == (unsigned)p.KB;
+        if (s_last) p.ticket[tile - p.full] = 0u;  // ready for the next call
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (!s_last) continue;
+      __threadfence();
+      const int64_t base = (int64_t)(tile - p.full) * p.KB;
+      int cl = (int)(base * p.Gr / p.rb);  // the first CTA with K blocks of this tile
+      while (cl > 0 && p.rb * cl / p.Gr > base) --cl;
+      while (p.rb * (cl + 1) / p.Gr <= base) ++cl;
+      for (int c0 = 0; c0 < nc; c0 += 16) {
+        int acc[16] = {};
+        for (int c = cl; c < p.Gr; ++c) {
+          const int64_t b0 = p.rb * c / p.Gr;
+          if (b0 >= base + p.KB) break;
+          const int32_t *ps = p.part + ((int64_t)c * 2 + (b0 > base ? 0 : 1)) * 128 * p.BN;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < nc) acc[j] += __ldcg(ps + (c0 + j) * 128 + row);
+        }
+        if (cok) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < nc) i8_store(p, t0 + c0 + j, ch, acc[j], wsc, bs, hb);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, p.tcols);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// the split of a call, and its workspace: [tickets, at a fixed place][parts][scales][codes]
+struct I8Plan {
+  I8Params p;
+  size_t part, s, q, total;
   int64_t q_ld;
 };
-static Int8Ws int8_ws(int m, int k) {
+static I8Plan i8_plan(int m, int n, int k) {
   auto al = [](size_t v) { return (v + 255) & ~(size_t)255; };
-  Int8Ws w;
+  I8Plan w = {};
+  I8Params &p = w.p;
+  p.m = m;
+  p.n = n;
+  p.KB = (k + I8_KB - 1) / I8_KB;
+  p.TN = (n + 127) / 128;
+  p.TM = (m + 255) / 256;
+  const int per = (m + p.TM - 1) / p.TM;
+  p.BN = per <= 16 ? 16 : (per + 31) / 32 * 32;
+  p.idesc = idesc_i8(p.BN);
+  p.tcols = 32;
+  while (p.tcols < 2u * p.BN) p.tcols *= 2;
+  p.G = std::min(device_sm_count(), I8_MAXCTA);
+  p.T = p.TN * p.TM;
+  p.full = p.T / p.G * p.G;
+  p.rb = (int64_t)(p.T - p.full) * p.KB;
+  p.Gr = (int)std::min<int64_t>(p.G, std::max<int64_t>(1, p.rb / I8_MINBLK));
+  if (p.full == 0) p.G = p.Gr;
+  w.part = al((size_t)I8_MAXCTA * 4);
+  w.s = w.part + al((size_t)p.Gr * 2 * 128 * p.BN * 4);
+  w.q = w.s + al((size_t)m * 4);
   w.q_ld = (k + 15) & ~15;
-  w.s = 0;
-  w.q = al((size_t)m * 4);
   w.total = w.q + al((size_t)m * w.q_ld);
   return w;
 }
 
+// a [rows, k] int8 matrix in boxes of `box` rows x 128 bytes, 128-byte swizzle
+static int i8_map(CUtensorMap *map, const void *base, int64_t rows, int k, int64_t ld, int box) {
+  static DevCache<PFN_cuTensorMapEncodeTiled_v12000> fn;
+  PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+  const int rc = fn.get(enc, [](PFN_cuTensorMapEncodeTiled_v12000 &f) {
+    void *v = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &v, 12000, cudaEnableDefault, &st);
+    if (e != cudaSuccess) return cuda_status(e, "cuTensorMapEncodeTiled lookup");
+    if (!v) {
+      set_error("the driver has no cuTensorMapEncodeTiled");
+      return (int)LBX_EUNSUPPORTED;
+    }
+    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(v);
+    return (int)LBX_OK;
+  });
+  if (rc) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t bx[2] = {(cuuint32_t)I8_KB, (cuuint32_t)box}, es[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, bx, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LBX_ECUDA;
+  }
+  return LBX_OK;
+}
+
 static int quant_tokens_launch(const void *x, int xdt, int64_t x_ld, int m, int k, int8_t *q, int64_t q_ld,
-                               float *scale, cudaStream_t stream) {
-  quant_tokens_kernel<<<m, Q8_THREADS, 0, stream>>>(x, xdt, x_ld, k, q, q_ld, scale);
-  return cuda_status(cudaGetLastError(), "quant_tokens launch");
+                               float *scale, bool pdl, cudaStream_t stream) {
+  return cuda_status(launch(quant_tokens_kernel, dim3(m), dim3(Q8_THREADS), 0, stream, pdl, x, xdt, x_ld, k, q, q_ld, scale),
+                     "quant_tokens launch");
 }
 
 }  // namespace lbx
@@ -115,12 +399,12 @@ extern "C" int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, in
   LBX_CHECK_ARG(x_ld >= k && q_ld >= k, "row strides must be at least k");
   if (m == 0) return LBX_OK;
   LBX_CHECK_ARG(x && q && scale, "NULL pointer");
-  return quant_tokens_launch(x, x_dtype, x_ld, m, k, q, q_ld, scale, stream);
+  return quant_tokens_launch(x, x_dtype, x_ld, m, k, q, q_ld, scale, false, stream);
 }
 
 extern "C" size_t lbx_linear_int8_workspace_size(int32_t m, int32_t n, int32_t k) {
   if (m < 1 || n < 1 || k < 1) return 0;
-  return lbx::int8_ws(m, k).total;
+  return lbx::i8_plan(m, n, k).total;
 }
 
 extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
@@ -134,15 +418,37 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   LBX_CHECK_ARG(a->x && a->w && a->w_scale && a->y, "NULL pointer");
   LBX_CHECK_ARG(a->x_ld >= a->k && a->w_ld >= a->k && a->y_ld >= a->n, "row strides smaller than the rows");
   LBX_CHECK_ARG(aligned16(a->w) && a->w_ld % 16 == 0, "weight rows must start on 16 bytes");
-  const Int8Ws W = int8_ws(a->m, a->k);
+  I8Plan W = i8_plan(a->m, a->n, a->k);
   LBX_CHECK_ARG(ws && ws_bytes >= W.total, "workspace too small (%zu < %zu)", ws_bytes, W.total);
+  LBX_CHECK_ARG(aligned16(ws), "the workspace must be 16-byte aligned");
   uint8_t *b = reinterpret_cast<uint8_t *>(ws);
   int8_t *q = reinterpret_cast<int8_t *>(b + W.q);
   float *s = reinterpret_cast<float *>(b + W.s);
-  int rc = quant_tokens_launch(a->x, a->x_dtype, a->x_ld, a->m, a->k, q, W.q_ld, s, stream);
+  I8Params &p = W.p;
+  static DevCache<size_t> smax_cache;
+  size_t smax = 0;
+  int rc = smax_cache.get(smax, [](size_t &out) {
+    return cuda_status(allow_max_smem(linear_int8_kernel, &out), "linear_int8 smem attribute");
+  });
   if (rc) return rc;
-  const dim3 grid((a->n + I8_T - 1) / I8_T, (a->m + I8_T - 1) / I8_T);
-  linear_int8_kernel<<<grid, 256, 0, stream>>>(q, W.q_ld, s, a->w, a->w_ld, a->w_scale, a->bias, a->m, a->n, a->k,
-                                               a->y, a->y_ld, a->y_dtype);
-  return cuda_status(cudaGetLastError(), "linear_int8 launch");
+  const int stage = (128 + p.BN) * I8_KB;
+  p.ST = std::min(I8_MAXST, (int)((smax - 1024) / stage));
+  p.s = s;
+  p.ws = a->w_scale;
+  p.bias = a->bias;
+  p.y = a->y;
+  p.y_ld = a->y_ld;
+  p.ydt = a->y_dtype;
+  p.part = reinterpret_cast<int32_t *>(b + W.part);
+  p.ticket = reinterpret_cast<unsigned *>(b);
+  CUtensorMap tw, tx;
+  rc = i8_map(&tw, a->w, a->n, a->k, a->w_ld, 128);
+  if (rc) return rc;
+  rc = i8_map(&tx, q, a->m, a->k, W.q_ld, p.BN);
+  if (rc) return rc;
+  rc = quant_tokens_launch(a->x, a->x_dtype, a->x_ld, a->m, a->k, q, W.q_ld, s, a->use_pdl != 0, stream);
+  if (rc) return rc;
+  return cuda_status(launch(linear_int8_kernel, dim3(p.G), dim3(I8_THREADS), (size_t)p.ST * stage + 1024, stream, true, tw,
+                            tx, p),
+                     "linear_int8 launch");
 }
