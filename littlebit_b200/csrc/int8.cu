@@ -15,22 +15,67 @@ namespace lbx {
 constexpr int Q8_THREADS = 256;
 constexpr int Q8_MAXK = 131072;
 
-// one CTA per row: the absolute maximum, then the codes
-__global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__restrict__ x, int xdt, int64_t x_ld,
-                                                                  int k, int8_t *__restrict__ q, int64_t q_ld,
+// One CTA a row: the absolute maximum, then the codes.  VEC: 16-byte loads, up to
+// Q8_NR of them held in registers from the first pass to the second (rows of up
+// to 8192 float / 16384 bf16 values are read once; what is longer is read again,
+// from L2).  The kernel is one round trip to memory and two block barriers long:
+// 4096 values 5.9 us with scalar loads in two passes.
+constexpr int Q8_NR = 8;
+LBX_DEV uint32_t q8_abs(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+LBX_DEV uint32_t q8_code(float v, float inv, bool fin) {
+  return fin ? (uint32_t)(__float2int_rn(__fmul_rn(v, inv)) & 255) : 0u;
+}
+template <int XDT>
+LBX_DEV void q8_unpack(const uint4 &r, float *v) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (XDT == LBX_F32) {
+      v[i] = __uint_as_float(w[i]);
+    } else {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+template <int XDT, bool VEC>
+__global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__restrict__ x, int64_t x_ld, int k,
+                                                                  int8_t *__restrict__ q, int64_t q_ld,
                                                                   float *__restrict__ scale) {
+  constexpr int E = XDT == LBX_F32 ? 4 : 8, ES = 16 / E;
   __shared__ uint32_t red[Q8_THREADS / 32];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   pdl_wait();
   pdl_trigger();  // (a kernel that starts early may count on all that came before this one)
+  const uint8_t *xr = reinterpret_cast<const uint8_t *>(x) + row * x_ld * ES;
+  const uint4 *xv = reinterpret_cast<const uint4 *>(xr);
+  int8_t *qr = q + row * q_ld;
+  const int nv = VEC ? k / E : 0;
+  uint4 r[Q8_NR];
   // |x| as an integer: the order of the non-negative floats, infinities and
   // NaNs (0x7f800000 and up) above every number
   uint32_t m = 0;
-  for (int i = tid; i < k; i += Q8_THREADS) {
-    const uint32_t b = __float_as_uint(load_act(x, xdt, row * x_ld + i)) & 0x7FFFFFFFu;
-    m = max(m, b);
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < Q8_NR; ++i) {
+    const int e = tid + i * Q8_THREADS;
+    r[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (e < nv) r[i] = __ldg(xv + e);
   }
+#pragma unroll
+  for (int i = 0; i < Q8_NR; ++i) {
+    q8_unpack<XDT>(r[i], v);
+#pragma unroll
+    for (int j = 0; j < E; ++j) m = max(m, q8_abs(v[j]));
+  }
+  for (int e = tid + Q8_NR * Q8_THREADS; e < nv; e += Q8_THREADS) {
+    q8_unpack<XDT>(__ldg(xv + e), v);
+#pragma unroll
+    for (int j = 0; j < E; ++j) m = max(m, q8_abs(v[j]));
+  }
+  for (int i = nv * E + tid; i < k; i += Q8_THREADS) m = max(m, q8_abs(load_act(xr, XDT, i)));
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
   __syncthreads();
@@ -40,10 +85,21 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
   const float a = __uint_as_float(m);
   const float inv = fin && a > 0.f ? __fdiv_rn(127.0f, a) : 0.f;
   if (tid == 0) scale[row] = fin ? __fmul_rn(a, 1.0f / 127.0f) : __uint_as_float(0x7FC00000u);
-  for (int i = tid; i < k; i += Q8_THREADS) {
-    const float v = load_act(x, xdt, row * x_ld + i);
-    q[row * q_ld + i] = (int8_t)(fin ? __float2int_rn(__fmul_rn(v, inv)) : 0);
-  }
+  auto put = [&](int e, const uint4 &w) {
+    q8_unpack<XDT>(w, v);
+    uint32_t c[E / 4];
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j)
+      c[j] = q8_code(v[4 * j], inv, fin) | q8_code(v[4 * j + 1], inv, fin) << 8 | q8_code(v[4 * j + 2], inv, fin) << 16 |
+             q8_code(v[4 * j + 3], inv, fin) << 24;
+    if constexpr (E == 4) reinterpret_cast<uint32_t *>(qr)[e] = c[0];
+    else reinterpret_cast<uint2 *>(qr)[e] = make_uint2(c[0], c[1]);
+  };
+#pragma unroll
+  for (int i = 0; i < Q8_NR; ++i)
+    if (tid + i * Q8_THREADS < nv) put(tid + i * Q8_THREADS, r[i]);
+  for (int e = tid + Q8_NR * Q8_THREADS; e < nv; e += Q8_THREADS) put(e, __ldg(xv + e));
+  for (int i = nv * E + tid; i < k; i += Q8_THREADS) qr[i] = (int8_t)q8_code(load_act(xr, XDT, i), inv, fin);
 }
 
 // ---------------------------------------------------------------------------
@@ -55,12 +111,19 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
 // sizes need no other care.  A lane of the accumulator is a channel, a column a
 // token: each column's store is 128 consecutive results.
 //
-// Tiles are dealt to one persistent CTA an SM: whole rounds of tiles first
-// ("full"), and what does not fill a round (everything, for few tiles) is cut
-// into equal runs of K blocks over the CTAs ("rest"), so that a single token's
-// 250 tiles keep all SMs streaming.  A tile that is cut leaves its parts as
-// int32 in the workspace and the CTA that completes it adds them: the
-// sums are exact, so neither the cut nor the order shows in the result.
+// The work is dealt to one persistent CTA an SM in one of three ways, whichever
+// i8_plan() reckons the cheapest:
+//   rounds  whole tiles, round after round
+//   cut     whole rounds, and the tiles that do not fill a round cut into equal
+//           runs of K blocks over the CTAs.  A cut tile leaves its parts as int32
+//           in the workspace and the CTA that completes it adds them: the sums
+//           are exact, so neither the cut nor the order shows in the result.
+//   even    one token tile: the channels dealt evenly in units of 32, a CTA's
+//           share in tiles of up to 128 (rows past it are multiplied and not
+//           stored).  For few tokens, where the weights' stream is the time:
+//           32000 channels are 7 units for each of 148 CTAs, nothing is joined.  Joining
+//           cost 10 us there: under a saturated memory a fence, an atomic or a
+//           load takes as long as the queue of loads ahead of it.
 // ---------------------------------------------------------------------------
 constexpr int I8_THREADS = 192;   // warp 0: copies, warp 1: MMA, warps 2-5: results
 constexpr int I8_KB = 128;        // K bytes a block
@@ -73,8 +136,9 @@ struct I8Params {
   int TN, TM, BN;      // channel tiles, token tiles, tokens a tile
   int full, T;         // tiles of whole rounds, all tiles
   int G, Gr;           // CTAs, CTAs that share the rest
+  int units;           // "even": units of 32 channels; else 0
   int64_t rb;          // K blocks of the rest
-  int ST;              // stages
+  int ST, KS;          // stages, K blocks a stage
   uint32_t idesc, tcols;
   const float *s, *ws, *bias;
   void *y; int64_t y_ld; int ydt;
@@ -82,44 +146,60 @@ struct I8Params {
   unsigned *ticket;    // [T - full] K blocks arrived, zero between calls
 };
 
-// a CTA's pieces: its run of the rest, then its whole tiles
+// a CTA's pieces: its run of the rest, then its whole tiles; or its even share
+// tile -> (channel tile, token tile): groups of 16 token tiles, so that the
+// tiles of a round share few weight and few token rows (both stay in L2)
+constexpr int I8_GT = 16;
+struct I8Piece {
+  int tile, k0, k1;
+  int ch0, rows, t0;  // first channel, channels, first token
+};
 struct I8Pieces {
+  const I8Params &p;
   int64_t r0, r1;
-  int t, G, full, KB;
-  LBX_DEV I8Pieces(const I8Params &p, int c) : r0(0), r1(0), t(c), G(p.G), full(p.full), KB(p.KB) {
-    if (c < p.Gr) {
+  int t, u, u1;
+  LBX_DEV I8Pieces(const I8Params &p, int c) : p(p), r0(0), r1(0), t(c), u(0), u1(0) {
+    if (p.units) {
+      u = (int)((int64_t)p.units * c / p.G);
+      u1 = (int)((int64_t)p.units * (c + 1) / p.G);
+    } else if (c < p.Gr) {
       r0 = p.rb * c / p.Gr;
       r1 = p.rb * (c + 1) / p.Gr;
     }
   }
-  LBX_DEV bool next(int &tile, int &k0, int &k1) {
+  LBX_DEV bool next(I8Piece &e) {
+    e.k0 = 0;
+    e.k1 = p.KB;
+    if (p.units) {
+      if (u >= u1) return false;
+      e.tile = 0;
+      e.t0 = 0;
+      e.ch0 = 32 * u;
+      const int nu = min(4, u1 - u);
+      e.rows = 32 * nu;
+      u += nu;
+      return true;
+    }
     if (r0 < r1) {
-      const int64_t q = r0 / KB;
-      tile = full + (int)q;
-      k0 = (int)(r0 - q * KB);
-      k1 = (int)min((int64_t)KB, k0 + (r1 - r0));
-      r0 += k1 - k0;
-      return true;
+      const int64_t q = r0 / p.KB;
+      e.tile = p.full + (int)q;
+      e.k0 = (int)(r0 - q * p.KB);
+      e.k1 = (int)min((int64_t)p.KB, e.k0 + (r1 - r0));
+      r0 += e.k1 - e.k0;
+    } else if (t < p.full) {
+      e.tile = t;
+      t += p.G;
+    } else {
+      return false;
     }
-    if (t < full) {
-      tile = t;
-      k0 = 0;
-      k1 = KB;
-      t += G;
-      return true;
-    }
-    return false;
+    const int g = e.tile / (p.TN * I8_GT), gs = min(I8_GT, p.TM - g * I8_GT), r = e.tile - g * p.TN * I8_GT;
+    const int tn = r / gs;
+    e.ch0 = 128 * tn;
+    e.rows = 128;
+    e.t0 = p.BN * (g * I8_GT + (r - tn * gs));
+    return true;
   }
 };
-
-// tile -> (channel tile, token tile): groups of 16 token tiles, so that the
-// tiles of a round share few weight and few token rows (both stay in L2)
-constexpr int I8_GT = 16;
-LBX_DEV void i8_tile(const I8Params &p, int tile, int &tn, int &tm) {
-  const int g = tile / (p.TN * I8_GT), gs = min(I8_GT, p.TM - g * I8_GT), r = tile - g * p.TN * I8_GT;
-  tn = r / gs;
-  tm = g * I8_GT + (r - tn * gs);
-}
 
 LBX_DEV void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
   asm volatile(
@@ -129,23 +209,43 @@ LBX_DEV void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *b
       : "memory");
 }
 
-LBX_DEV void i8_store(const I8Params &p, int64_t t, int ch, int acc, float wsc, float b, bool has_b) {
-  float v = __int2float_rn(acc) * __ldcg(p.s + t) * wsc;
-  if (has_b) v += b;
-  if (p.ydt == LBX_F32) reinterpret_cast<float *>(p.y)[t * p.y_ld + ch] = v;
-  else reinterpret_cast<uint16_t *>(p.y)[t * p.y_ld + ch] = f32_to_bf16(v);
+// results of 16 tokens from t on (nc of them in range) at channel ch.  The
+// tokens' scales are all loaded before the first store: a load behind a store
+// to memory that may be the same waits for its turn, and one such wait a token
+// (256 x 700 cycles a tile) held the whole kernel at a quarter of its rate.
+LBX_DEV void i8_store16(const I8Params &p, int64_t t, int nc, int ch, const int *acc, float wsc, float b, bool has_b) {
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = j < nc ? __ldcg(p.s + t + j) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    v[j] = __int2float_rn(acc[j]) * v[j] * wsc;
+    if (has_b) v[j] += b;
+  }
+  if (p.ydt == LBX_F32) {
+    float *y = reinterpret_cast<float *>(p.y) + t * p.y_ld + ch;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < nc) y[j * p.y_ld] = v[j];
+  } else {
+    uint16_t *y = reinterpret_cast<uint16_t *>(p.y) + t * p.y_ld + ch;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < nc) y[j * p.y_ld] = f32_to_bf16(v[j]);
+  }
 }
 
 __global__ void __launch_bounds__(I8_THREADS, 1)
-    linear_int8_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
-                       const __grid_constant__ I8Params p) {
+    linear_int8_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tw32,
+                       const __grid_constant__ CUtensorMap tx, const __grid_constant__ I8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = align1024(smem_raw);
   __shared__ __align__(8) uint64_t full[I8_MAXST], empty[I8_MAXST], tfull[2], tempty[2], drain;
   __shared__ uint32_t tbase;
   __shared__ int abort_flag, s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
-  const int abytes = 128 * I8_KB, bbytes = p.BN * I8_KB, stage = abytes + bbytes;
+  // a stage: KS tiles of weights, then KS of tokens
+  const int abytes = 128 * I8_KB, bbytes = p.BN * I8_KB, stage = p.KS * (abytes + bbytes), boff = p.KS * abytes;
   volatile int *abrt = &abort_flag;
   if (tid == 0) {
     for (int i = 0; i < p.ST; ++i) {
@@ -169,39 +269,47 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
   if (warp == 0 && lane == 0) {
     // ---- copies.  The weights do not come from the kernel before this one:
     // the first stages' are on their way before its codes are waited for.
-    auto load_w = [&](int j, int tile, int kb) {
-      int tn, tm;
-      i8_tile(p, tile, tn, tm);
-      uint8_t *d = sm + (j % p.ST) * stage;
-      mbar_arrive_expect_tx(&full[j % p.ST], (uint32_t)stage);
-      tma_2d(d, &tw, kb * I8_KB, tn * 128, &full[j % p.ST]);
+    auto load_w = [&](int st, const I8Piece &e, int kb) {
+      const int nk = min(p.KS, e.k1 - kb);
+      mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * (e.rows * I8_KB + bbytes)));
+      for (int i = 0; i < nk; ++i) {
+        uint8_t *d = sm + st * stage + i * abytes;
+        if (e.rows == 128) {
+          tma_2d(d, &tw, (kb + i) * I8_KB, e.ch0, &full[st]);
+        } else {
+          for (int r = 0; r < e.rows; r += 32) tma_2d(d + r * I8_KB, &tw32, (kb + i) * I8_KB, e.ch0 + r, &full[st]);
+        }
+      }
     };
-    auto load_x = [&](int j, int tile, int kb) {
-      int tn, tm;
-      i8_tile(p, tile, tn, tm);
-      tma_2d(sm + (j % p.ST) * stage + abytes, &tx, kb * I8_KB, tm * p.BN, &full[j % p.ST]);
-    };
-    int tile, k0, k1, j = 0;
+    I8Piece e;
+    int j = 0;
     {
       I8Pieces pre(p, cta);
-      while (j < p.ST && pre.next(tile, k0, k1))
-        for (int kb = k0; kb < k1 && j < p.ST; ++kb) load_w(j++, tile, kb);
+      while (j < p.ST && pre.next(e))
+        for (int kb = e.k0; kb < e.k1 && j < p.ST; kb += p.KS) load_w(j++, e, kb);
     }
     const int npre = j;
     pdl_wait();
     I8Pieces it(p, cta);
+    int st = 0;
+    uint32_t ph = 1;  // parity of the stage's last release
     j = 0;
     bool ok = true;
-    while (ok && it.next(tile, k0, k1)) {
-      for (int kb = k0; kb < k1; ++kb, ++j) {
+    while (ok && it.next(e)) {
+      for (int kb = e.k0; kb < e.k1; kb += p.KS, ++j) {
         if (j >= npre) {
-          if (!wd_wait(&empty[j % p.ST], (uint32_t)(j / p.ST - 1) & 1u, 0x821, abrt)) {
+          if (!wd_wait(&empty[st], ph, 0x821, abrt)) {
             ok = false;
             break;
           }
-          load_w(j, tile, kb);
+          load_w(st, e, kb);
         }
-        load_x(j, tile, kb);
+        for (int i = 0; i < p.KS && kb + i < e.k1; ++i)
+          tma_2d(sm + st * stage + boff + i * bbytes, &tx, (kb + i) * I8_KB, e.t0, &full[st]);
+        if (++st == p.ST) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
     }
     if (*abrt) {  // copies in flight land before shared memory is given up
@@ -211,23 +319,31 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
   } else if (warp == 1 && lane == 0) {
     // ---- MMA
     I8Pieces it(p, cta);
-    int tile, k0, k1, j = 0, n = 0;
+    I8Piece e;
+    int n = 0, st = 0;
+    uint32_t ph = 0;
     bool ok = true;
-    while (ok && it.next(tile, k0, k1)) {
+    while (ok && it.next(e)) {
       const uint32_t d = tmem + (uint32_t)(n & 1) * tbuf;
       if (n >= 2 && !wd_wait(&tempty[n & 1], (uint32_t)(n / 2 - 1) & 1u, 0x823, abrt)) break;
       tc_fence_after();
-      for (int kb = k0; kb < k1; ++kb, ++j) {
-        if (!wd_wait(&full[j % p.ST], (uint32_t)(j / p.ST) & 1u, 0x824, abrt)) {
+      for (int kb = e.k0; kb < e.k1; kb += p.KS) {
+        if (!wd_wait(&full[st], ph, 0x824, abrt)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t a = smem_u32(sm + (j % p.ST) * stage), b = a + (uint32_t)abytes;
+        uint64_t a = sw128_desc(smem_u32(sm + st * stage)), b = sw128_desc(smem_u32(sm + st * stage + boff));
+        for (int i = 0; i < p.KS && kb + i < e.k1; ++i, a += abytes >> 4, b += bbytes >> 4) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          umma_i8(d, sw128_desc(a + 32 * q), sw128_desc(b + 32 * q), p.idesc, kb > k0 || q > 0 ? 1u : 0u);
-        umma_commit(&empty[j % p.ST]);
+          for (int q = 0; q < 4; ++q)  // (32 bytes on: 2 in the descriptors' address units)
+            umma_i8(d, a + 2 * q, b + 2 * q, p.idesc, kb + i > e.k0 || q > 0 ? 1u : 0u);
+        }
+        umma_commit(&empty[st]);
+        if (++st == p.ST) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
       if (ok) umma_commit(&tfull[n & 1]);
       ++n;
@@ -243,17 +359,17 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lq = (uint32_t)(32 * (warp & 3)) << 16;
     I8Pieces it(p, cta);
-    int tile, k0, k1, n = 0;
-    while (it.next(tile, k0, k1)) {
+    I8Piece e;
+    int n = 0;
+    while (it.next(e)) {
       // (after a wait that gave up all four warps still go through the same
       // barriers: the pieces left then pass at once, and the call has failed)
       wd_wait(&tfull[n & 1], (uint32_t)(n / 2) & 1u, 0x826, abrt);
       __syncwarp();
       tc_fence_after();
-      int tn, tm;
-      i8_tile(p, tile, tn, tm);
-      const int ch = tn * 128 + row, t0 = tm * p.BN, nc = min(p.BN, p.m - t0);
-      const bool cok = ch < p.n, whole = k0 == 0 && k1 == p.KB, hb = p.bias != nullptr;
+      const int tile = e.tile, k0 = e.k0, k1 = e.k1;
+      const int ch = e.ch0 + row, t0 = e.t0, nc = min(p.BN, p.m - t0);
+      const bool cok = row < e.rows && ch < p.n, whole = k0 == 0 && k1 == p.KB, hb = p.bias != nullptr;
       const float wsc = cok ? p.ws[ch] : 0.f, bs = cok && hb ? p.bias[ch] : 0.f;
       int32_t *slot = p.part + ((int64_t)cta * 2 + (k0 > 0 ? 0 : 1)) * 128 * p.BN;
       const uint32_t ta = tmem + (uint32_t)(n & 1) * tbuf + lq;
@@ -262,11 +378,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         tmem_ld<16>(ta + c0, r);
         tmem_ld_wait();
         if (whole) {
-          if (cok) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c0 + j < nc) i8_store(p, t0 + c0 + j, ch, (int)r[j], wsc, bs, hb);
-          }
+          if (cok) i8_store16(p, t0 + c0, nc - c0, ch, reinterpret_cast<const int *>(r), wsc, bs, hb);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
@@ -289,25 +401,36 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (!s_last) continue;
       __threadfence();
-      const int64_t base = (int64_t)(tile - p.full) * p.KB;
-      int cl = (int)(base * p.Gr / p.rb);  // the first CTA with K blocks of this tile
+      // the parts: those of CTAs cl .. ch_, four at a time so that their loads
+      // are in flight together
+      const int base = (tile - p.full) * p.KB;
+      int cl = (int)((int64_t)base * p.Gr / p.rb);  // the first CTA with K blocks of this tile
       while (cl > 0 && p.rb * cl / p.Gr > base) --cl;
       while (p.rb * (cl + 1) / p.Gr <= base) ++cl;
+      int ce = (int)((int64_t)(base + p.KB) * p.Gr / p.rb);  // and the first without any more
+      while (ce > cl && p.rb * ce / p.Gr >= base + p.KB) --ce;
+      while (ce < p.Gr && p.rb * ce / p.Gr < base + p.KB) ++ce;
+      const int32_t *p0 = p.part + ((int64_t)cl * 2 + (p.rb * cl / p.Gr > base ? 0 : 1)) * 128 * p.BN + row;
+      const int32_t *pn = p.part + (int64_t)(cl + 1) * 2 * 128 * p.BN + row;  // (the others start inside the tile)
+      const int64_t ps = (int64_t)2 * 128 * p.BN;
+      const int np = ce - cl;
       for (int c0 = 0; c0 < nc; c0 += 16) {
-        int acc[16] = {};
-        for (int c = cl; c < p.Gr; ++c) {
-          const int64_t b0 = p.rb * c / p.Gr;
-          if (b0 >= base + p.KB) break;
-          const int32_t *ps = p.part + ((int64_t)c * 2 + (b0 > base ? 0 : 1)) * 128 * p.BN;
+        int acc[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < nc) acc[j] += __ldcg(ps + (c0 + j) * 128 + row);
-        }
-        if (cok) {
+        for (int j = 0; j < 16; ++j) acc[j] = c0 + j < nc ? __ldcg(p0 + (c0 + j) * 128) : 0;
+        for (int c = 1; c < np; c += 4) {
+          int v[4][16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < nc) i8_store(p, t0 + c0 + j, ch, acc[j], wsc, bs, hb);
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              v[u][j] = c + u < np && c0 + j < nc ? __ldcg(pn + (c - 1 + u) * ps + (c0 + j) * 128) : 0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[j] += v[u][j];
         }
+        if (cok) i8_store16(p, t0 + c0, nc - c0, ch, acc, wsc, bs, hb);
       }
     }
   }
@@ -334,18 +457,54 @@ static I8Plan i8_plan(int m, int n, int k) {
   p.n = n;
   p.KB = (k + I8_KB - 1) / I8_KB;
   p.TN = (n + 127) / 128;
-  p.TM = (m + 255) / 256;
-  const int per = (m + p.TM - 1) / p.TM;
-  p.BN = per <= 16 ? 16 : (per + 31) / 32 * 32;
+  const int sms = std::min(device_sm_count(), I8_MAXCTA);
+  // The cheapest of tokens a tile and of the ways to deal, by the cycles of the
+  // busiest SM.  A K block costs the longest of: its MMAs (2 BN cycles, 81 an MMA
+  // at least), its bytes from L2 (37 a cycle and SM, measured with every SM
+  // loading), its weights' share of memory (23.7 a cycle and SM, once for all token tiles).
+  // A tile's results cost 20 cycles a token and 1000; a cut tile's parts go to
+  // L2 and back (40 bytes a cycle, 4000 cycles of latency).
+  auto block = [&](int bn, int tm, int rows) {
+    return std::max({324.0, 2.0 * bn, (rows + bn) * 128.0 / 37, rows * 128.0 / 23.7 / tm});
+  };
+  double best = 0;
+  auto take = [&](double c) {
+    if (best != 0 && c >= best) return false;
+    best = c;
+    return true;
+  };
+  for (int bn = 16; bn <= 256; bn += bn < 32 ? 16 : 32) {
+    const int tm = (m + bn - 1) / bn;
+    const int64_t T = (int64_t)p.TN * tm;
+    if (T > 0x3fffffff) continue;
+    const double out = 20.0 * std::min(bn, m) + 1000, tile = p.KB * block(bn, tm, 128) + out;
+    const int64_t full = T / sms * sms, rb = (T - full) * p.KB;
+    const int gr = (int)std::min<int64_t>(sms, std::max<int64_t>(1, rb / I8_MINBLK));
+    auto set = [&](int64_t nfull, int64_t nrb, int ngr, int units) {
+      p.BN = bn;
+      p.TM = tm;
+      p.T = (int)T;
+      p.full = (int)nfull;
+      p.rb = nrb;
+      p.Gr = ngr;
+      p.units = units;
+      p.G = (int)std::min<int64_t>(sms, units ? units : nfull ? T : ngr);
+    };
+    if (take((double)((T + sms - 1) / sms) * tile)) set(T, 0, 1, 0);
+    if (rb) {
+      const double parts = 2 + (double)gr / (T - full);
+      if (take((double)(T / sms) * tile + (double)rb / gr * block(bn, tm, 128) + out + 4000 +
+               parts * std::min(bn, m) * 512 / 40))
+        set(full, rb, gr, 0);
+    }
+    if (tm == 1) {
+      const int units = (n + 31) / 32, per = (units + sms - 1) / sms, tail = per % 4;
+      if (take((per / 4) * tile + (tail ? p.KB * block(bn, 1, 32 * tail) + out : 0))) set(0, 0, 1, units);
+    }
+  }
   p.idesc = idesc_i8(p.BN);
   p.tcols = 32;
   while (p.tcols < 2u * p.BN) p.tcols *= 2;
-  p.G = std::min(device_sm_count(), I8_MAXCTA);
-  p.T = p.TN * p.TM;
-  p.full = p.T / p.G * p.G;
-  p.rb = (int64_t)(p.T - p.full) * p.KB;
-  p.Gr = (int)std::min<int64_t>(p.G, std::max<int64_t>(1, p.rb / I8_MINBLK));
-  if (p.full == 0) p.G = p.Gr;
   w.part = al((size_t)I8_MAXCTA * 4);
   w.s = w.part + al((size_t)p.Gr * 2 * 128 * p.BN * 4);
   w.q = w.s + al((size_t)m * 4);
@@ -385,8 +544,12 @@ static int i8_map(CUtensorMap *map, const void *base, int64_t rows, int k, int64
 
 static int quant_tokens_launch(const void *x, int xdt, int64_t x_ld, int m, int k, int8_t *q, int64_t q_ld,
                                float *scale, bool pdl, cudaStream_t stream) {
-  return cuda_status(launch(quant_tokens_kernel, dim3(m), dim3(Q8_THREADS), 0, stream, pdl, x, xdt, x_ld, k, q, q_ld, scale),
-                     "quant_tokens launch");
+  const int es = xdt == LBX_F32 ? 4 : 2, e = 16 / es;
+  const bool vec = aligned16(x) && x_ld * es % 16 == 0 && reinterpret_cast<uintptr_t>(q) % e == 0 && q_ld % e == 0;
+  auto go = [&](auto kern) { return launch(kern, dim3(m), dim3(Q8_THREADS), 0, stream, pdl, x, x_ld, k, q, q_ld, scale); };
+  const cudaError_t r = xdt == LBX_F32 ? (vec ? go(quant_tokens_kernel<LBX_F32, true>) : go(quant_tokens_kernel<LBX_F32, false>))
+                                       : (vec ? go(quant_tokens_kernel<LBX_BF16, true>) : go(quant_tokens_kernel<LBX_BF16, false>));
+  return cuda_status(r, "quant_tokens launch");
 }
 
 }  // namespace lbx
@@ -419,6 +582,7 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   LBX_CHECK_ARG(a->x_ld >= a->k && a->w_ld >= a->k && a->y_ld >= a->n, "row strides smaller than the rows");
   LBX_CHECK_ARG(aligned16(a->w) && a->w_ld % 16 == 0, "weight rows must start on 16 bytes");
   I8Plan W = i8_plan(a->m, a->n, a->k);
+  LBX_CHECK_SUP(W.p.BN > 0, "too many tiles");
   LBX_CHECK_ARG(ws && ws_bytes >= W.total, "workspace too small (%zu < %zu)", ws_bytes, W.total);
   LBX_CHECK_ARG(aligned16(ws), "the workspace must be 16-byte aligned");
   uint8_t *b = reinterpret_cast<uint8_t *>(ws);
@@ -431,8 +595,14 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
     return cuda_status(allow_max_smem(linear_int8_kernel, &out), "linear_int8 smem attribute");
   });
   if (rc) return rc;
-  const int stage = (128 + p.BN) * I8_KB;
-  p.ST = std::min(I8_MAXST, (int)((smax - 1024) / stage));
+  const int blk = (128 + p.BN) * I8_KB;
+  // The even deal is a stream from memory: up to 4 K blocks a stage, so that 512
+  // consecutive bytes of a row are asked for together (262 MB for 8 tokens: 72.7 us with
+  // one block a stage, 66.6 with two, 64.5 with four), with three stages at least.
+  const int st_max = (int)((smax - 1024) / blk);
+  p.KS = !p.units ? 1 : st_max >= 12 ? 4 : st_max >= 6 ? 2 : 1;
+  p.ST = std::min(I8_MAXST, st_max / p.KS);
+  const int stage = p.KS * blk;
   p.s = s;
   p.ws = a->w_scale;
   p.bias = a->bias;
@@ -441,14 +611,16 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   p.ydt = a->y_dtype;
   p.part = reinterpret_cast<int32_t *>(b + W.part);
   p.ticket = reinterpret_cast<unsigned *>(b);
-  CUtensorMap tw, tx;
+  CUtensorMap tw, tw32, tx;
   rc = i8_map(&tw, a->w, a->n, a->k, a->w_ld, 128);
+  if (rc) return rc;
+  rc = i8_map(&tw32, a->w, a->n, a->k, a->w_ld, 32);
   if (rc) return rc;
   rc = i8_map(&tx, q, a->m, a->k, W.q_ld, p.BN);
   if (rc) return rc;
   rc = quant_tokens_launch(a->x, a->x_dtype, a->x_ld, a->m, a->k, q, W.q_ld, s, a->use_pdl != 0, stream);
   if (rc) return rc;
   return cuda_status(launch(linear_int8_kernel, dim3(p.G), dim3(I8_THREADS), (size_t)p.ST * stage + 1024, stream, true, tw,
-                            tx, p),
+                            tw32, tx, p),
                      "linear_int8 launch");
 }
