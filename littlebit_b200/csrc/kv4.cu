@@ -3,7 +3,9 @@
 // Each head and slot holds head_dim codes and, for each group of 64
 // dimensions, (step, least) in bf16; a value is least + step * code.
 // See include/lbx.h for the layout.
-#include "common.cuh"
+#include <cuda_fp16.h>
+
+#include "tcgen05.cuh"
 
 namespace lbx {
 
@@ -155,95 +157,589 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
   o[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// ---------------------------------------------------------------------------
+// Attention: o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(s_ij - m_i),
+// s_ij = q_i . k_j (q scaled by scale * log2 e), one pass with the running maximum.
+//
+// Both products run on the tensor cores (mma.m16n8k16, fp16 in, fp32 sums)
+// straight from the packed codes.  Keys: a code c in the low bits of a 16-bit lane IS
+// the fp16 subnormal c * 2^-24, which the tensor cores multiply exactly, so a pair
+// of codes costs one AND (and every second pair a shift, nibbles 1 and 3 being left
+// at 16 times their value).  With step and least value of a group of dimensions
+// outside the sum,
+//
+//   q . k = sum_g [ step_g (sum_{d in g} q_d c_d) + least_g (sum_{d in g} q_d) ]
+//   o_d   = sum_j (p_j step_jg) (c_jd - 8) + sum_j p_j (least_jg + 8 step_jg)
+//
+// so codes enter as they are stored and only the queries and p * step are
+// rounded to fp16.  The values' codes are centred first (one subtraction a pair): the
+// tensor cores round their sums towards zero, and over thousands of slots of one
+// sign that showed (4e-5 of the result at 4000 slots, 6e-4 at 130 000).  Queries and p * step are
+// brought to [2^14, 2^15) by a power of two (a query by its group's largest, p * step
+// by the largest step the row has seen).
+// float32 (SPLIT): rows 0-7 of the MMA hold the leading 11 bits and rows 8-15 the
+// next 11 of the same eight query rows: 22 bits, float32's own error.
+// bfloat16: 16 query rows (H2) or 8, 11 bits against the result's 8.
+//
+// Work: a warp takes one sub-chunk of CK slots for one tile of query rows, 32
+// slots a step, and leaves (m, l, o) to be merged in sub-chunk order; the row
+// tiles of a block share the ring of bulk copies.  Sub-chunks and steps lie at
+// fixed slots and a row's arithmetic involves no other row, so its bits do not
+// depend on what else the call holds.
+// ---------------------------------------------------------------------------
+constexpr int KA_STEP = 32;     // slots a step (one stage of the ring)
+constexpr int KA_ST = 4;        // stages
+constexpr int KA_WARPS = 4;     // warps a block at most
+
 struct Kv4AttnParams {
   Kv4View c;
   int n, heads, rep, max_prefix, dtype;
-  float scale;
+  int i0, R;           // first token of this launch's rows, query rows of a kv head
+  int ck, nsub;        // slots a sub-chunk, sub-chunks of the longest sequence
+  int kw, rw, ntile;   // sub-chunks and row tiles a block, row tiles in all
+  float scale;         // times log2 e
   const int32_t *prefix;
   const void *q; int64_t q_ld;
   const float2 *rope;
   const uint64_t *tree;
   void *out;
+  float *part_o;       // [n_seq][kvh][nsub][R][D]
+  float2 *part_ml;     // [n_seq][kvh][nsub][R]
 };
 
-// does query i of its sequence see slot j
-LBX_DEV bool kv4_sees(int j, int prefix, int n, int i, const uint64_t *mask) {
-  if (j < prefix) return true;
-  const int t = j - prefix;
-  return t < n && (mask ? (t < 64 && ((*mask >> t) & 1ull)) : t <= i);
+LBX_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+LBX_DEV uint32_t f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// what the fp16 rounding of (lo, hi) in r left over, as fp16
+LBX_DEV uint32_t f16x2_rest(uint32_t r, float lo, float hi) {
+  const __half2 h = *reinterpret_cast<const __half2 *>(&r);
+  return f16x2(lo - __low2float(h), hi - __high2float(h));
+}
+// exponent of |x| <- its bits, within what the power-of-two factors below reach
+LBX_DEV int kv4_exp(uint32_t bits) { return min(max((int)(bits >> 23) - 127, -112), 100); }
+LBX_DEV float kv4_up(int e) { return __uint_as_float((uint32_t)(141 - e) << 23); }    // 2^(14 - e)
+LBX_DEV float kv4_down(int e) { return __uint_as_float((uint32_t)(113 + e) << 23); }  // 2^(e - 14)
+// codes in bits 4 N .. 4 N + 3 of both halves -> 16^N (code - 8) as fp16: 1024 + 16^N code by
+// its bits, less 1024 + 8 * 16^N, both exact
+template <int N>
+LBX_DEV uint32_t kv4_mid(uint32_t x) {
+  const uint32_t v = (x & (N ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u, off = N ? 0x64806480u : 0x64086408u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&off));
+  return *reinterpret_cast<const uint32_t *>(&d);
+}
+LBX_DEV float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+LBX_DEV float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+LBX_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// One CTA a (query head, token row): 128 slots at a time, a thread each for the
-// scores, a thread a dimension for the sums; one pass with the running maximum.
+// does query i of its sequence see slot j
+LBX_DEV bool kv4_sees(int j, int prefix, int n, int i, bool tree, uint64_t mask) {
+  if (j < prefix) return true;
+  const int t = j - prefix;
+  return t < n && (tree ? (t < 64 && ((mask >> t) & 1ull)) : t <= i);
+}
+
+// slot, among the eight of an MMA's column tile, of column rho: neighbours keep
+// opposite parity (two rows of keys per shared-memory wavefront), and so do
+// columns 0, 2, 4, 6 in turn (the value rows a warp reads together)
+LBX_DEV int kv4_key(int rho) { return rho ^ ((rho >> 1) & 1); }
+
 template <int D>
-__global__ void __launch_bounds__(128) kv4_attn_simple_kernel(const __grid_constant__ Kv4AttnParams p) {
-  __shared__ float qs[D], ps[128], red[4];
-  const int tid = threadIdx.x, hq = blockIdx.x, h = hq / p.rep;
-  const int64_t row = blockIdx.y;
-  const int s = (int)(row / p.n), i = (int)(row - (int64_t)s * p.n);
-  const int prefix = p.prefix ? p.prefix[s] : p.max_prefix;
-  const int64_t o = row * (int64_t)p.heads * D + (int64_t)hq * D;
-  auto store = [&](int t, float v) {
-    if (p.dtype == LBX_F32) reinterpret_cast<float *>(p.out)[o + t] = v;
-    else reinterpret_cast<uint16_t *>(p.out)[o + t] = f32_to_bf16(v);
-  };
-  if (prefix < 0 || prefix > p.max_prefix) {
-    if (tid == 0) atomicCAS(&g_lbx_device_error, 0, 0x803);
-    if (tid < D) store(tid, __uint_as_float(0x7FC00000u));
-    return;
+struct Kv4Stage {
+  static constexpr int CB = KA_STEP * D / 2, PB = KA_STEP * (D / KV4_G) * 4;  // bytes of codes, of params
+  static constexpr int BYTES = 2 * (CB + PB);
+};
+
+// One query row's fragment values: the 8-dimension blocks of lane j (block
+// b(t) = (t >> 1) * 8 + (t & 1) * 4 + j for head_dim 128, t * 4 + j for 64),
+// rotated and scaled; both members of every rotation pair are the lane's own.
+template <int D>
+LBX_DEV void kv4_load_q(const Kv4AttnParams &p, int64_t row, int hq, int j, bool ok, float (&x)[D / 4]) {
+  constexpr int NW = D / 32;  // blocks a lane
+#pragma unroll
+  for (int t = 0; t < NW; ++t) {
+    const int b = D == 128 ? (t >> 1) * 8 + (t & 1) * 4 + j : t * 4 + j;
+    const int64_t o = row * p.q_ld + (int64_t)hq * D + 8 * b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[8 * t + i] = ok ? load_act(p.q, p.dtype, o + i) : 0.f;
   }
-  for (int j = tid; j < D / 2; j += 128) {
-    const int64_t qo = row * p.q_ld + (int64_t)hq * D;
-    const float x1 = load_act(p.q, p.dtype, qo + j), x2 = load_act(p.q, p.dtype, qo + j + D / 2);
-    const float2 cs = p.rope ? p.rope[row * (D / 2) + j] : make_float2(1.f, 0.f);
-    qs[j] = (x1 * cs.x - x2 * cs.y) * p.scale;
-    qs[j + D / 2] = (x2 * cs.x + x1 * cs.y) * p.scale;
+  if (p.rope && ok) {
+#pragma unroll
+    for (int t = 0; t < NW / 2; ++t) {
+      const int b = t * 4 + j;  // (first half of the dimensions)
+      const float2 *cs = p.rope + row * (D / 2) + 8 * b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 c = __ldg(cs + i);
+        const float x1 = x[8 * t + i], x2 = x[8 * (t + NW / 2) + i];
+        x[8 * t + i] = x1 * c.x - x2 * c.y;
+        x[8 * (t + NW / 2) + i] = x2 * c.x + x1 * c.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i) x[i] *= p.scale;
+}
+
+template <int D, bool SPLIT, bool H2>
+__global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int NG = D / KV4_G, NW = D / 32, NH = H2 ? 2 : 1;
+  constexpr int RT = H2 ? 16 : 8;  // query rows a tile
+  using Stage = Kv4Stage<D>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[KA_WARPS][KA_ST], empty[KA_WARPS][KA_ST];
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, j = lane & 3;
+  const int kg = warp / p.rw, rt = warp - kg * p.rw;  // this warp's sub-chunk and row tile in the block
+  const int rgroups = (p.ntile + p.rw - 1) / p.rw;
+  const int cblk = blockIdx.x / rgroups, rg = blockIdx.x - cblk * rgroups;
+  const int c = cblk * p.kw + kg, h = blockIdx.y, s = blockIdx.z;
+  volatile int *abrt = &abort_flag;
+  if (tid == 0) {
+    for (int g = 0; g < p.kw; ++g)
+      for (int i = 0; i < KA_ST; ++i) {
+        mbar_init(&full[g][i], 1);
+        mbar_init(&empty[g][i], p.rw);
+      }
+    fence_mbar_init();
+    abort_flag = 0;
   }
   __syncthreads();
-  const uint64_t *mask = p.tree ? p.tree + row : nullptr;
-  const int top = prefix + p.n;
-  const int64_t base = ((int64_t)s * p.c.kvh + h) * p.c.max_seq;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int j0 = 0; j0 < top; j0 += 128) {
-    const int j = j0 + tid;
-    float sc = -INFINITY;
-    if (j < top && kv4_sees(j, prefix, p.n, i, mask)) {
-      const uint32_t *w = reinterpret_cast<const uint32_t *>(p.c.kc + (base + j) * (D / 2));
-      sc = 0.f;
-      for (int b = 0; b < D / 8; ++b) {
-        const uint32_t x = w[kv4_word<D, false>(b)];
-        const uint32_t par = p.c.kp[(base + j) * (D / KV4_G) + (b >> 3)];
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          sc = fmaf(qs[8 * b + t], fmaf(kv4_step(par), (float)((x >> (4 * t)) & 15u), kv4_least(par)), sc);
+  pdl_trigger();
+  pdl_wait();
+  const int prefix = p.prefix ? __ldg(p.prefix + s) : p.max_prefix;
+  if (prefix < 0 || prefix > p.max_prefix) {
+    if (tid == 0) atomicCAS(&g_lbx_device_error, 0, 0x803);
+    if (p.nsub > 1 || kg > 0) return;  // (the merge tells the rows)
+    for (int R = (rg * p.rw + rt) * RT; R < min(p.R, (rg * p.rw + rt + 1) * RT); ++R) {
+      const int i = p.i0 + R / p.rep;
+      const int64_t d0 = (((int64_t)s * p.n + i) * p.heads + h * p.rep + R % p.rep) * D;
+      for (int d = lane; d < D; d += 32) {
+        if (p.dtype == LBX_F32) reinterpret_cast<float *>(p.out)[d0 + d] = __uint_as_float(0x7FC00000u);
+        else reinterpret_cast<uint16_t *>(p.out)[d0 + d] = KV4_NAN;
       }
     }
-    const float wm = warp_max(sc);
-    if ((tid & 31) == 0) red[tid >> 5] = wm;
-    __syncthreads();
-    const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    ps[tid] = sc == -INFINITY ? 0.f : expf(sc - mn);
-    __syncthreads();
-    const float f = m == -INFINITY ? 0.f : expf(m - mn);
-    l *= f;
-    acc *= f;
-    m = mn;
-    const int jn = min(128, top - j0);
-    for (int jj = 0; jj < jn; ++jj) {
-      const float pr = ps[jj];
-      if (!(pr > 0.f) && pr == pr) continue;
-      l += pr;
-      if (tid < D) {
-        const int b = tid >> 3;
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(p.c.vc + (base + j0 + jj) * (D / 2));
-        const uint32_t x = w[kv4_word<D, true>(b)];
-        const uint32_t par = p.c.vp[(base + j0 + jj) * (D / KV4_G) + (b >> 3)];
-        acc = fmaf(pr, fmaf(kv4_step(par), (float)((x >> (4 * (tid & 7))) & 15u), kv4_least(par)), acc);
-      }
-    }
-    __syncthreads();
+    return;
   }
-  if (tid < D) store(tid, l == 0.f ? 0.f : acc / l);
+  // slots this block's row tiles see, and this warp's
+  const int t0 = rg * p.rw, tl = min(t0 + p.rw, p.ntile) - 1;  // first and last tile of the block
+  const int tile = t0 + rt;
+  auto seen_end = [&](int tl_) {
+    return prefix + (p.tree ? p.n : p.i0 + (min(p.R, (tl_ + 1) * RT) - 1) / p.rep + 1);
+  };
+  const int lo = c * p.ck;
+  const int hi_blk = min(lo + p.ck, seen_end(tl));
+  const int nst = hi_blk > lo ? (hi_blk - lo + KA_STEP - 1) / KA_STEP : 0;
+  if (nst == 0 || c >= p.nsub) return;  // (every warp of this ring)
+  const bool live_tile = tile < p.ntile;
+  const int my_end = live_tile ? min(lo + p.ck, seen_end(tile)) : 0;
+
+  uint8_t *ring = smem_raw + kg * KA_ST * Stage::BYTES;
+  const int64_t base = ((int64_t)s * p.c.kvh + h) * p.c.max_seq + lo;
+  auto issue = [&](int i) {  // (one lane)
+    const int st = i % KA_ST;
+    uint8_t *d = ring + st * Stage::BYTES;
+    const int64_t slot = base + (int64_t)i * KA_STEP;
+    mbar_arrive_expect_tx(&full[kg][st], Stage::BYTES);
+    bulk_g2s(d, p.c.kc + slot * (D / 2), Stage::CB, &full[kg][st]);
+    bulk_g2s(d + Stage::CB, p.c.kp + slot * NG, Stage::PB, &full[kg][st]);
+    bulk_g2s(d + Stage::CB + Stage::PB, p.c.vc + slot * (D / 2), Stage::CB, &full[kg][st]);
+    bulk_g2s(d + 2 * Stage::CB + Stage::PB, p.c.vp + slot * NG, Stage::PB, &full[kg][st]);
+  };
+  int issued = 0;
+  if (rt == 0 && lane == 0)
+    for (; issued < KA_ST && issued < nst; ++issued) issue(issued);
+
+  // ---- the queries' fragments
+  uint32_t qa[2 * NW][4];
+  float fq[NH][NG], qs[NH][NG];
+  int qi[NH];         // token index of the row(s)
+  int64_t qrow[NH];   // its row, query head
+  int qh[NH];
+  bool rok[NH];
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    const int R = tile * RT + r + 8 * u;
+    rok[u] = live_tile && R < p.R;
+    qi[u] = p.i0 + (rok[u] ? R / p.rep : 0);
+    qh[u] = h * p.rep + (rok[u] ? R % p.rep : 0);
+    qrow[u] = (int64_t)s * p.n + qi[u];
+    float x[D / 4];
+    kv4_load_q<D>(p, qrow[u], qh[u], j, rok[u], x);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      constexpr int PER = D / 4 / NG;
+      float m = 0.f, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        m = fmaxf(m, fabsf(x[g * PER + i]));
+        sum += x[g * PER + i];
+      }
+      const int e = kv4_exp(__float_as_uint(quad_max(m)));
+      const float up = kv4_up(e);
+      fq[u][g] = kv4_down(e) * 16777216.f;  // (codes enter as 2^-24 of their value)
+      qs[u][g] = quad_sum(sum);
+#pragma unroll
+      for (int t = g * NW / NG; t < (g + 1) * NW / NG; ++t) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[8 * t + i] * ((i & 1) ? up * 0.0625f : up);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // (k step 2t + k: dimensions 2k, 2k+4 and 2k+1, 2k+5 of the block)
+          const uint32_t a0 = f16x2(y[2 * k], y[2 * k + 4]), a2 = f16x2(y[2 * k + 1], y[2 * k + 5]);
+          if (SPLIT) {
+            qa[2 * t + k][0] = a0;
+            qa[2 * t + k][2] = a2;
+            qa[2 * t + k][1] = f16x2_rest(a0, y[2 * k], y[2 * k + 4]);
+            qa[2 * t + k][3] = f16x2_rest(a2, y[2 * k + 1], y[2 * k + 5]);
+          } else {
+            qa[2 * t + k][u] = a0;
+            qa[2 * t + k][2 + u] = a2;
+            if (!H2) qa[2 * t + k][1] = qa[2 * t + k][3] = 0u;
+          }
+        }
+      }
+    }
+  }
+  const bool tree = p.tree != nullptr;
+  uint64_t mask[NH];
+#pragma unroll
+  for (int u = 0; u < NH; ++u) mask[u] = tree && rok[u] ? __ldg(p.tree + qrow[u]) : 0ull;
+
+  float o[D / 8][4];  // column tile 8 g + i: dimensions 64 g + 8 n + i
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[NH], l[NH], om[NH][NG];
+  int eo[NH];
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+    eo[u] = -112;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) om[u][g] = 0.f;
+  }
+
+  bool ok = true;
+  for (int i = 0; i < nst; ++i) {
+    const int st = i % KA_ST;
+    // the stage read in the step before is free once all row tiles have read it
+    if (rt == 0 && lane == 0 && i > 0 && issued < nst &&
+        wd_wait(&empty[kg][(i - 1) % KA_ST], (uint32_t)((i - 1) / KA_ST) & 1u, 0x805, abrt))
+      issue(issued++);
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, wd_wait(&full[kg][st], (uint32_t)(i / KA_ST) & 1u, 0x804, abrt))) {
+      ok = false;
+      break;
+    }
+    const int j0 = lo + i * KA_STEP;
+    if (j0 < my_end) {
+      const uint8_t *sk = ring + st * Stage::BYTES;
+      const uint32_t *skp = reinterpret_cast<const uint32_t *>(sk + Stage::CB);
+      const uint8_t *sv = sk + Stage::CB + Stage::PB;
+      const uint32_t *svp = reinterpret_cast<const uint32_t *>(sv + Stage::CB);
+      // ---- scores: sc[u][2 t + k], column tile t, this lane's slot kv4_key(2 j + k) of its eight
+      float sc[NH][8];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t w[NW];
+        const uint8_t *kr = sk + (8 * t + kv4_key(r)) * (D / 2) + j * (D / 8);
+        if constexpr (D == 128) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(kr);
+          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2 *>(kr);
+          w[0] = v.x; w[1] = v.y;
+        }
+        float acc[NG][4];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) {
+          const uint32_t y = w[q] >> 8;
+          mma_f16(acc[q * NG / NW], qa[2 * q], w[q] & 0x000F000Fu, w[q] & 0x00F000F0u);
+          mma_f16(acc[q * NG / NW], qa[2 * q + 1], y & 0x000F000Fu, y & 0x00F000F0u);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t *pr = skp + (8 * t + kv4_key(2 * j + k)) * NG;
+#pragma unroll
+          for (int u = 0; u < NH; ++u) sc[u][2 * t + k] = 0.f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t pp = pr[g];
+#pragma unroll
+            for (int u = 0; u < NH; ++u) {
+              const float a = SPLIT ? acc[g][k] + acc[g][2 + k] : acc[g][2 * u + k];
+              sc[u][2 * t + k] = fmaf(a, kv4_step(pp) * fq[u][g], fmaf(kv4_least(pp), qs[u][g], sc[u][2 * t + k]));
+            }
+          }
+        }
+      }
+      // ---- what each row sees of the step; the values' steps, theirs to be kept within fp16
+      const bool whole = j0 + KA_STEP <= prefix;
+      float stp[8][NG], lst[8][NG];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const uint32_t *pr = svp + (8 * (t >> 1) + kv4_key(2 * j + (t & 1))) * NG;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t pp = pr[g];
+          stp[t][g] = kv4_step(pp);
+          lst[t][g] = fmaf(8.f, stp[t][g], kv4_least(pp));
+        }
+      }
+      uint32_t vis[NH];
+#pragma unroll
+      for (int u = 0; u < NH; ++u) {
+        vis[u] = 0xFFu;
+        if (!whole) {
+          vis[u] = 0u;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            if (rok[u] && kv4_sees(j0 + 8 * (t >> 1) + kv4_key(2 * j + (t & 1)), prefix, p.n, qi[u], tree, mask[u]))
+              vis[u] |= 1u << t;
+            else
+              sc[u][t] = -INFINITY;
+          }
+        }
+      }
+      float f[NH];
+      bool change = false;
+      float al[NH];
+#pragma unroll
+      for (int u = 0; u < NH; ++u) {
+        float mx = sc[u][0], sx = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          mx = fmaxf(mx, sc[u][t]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const float a = fabsf(stp[t][g]);
+            if ((whole || (vis[u] >> t & 1u)) && a < INFINITY) sx = fmaxf(sx, a);
+          }
+        }
+        mx = fmaxf(quad_max(mx), m[u]);
+        const int e = max(kv4_exp(__float_as_uint(quad_max(sx))), eo[u]);
+        const bool ch = mx > m[u] || e > eo[u];
+        change |= ch;
+        // (nothing seen so far: any finite reference gives weights 0)
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        al[u] = m[u] == -INFINITY ? 0.f : ex2(m[u] - ref);
+        l[u] *= al[u];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) om[u][g] *= al[u];
+        al[u] *= __uint_as_float((uint32_t)(127 + max(eo[u] - e, -126)) << 23);
+        m[u] = mx;
+        eo[u] = e;
+        f[u] = kv4_up(e);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) sc[u][t] = ex2(sc[u][t] - ref);
+      }
+      if (__any_sync(0xffffffffu, change)) {
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t) {
+          o[t][0] *= al[0];
+          o[t][1] *= al[0];
+          o[t][2] *= al[NH - 1];
+          o[t][3] *= al[NH - 1];
+        }
+      }
+      // ---- values, 16 slots an MMA step: slots of column tiles 2 a (first eight) and 2 a + 1
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        uint32_t pa[NG][4];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const int t = 4 * a + 2 * hf;
+#pragma unroll
+            for (int u = 0; u < NH; ++u) {
+              float x0 = sc[u][t] * f[u] * stp[t][g], x1 = sc[u][t + 1] * f[u] * stp[t + 1][g];
+              float y0 = sc[u][t] * lst[t][g], y1 = sc[u][t + 1] * lst[t + 1][g];
+              if (!whole) {  // (a stale step may be NaN)
+                if (!(vis[u] >> t & 1u)) x0 = y0 = 0.f;
+                if (!(vis[u] >> (t + 1) & 1u)) x1 = y1 = 0.f;
+              }
+              om[u][g] += y0 + y1;
+              const uint32_t hi = f16x2(x0, x1);
+              if (SPLIT) {
+                pa[g][2 * hf] = hi;
+                pa[g][2 * hf + 1] = f16x2_rest(hi, x0, x1);
+              } else {
+                pa[g][2 * hf + u] = hi;
+                if (!H2) pa[g][2 * hf + 1] = 0u;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < NH; ++u) l[u] += (sc[u][4 * a] + sc[u][4 * a + 1]) + (sc[u][4 * a + 2] + sc[u][4 * a + 3]);
+        uint32_t vw[4][NG];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint8_t *vr = sv + (16 * a + 8 * (k >> 1) + kv4_key(2 * j + (k & 1))) * (D / 2) + r * (D / 16);
+          if constexpr (D == 128) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(vr);
+            vw[k][0] = v.x;
+            vw[k][1] = v.y;
+          } else {
+            vw[k][0] = *reinterpret_cast<const uint32_t *>(vr);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {  // nibbles 0-3, 4-7 of the word
+            uint32_t b0 = __byte_perm(vw[0][g], vw[1][g], hf ? 0x7632 : 0x5410);
+            uint32_t b1 = __byte_perm(vw[2][g], vw[3][g], hf ? 0x7632 : 0x5410);
+            mma_f16(o[8 * g + 4 * hf], pa[g], kv4_mid<0>(b0), kv4_mid<0>(b1));
+            mma_f16(o[8 * g + 4 * hf + 1], pa[g], kv4_mid<1>(b0), kv4_mid<1>(b1));
+            b0 >>= 8;
+            b1 >>= 8;
+            mma_f16(o[8 * g + 4 * hf + 2], pa[g], kv4_mid<0>(b0), kv4_mid<0>(b1));
+            mma_f16(o[8 * g + 4 * hf + 3], pa[g], kv4_mid<1>(b0), kv4_mid<1>(b1));
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(&empty[kg][st]);
+  }
+  if (rt == 0 && lane == 0 && *abrt) {  // copies in flight land before shared memory is given up
+    int none = 0;
+    for (int i = max(0, issued - KA_ST); i < issued; ++i)
+      wd_wait(&full[kg][i % KA_ST], (uint32_t)(i / KA_ST) & 1u, 0x806, &none);
+  }
+  if (!ok || my_end <= lo) return;
+
+  // ---- this row's (m, l, o): lane (r, j) holds dimensions 64 g + 16 j .. + 15
+  const bool single = p.nsub == 1;
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    const float lsum = quad_sum(l[u]);
+    float oms[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) oms[g] = quad_sum(om[u][g]);
+    if (!rok[u]) continue;
+    const int R = tile * RT + r + 8 * u;
+    const float dn = kv4_down(eo[u]);
+    const int64_t pr = (((int64_t)s * p.c.kvh + h) * p.nsub + c) * p.R + R;
+    if (!single && j == 0) p.part_ml[pr] = make_float2(m[u], lsum);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = SPLIT ? o[8 * g + i][k] + o[8 * g + i][2 + k] : o[8 * g + i][2 * u + k];
+          v[i] = fmaf(a, (i & 1) ? dn * 0.0625f : dn, oms[g]);
+          if (single) v[i] = lsum == 0.f ? 0.f : v[i] / lsum;  // (as the merge of one sub-chunk)
+        }
+        const int d = 64 * g + 8 * (2 * j + k);
+        if (!single || p.dtype == LBX_F32) {
+          float *dst = single ? reinterpret_cast<float *>(p.out) + (qrow[u] * p.heads + qh[u]) * D + d : p.part_o + pr * D + d;
+          reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          uint16_t *dst = reinterpret_cast<uint16_t *>(p.out) + (qrow[u] * p.heads + qh[u]) * D + d;
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | (uint32_t)f32_to_bf16(v[2 * i + 1]) << 16;
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+  }
+}
+
+// Merge of the sub-chunks' (m, l, o), one block a query row: warp w adds sub-chunks
+// w, w + 4, ... in order, a lane D / 32 dimensions, then the warps in order.
+constexpr int KM_BATCH = 8;  // partial sums loaded together
+template <int D>
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int V = D / 32;
+  __shared__ float red[4], wo[4][D], wl[4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int R = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
+  const int i = p.i0 + R / p.rep, hq = h * p.rep + R % p.rep;
+  pdl_wait();
+  const int prefix = p.prefix ? __ldg(p.prefix + s) : p.max_prefix;
+  const bool bad = prefix < 0 || prefix > p.max_prefix;
+  const int end = prefix + (p.tree ? p.n : i + 1), ns = bad ? 0 : (end + p.ck - 1) / p.ck;
+  const int64_t base = ((int64_t)s * p.c.kvh + h) * p.nsub * p.R + R;
+  float mx = -INFINITY;
+  for (int c = tid; c < ns; c += 128) mx = fmaxf(mx, __ldcg(p.part_ml + base + (int64_t)c * p.R).x);
+  mx = warp_max(mx);
+  if (lane == 0) red[warp] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float o[V], l = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = 0.f;
+  for (int c0 = warp; c0 < ns; c0 += 4 * KM_BATCH) {
+    float2 ml[KM_BATCH];
+    float x[KM_BATCH][V];
+#pragma unroll
+    for (int b = 0; b < KM_BATCH; ++b) {
+      const int c = c0 + 4 * b;
+      ml[b] = make_float2(-INFINITY, 0.f);
+      if (c < ns) {
+        const int64_t pr = base + (int64_t)c * p.R;
+        ml[b] = __ldcg(p.part_ml + pr);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[b][v] = __ldcg(p.part_o + pr * D + lane * V + v);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < KM_BATCH; ++b) {
+      if (ml[b].x == -INFINITY && ml[b].y == 0.f) continue;  // (no sub-chunk, or one without a visible slot)
+      const float w = exp2f(ml[b].x - ref);
+      l = fmaf(w, ml[b].y, l);
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = fmaf(w, x[b][v], o[v]);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) wo[warp][lane * V + v] = o[v];
+  if (lane == 0) wl[warp] = l;
+  __syncthreads();
+  if (tid < D) {
+    const float lt = ((wl[0] + wl[1]) + wl[2]) + wl[3];
+    const float ot = ((wo[0][tid] + wo[1][tid]) + wo[2][tid]) + wo[3][tid];
+    const float y = bad ? __uint_as_float(0x7FC00000u) : lt == 0.f ? 0.f : ot / lt;
+    const int64_t d = (((int64_t)s * p.n + i) * p.heads + hq) * D + tid;
+    if (p.dtype == LBX_F32) reinterpret_cast<float *>(p.out)[d] = y;
+    else reinterpret_cast<uint16_t *>(p.out)[d] = f32_to_bf16(y);
+  }
+}
+
+// slots a sub-chunk: by the cache's size alone (a row's bits then do not depend
+// on the lengths a call is given), 32 sub-chunks of a full cache
+static int kv4_sub_chunk(int max_seq) {
+  int ck = 128;
+  while (ck < 1024 && ck * 32 < max_seq) ck *= 2;
+  return ck;
 }
 
 // the cache's checks, shared by the three calls
@@ -280,7 +776,7 @@ static int kv4_attn_prep(const lbx_kv4_attn_args *a, Kv4AttnParams &p) {
   p.rep = a->heads / a->cache.kv_heads;
   p.max_prefix = a->max_prefix;
   p.dtype = a->dtype;
-  p.scale = a->scale;
+  p.scale = a->scale * 1.4426950408889634f;
   p.prefix = a->prefix;
   p.q = a->q;
   p.q_ld = a->q_ld;
@@ -346,25 +842,87 @@ extern "C" int lbx_kv4_read(const lbx_kv4_cache *c, const int32_t *start, int32_
   return cuda_status(cudaGetLastError(), "kv4_read launch");
 }
 
+namespace lbx {
+// tokens a launch (its partial results stay within a gigabyte) and their bytes
+static int kv4_slice(const Kv4AttnParams &p, int D, int64_t &bytes) {
+  const int ck = kv4_sub_chunk(p.c.max_seq), nsub = (p.max_prefix + p.n + ck - 1) / ck;
+  if (nsub <= 1) {
+    bytes = 0;
+    return p.n;
+  }
+  const int64_t per = (int64_t)p.c.n_seq * p.c.kvh * nsub * p.rep * (D * 4 + 8);
+  const int sl = (int)std::min<int64_t>(p.n, std::max<int64_t>(1, (1ll << 30) / per));
+  bytes = per * sl;
+  return sl;
+}
+
+template <int D>
+static int kv4_attn_launch(Kv4AttnParams p, void *ws, bool pdl, cudaStream_t stream) {
+  const bool split = p.dtype == LBX_F32;
+  p.ck = kv4_sub_chunk(p.c.max_seq);
+  int64_t bytes = 0;
+  const int sl = kv4_slice(p, D, bytes);
+  static DevCache<int> attr;
+  int unused = 0;
+  int rc = attr.get(unused, [](int &) {
+    cudaError_t e = allow_max_smem(kv4_attn_kernel<D, true, false>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, false>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, true>);
+    return cuda_status(e, "kv4_attn smem attribute");
+  });
+  if (rc) return rc;
+  for (int i0 = 0; i0 < p.n; i0 += sl) {
+    const int nt = std::min(sl, p.n - i0);
+    p.i0 = i0;
+    p.R = nt * p.rep;
+    p.nsub = (p.max_prefix + (p.tree ? p.n : i0 + nt) + p.ck - 1) / p.ck;
+    const bool h2 = !split && p.R > 8;
+    p.ntile = (p.R + (h2 ? 15 : 7)) / (h2 ? 16 : 8);
+    // row tiles a block, evenly; the warps left take further sub-chunks
+    const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
+    p.rw = (p.ntile + groups - 1) / groups;
+    p.kw = std::min(KA_WARPS / p.rw, p.nsub);
+    p.part_ml = reinterpret_cast<float2 *>(ws);
+    const int64_t rows = (int64_t)p.c.n_seq * p.c.kvh * p.nsub * p.R;
+    p.part_o = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(ws) + ((rows * 8 + 255) & ~(int64_t)255));
+    const int64_t gx = (int64_t)((p.nsub + p.kw - 1) / p.kw) * ((p.ntile + p.rw - 1) / p.rw);
+    LBX_CHECK_SUP(gx <= 0x7fffffff && p.c.kvh <= 65535 && p.c.n_seq <= 65535, "too many heads, sequences or rows");
+    const dim3 grid((unsigned)gx, p.c.kvh, p.c.n_seq), block(32 * p.kw * p.rw);
+    const size_t smem = (size_t)p.kw * KA_ST * Kv4Stage<D>::BYTES;
+    const bool dep = pdl || i0 > 0;  // (every kernel here waits for the one before it)
+    const cudaError_t e = split ? launch(kv4_attn_kernel<D, true, false>, grid, block, smem, stream, dep, p)
+                          : h2  ? launch(kv4_attn_kernel<D, false, true>, grid, block, smem, stream, dep, p)
+                                : launch(kv4_attn_kernel<D, false, false>, grid, block, smem, stream, dep, p);
+    rc = cuda_status(e, "kv4_attn launch");
+    if (rc) return rc;
+    if (p.nsub > 1) {
+      rc = cuda_status(launch(kv4_merge_kernel<D>, dim3(p.R, p.c.kvh, p.c.n_seq), dim3(128), 0, stream, true, p),
+                       "kv4_merge launch");
+      if (rc) return rc;
+    }
+  }
+  return LBX_OK;
+}
+}  // namespace lbx
+
 extern "C" size_t lbx_kv4_attn_workspace_size(const lbx_kv4_attn_args *a) {
   lbx::Kv4AttnParams p = {};
   if (lbx::kv4_attn_prep(a, p)) return 0;
-  return 256;
+  int64_t bytes = 0;
+  lbx::kv4_slice(p, a->cache.head_dim, bytes);
+  return (size_t)bytes + 512;
 }
 
 extern "C" int lbx_kv4_attn(const lbx_kv4_attn_args *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
   using namespace lbx;
   Kv4AttnParams p = {};
-  const int rc = kv4_attn_prep(a, p);
+  int rc = kv4_attn_prep(a, p);
   if (rc) return rc;
   LBX_CHECK_ARG(a->q && a->out, "NULL pointer");
-  LBX_CHECK_ARG(ws && ws_bytes >= 256, "workspace too small");
-  const int64_t rows = (int64_t)a->cache.n_seq * a->n;
-  LBX_CHECK_SUP(rows <= 65535, "too many query rows");
-  const dim3 grid(a->heads, (unsigned)rows);
-  if (a->cache.head_dim == 128)
-    kv4_attn_simple_kernel<128><<<grid, 128, 0, stream>>>(p);
-  else
-    kv4_attn_simple_kernel<64><<<grid, 128, 0, stream>>>(p);
-  return cuda_status(cudaGetLastError(), "kv4_attn launch");
+  LBX_CHECK_ARG(aligned16(a->out), "out must be 16-byte aligned");
+  const size_t need = lbx_kv4_attn_workspace_size(a);
+  LBX_CHECK_ARG(ws && ws_bytes >= need, "workspace too small (%zu < %zu)", ws_bytes, need);
+  LBX_CHECK_ARG(aligned16(ws), "the workspace must be 16-byte aligned");
+  return a->cache.head_dim == 128 ? kv4_attn_launch<128>(p, ws, a->use_pdl != 0, stream)
+                                  : kv4_attn_launch<64>(p, ws, a->use_pdl != 0, stream);
 }
