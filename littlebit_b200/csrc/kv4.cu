@@ -162,33 +162,42 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 // s_ij = q_i . k_j (q scaled by scale * log2 e), one pass with the running maximum.
 //
 // Both products run on the tensor cores (mma.m16n8k16, fp16 in, fp32 sums)
-// straight from the packed codes.  Keys: a code c in the low bits of a 16-bit lane IS
-// the fp16 subnormal c * 2^-24, which the tensor cores multiply exactly, so a pair
-// of codes costs one AND (and every second pair a shift, nibbles 1 and 3 being left
-// at 16 times their value).  With step and least value of a group of dimensions
-// outside the sum,
+// straight from the packed codes.  With step and least value of a group of
+// dimensions outside the sum,
 //
-//   q . k = sum_g [ step_g (sum_{d in g} q_d c_d) + least_g (sum_{d in g} q_d) ]
+//   q . k = sum_g [ step_g (sum_{d in g} q_d (c_d - 8)) + (least_g + 8 step_g) (sum_{d in g} q_d) ]
 //   o_d   = sum_j (p_j step_jg) (c_jd - 8) + sum_j p_j (least_jg + 8 step_jg)
 //
-// so codes enter as they are stored and only the queries and p * step are
-// rounded to fp16.  The values' codes are centred first (one subtraction a pair): the
-// tensor cores round their sums towards zero, and over thousands of slots of one
-// sign that showed (4e-5 of the result at 4000 slots, 6e-4 at 130 000).  Queries and p * step are
-// brought to [2^14, 2^15) by a power of two (a query by its group's largest, p * step
-// by the largest step the row has seen).
-// float32 (SPLIT): rows 0-7 of the MMA hold the leading 11 bits and rows 8-15 the
-// next 11 of the same eight query rows: 22 bits, float32's own error.
-// bfloat16: 16 query rows (H2) or 8, 11 bits against the result's 8.
+// only the queries and p * step are rounded to fp16; they are brought to
+// [2^14, 2^15) by a power of two first (a query by its group's largest, p * step by the
+// largest step the row has seen).  A pair of codes becomes fp16 by two logic
+// operations at most and one exact subtraction.  Codes are centred because the
+// tensor cores round their sums towards zero, and sums of one sign drift: 4e-5 of the
+// result at 4000 slots, 6e-4 at 130 000, against 3e-7 and 5e-6.  The keys of bfloat16 calls
+// (64 terms a sum, drift 1e-6) keep c: in the low bits of a 16-bit lane it IS the
+// fp16 subnormal c * 2^-24, which the tensor cores multiply exactly.  Nibbles 1 and 3 are left
+// at 16 times their value.
+// Codes are the A operand (16 slots x 16 dimensions of the keys, 16 dimensions x 16
+// slots of the values) and query rows the columns of B, eight to a column tile, so that
+// a decode step's few rows waste half a tile at most, the running sums take
+// D / 16 x 4 registers a column tile, and NT column tiles share the unpacked codes.
+// The weights reach B's layout by one 8 x 8 transposition (movmatrix) a tile.
+// (Rows as A measured 500 instructions per 16 slots, half of them moves and masks; this
+// form is half that, which is what bounds the kernel: 6.5 TB/s is 400 issue slots per 16
+// slots of 128-wide keys and values.)
+// float32 calls (SPLIT) take each query and weight in two fp16 terms, 22 bits;
+// bfloat16 ones in one, 11 bits against the result's 8.
 //
-// Work: a warp takes one sub-chunk of CK slots for one tile of query rows, 32
-// slots a step, and leaves (m, l, o) to be merged in sub-chunk order; the row
-// tiles of a block share the ring of bulk copies.  Sub-chunks and steps lie at
+// Work: a warp takes a run of sub-chunks of ck slots for one tile of query rows, 32
+// slots a step, and leaves each sub-chunk's (m, l, o) to be merged in order; the
+// row tiles of a block share the ring of bulk copies.  Sub-chunks and steps lie at
 // fixed slots and a row's arithmetic involves no other row, so its bits do not
 // depend on what else the call holds.
 // ---------------------------------------------------------------------------
-constexpr int KA_STEP = 32;     // slots a step (one stage of the ring)
-constexpr int KA_ST = 4;        // stages
+constexpr int KA_STEP = 32;     // slots a step of the softmax
+constexpr int KA_SLOTS = 64;    // slots a stage of the ring
+constexpr int KA_ST = 2;        // stages
+constexpr float KA_LAZY = 8.f;  // a row's reference moves when its maximum is 2^8 above it
 constexpr int KA_WARPS = 4;     // warps a block at most
 
 struct Kv4AttnParams {
@@ -196,7 +205,8 @@ struct Kv4AttnParams {
   int n, heads, rep, max_prefix, dtype;
   int i0, R;           // first token of this launch's rows, query rows of a kv head
   int ck, nsub;        // slots a sub-chunk, sub-chunks of the longest sequence
-  int kw, rw, ntile;   // sub-chunks and row tiles a block, row tiles in all
+  int kw, rw, ntile;   // warps' runs and row tiles a block, row tiles in all
+  int cpw;             // sub-chunks a warp's run
   float scale;         // times log2 e
   const int32_t *prefix;
   const void *q; int64_t q_ld;
@@ -207,11 +217,21 @@ struct Kv4AttnParams {
   float2 *part_ml;     // [n_seq][kvh][nsub][R]
 };
 
-LBX_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+// d[16 x 8] (+)= a[16 x 16] b[16 x 8]
+LBX_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+LBX_DEV void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+LBX_DEV uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 LBX_DEV uint32_t f16x2(float lo, float hi) {
   uint32_t r;
@@ -223,17 +243,34 @@ LBX_DEV uint32_t f16x2_rest(uint32_t r, float lo, float hi) {
   const __half2 h = *reinterpret_cast<const __half2 *>(&r);
   return f16x2(lo - __low2float(h), hi - __high2float(h));
 }
-// exponent of |x| <- its bits, within what the power-of-two factors below reach
+// exponent of |x| <- its bits, within what the power-of-two factors reach
 LBX_DEV int kv4_exp(uint32_t bits) { return min(max((int)(bits >> 23) - 127, -112), 100); }
-LBX_DEV float kv4_up(int e) { return __uint_as_float((uint32_t)(141 - e) << 23); }    // 2^(14 - e)
-LBX_DEV float kv4_down(int e) { return __uint_as_float((uint32_t)(113 + e) << 23); }  // 2^(e - 14)
+LBX_DEV float kv4_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// The masks of the unpacking, in registers: with both a mask and bits to set,
+// immediates would make two instructions of each.
+struct Kv4Masks {
+  uint32_t m0, m1, one;
+  LBX_DEV Kv4Masks() {
+    asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(m0));
+    asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(m1));
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(one));
+  }
+};
 // codes in bits 4 N .. 4 N + 3 of both halves -> 16^N (code - 8) as fp16: 1024 + 16^N code by
 // its bits, less 1024 + 8 * 16^N, both exact
 template <int N>
-LBX_DEV uint32_t kv4_mid(uint32_t x) {
-  const uint32_t v = (x & (N ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u, off = N ? 0x64806480u : 0x64086408u;
+LBX_DEV uint32_t kv4_mid(const Kv4Masks &k, uint32_t x) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(x), "r"(N ? k.m1 : k.m0), "r"(k.one));  // (x & mask) | one
+  const uint32_t off = N ? 0x64806480u : 0x64086408u;
   const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&off));
   return *reinterpret_cast<const uint32_t *>(&d);
+}
+// a pair of the keys' codes: centred, or as the subnormals 2^-24 code
+template <bool MID, int N>
+LBX_DEV uint32_t kv4_kcode(const Kv4Masks &k, uint32_t x) {
+  if constexpr (MID) return kv4_mid<N>(k, x);
+  return x & (N ? 0x00F000F0u : 0x000F000Fu);
 }
 LBX_DEV float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -242,6 +279,17 @@ LBX_DEV float quad_max(float v) {
 LBX_DEV float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// over the eight lanes of one j
+LBX_DEV float col_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+LBX_DEV float col_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 LBX_DEV float ex2(float x) {
   float r;
@@ -261,9 +309,20 @@ LBX_DEV bool kv4_sees(int j, int prefix, int n, int i, bool tree, uint64_t mask)
 // columns 0, 2, 4, 6 in turn (the value rows a warp reads together)
 LBX_DEV int kv4_key(int rho) { return rho ^ ((rho >> 1) & 1); }
 
+template <int NG>
+LBX_DEV void kv4_params(const uint32_t *a, uint32_t (&pp)[NG]) {
+  if constexpr (NG == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(a);
+    pp[0] = v.x;
+    pp[1] = v.y;
+  } else {
+    pp[0] = *a;
+  }
+}
+
 template <int D>
 struct Kv4Stage {
-  static constexpr int CB = KA_STEP * D / 2, PB = KA_STEP * (D / KV4_G) * 4;  // bytes of codes, of params
+  static constexpr int CB = KA_SLOTS * D / 2, PB = KA_SLOTS * (D / KV4_G) * 4;  // bytes of codes, of params
   static constexpr int BYTES = 2 * (CB + PB);
 };
 
@@ -298,10 +357,10 @@ LBX_DEV void kv4_load_q(const Kv4AttnParams &p, int64_t row, int hq, int j, bool
   for (int i = 0; i < D / 4; ++i) x[i] *= p.scale;
 }
 
-template <int D, bool SPLIT, bool H2>
-__global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
-  constexpr int NG = D / KV4_G, NW = D / 32, NH = H2 ? 2 : 1;
-  constexpr int RT = H2 ? 16 : 8;  // query rows a tile
+template <int D, bool SPLIT, int NT>
+__global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int NG = D / KV4_G, NW = D / 32, NS = SPLIT ? 2 : 1;
+  constexpr int RT = 8 * NT;  // query rows a tile
   using Stage = Kv4Stage<D>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[KA_WARPS][KA_ST], empty[KA_WARPS][KA_ST];
@@ -310,7 +369,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
   const int kg = warp / p.rw, rt = warp - kg * p.rw;  // this warp's sub-chunk and row tile in the block
   const int rgroups = (p.ntile + p.rw - 1) / p.rw;
   const int cblk = blockIdx.x / rgroups, rg = blockIdx.x - cblk * rgroups;
-  const int c = cblk * p.kw + kg, h = blockIdx.y, s = blockIdx.z;
+  const int c0 = (cblk * p.kw + kg) * p.cpw, h = blockIdx.y, s = blockIdx.z;  // (first sub-chunk)
   volatile int *abrt = &abort_flag;
   if (tid == 0) {
     for (int g = 0; g < p.kw; ++g)
@@ -344,19 +403,20 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
   auto seen_end = [&](int tl_) {
     return prefix + (p.tree ? p.n : p.i0 + (min(p.R, (tl_ + 1) * RT) - 1) / p.rep + 1);
   };
-  const int lo = c * p.ck;
-  const int hi_blk = min(lo + p.ck, seen_end(tl));
-  const int nst = hi_blk > lo ? (hi_blk - lo + KA_STEP - 1) / KA_STEP : 0;
-  if (nst == 0 || c >= p.nsub) return;  // (every warp of this ring)
+  const int lo = c0 * p.ck;
+  const int run = min(p.cpw, p.nsub - c0) * p.ck;
+  const int hi_blk = run > 0 ? min(lo + run, seen_end(tl)) : 0;
+  const int nst = hi_blk > lo ? (hi_blk - lo + KA_SLOTS - 1) / KA_SLOTS : 0;
+  if (nst == 0) return;  // (every warp of this ring)
   const bool live_tile = tile < p.ntile;
-  const int my_end = live_tile ? min(lo + p.ck, seen_end(tile)) : 0;
+  const int my_end = live_tile ? min(lo + run, seen_end(tile)) : 0;
 
   uint8_t *ring = smem_raw + kg * KA_ST * Stage::BYTES;
   const int64_t base = ((int64_t)s * p.c.kvh + h) * p.c.max_seq + lo;
   auto issue = [&](int i) {  // (one lane)
     const int st = i % KA_ST;
     uint8_t *d = ring + st * Stage::BYTES;
-    const int64_t slot = base + (int64_t)i * KA_STEP;
+    const int64_t slot = base + (int64_t)i * KA_SLOTS;
     mbar_arrive_expect_tx(&full[kg][st], Stage::BYTES);
     bulk_g2s(d, p.c.kc + slot * (D / 2), Stage::CB, &full[kg][st]);
     bulk_g2s(d + Stage::CB, p.c.kp + slot * NG, Stage::PB, &full[kg][st]);
@@ -367,232 +427,252 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
   if (rt == 0 && lane == 0)
     for (; issued < KA_ST && issued < nst; ++issued) issue(issued);
 
-  // ---- the queries' fragments
-  uint32_t qa[2 * NW][4];
-  float fq[NH][NG], qs[NH][NG];
-  int qi[NH];         // token index of the row(s)
-  int64_t qrow[NH];   // its row, query head
-  int qh[NH];
-  bool rok[NH];
+  // ---- the queries' fragments: lane (r, j) makes its dimensions of row r of each
+  // column tile; as accumulator columns it owns rows 2 j and 2 j + 1
+  uint32_t qb[NT][NS][2 * NW][2];
+  float fq[NT][2], qs[NT][2][NG];  // the queries' unit, and their sums in it
+  int qi[NT][2];                   // token index of the rows
+  bool rok[NT][2];
+  const bool tree = p.tree != nullptr;
+  uint64_t mask[NT][2];
+  const int64_t qrow0 = (int64_t)s * p.n + p.i0;
 #pragma unroll
-  for (int u = 0; u < NH; ++u) {
-    const int R = tile * RT + r + 8 * u;
-    rok[u] = live_tile && R < p.R;
-    qi[u] = p.i0 + (rok[u] ? R / p.rep : 0);
-    qh[u] = h * p.rep + (rok[u] ? R % p.rep : 0);
-    qrow[u] = (int64_t)s * p.n + qi[u];
+  for (int u = 0; u < NT; ++u) {
     float x[D / 4];
-    kv4_load_q<D>(p, qrow[u], qh[u], j, rok[u], x);
+    {
+      const int R = tile * RT + 8 * u + r;
+      const bool ok = live_tile && R < p.R;
+      kv4_load_q<D>(p, qrow0 + (ok ? R / p.rep : 0), h * p.rep + (ok ? R % p.rep : 0), j, ok, x);
+    }
+    float mq = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) mq = fmaxf(mq, fabsf(x[i]));
+    const int e = kv4_exp(__float_as_uint(quad_max(mq)));
+    const float up = kv4_pow2(14 - e), unit = kv4_pow2(e - 14) * (SPLIT ? 1.f : 16777216.f);
+    float sum[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       constexpr int PER = D / 4 / NG;
-      float m = 0.f, sum = 0.f;
+      float a = 0.f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        m = fmaxf(m, fabsf(x[g * PER + i]));
-        sum += x[g * PER + i];
-      }
-      const int e = kv4_exp(__float_as_uint(quad_max(m)));
-      const float up = kv4_up(e);
-      fq[u][g] = kv4_down(e) * 16777216.f;  // (codes enter as 2^-24 of their value)
-      qs[u][g] = quad_sum(sum);
+      for (int i = 0; i < PER; ++i) a += x[g * PER + i];
+      sum[g] = quad_sum(a) * (SPLIT ? up : up * 5.9604644775390625e-8f);
+    }
 #pragma unroll
-      for (int t = g * NW / NG; t < (g + 1) * NW / NG; ++t) {
-        float y[8];
+    for (int b = 0; b < 2; ++b) {  // (from the lanes that made rows 2 j + b)
+      const int src = 4 * (2 * j + b);
+      fq[u][b] = __shfl_sync(0xffffffffu, unit, src);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[8 * t + i] * ((i & 1) ? up * 0.0625f : up);
+      for (int g = 0; g < NG; ++g) qs[u][b][g] = __shfl_sync(0xffffffffu, sum[g], src);
+      const int R = tile * RT + 8 * u + 2 * j + b;
+      rok[u][b] = live_tile && R < p.R;
+      qi[u][b] = p.i0 + (rok[u][b] ? R / p.rep : 0);
+      mask[u][b] = tree && rok[u][b] ? __ldg(p.tree + (int64_t)s * p.n + qi[u][b]) : 0ull;
+    }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // (k step 2t + k: dimensions 2k, 2k+4 and 2k+1, 2k+5 of the block)
-          const uint32_t a0 = f16x2(y[2 * k], y[2 * k + 4]), a2 = f16x2(y[2 * k + 1], y[2 * k + 5]);
-          if (SPLIT) {
-            qa[2 * t + k][0] = a0;
-            qa[2 * t + k][2] = a2;
-            qa[2 * t + k][1] = f16x2_rest(a0, y[2 * k], y[2 * k + 4]);
-            qa[2 * t + k][3] = f16x2_rest(a2, y[2 * k + 1], y[2 * k + 5]);
-          } else {
-            qa[2 * t + k][u] = a0;
-            qa[2 * t + k][2 + u] = a2;
-            if (!H2) qa[2 * t + k][1] = qa[2 * t + k][3] = 0u;
-          }
+    for (int t = 0; t < NW; ++t) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[8 * t + i] * ((i & 1) ? up * 0.0625f : up);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // (k step 2t + k: dimensions 2k, 2k+4 and 2k+1, 2k+5 of the block)
+        const uint32_t b0 = f16x2(y[2 * k], y[2 * k + 4]), b1 = f16x2(y[2 * k + 1], y[2 * k + 5]);
+        qb[u][0][2 * t + k][0] = b0;
+        qb[u][0][2 * t + k][1] = b1;
+        if constexpr (SPLIT) {
+          qb[u][1][2 * t + k][0] = f16x2_rest(b0, y[2 * k], y[2 * k + 4]);
+          qb[u][1][2 * t + k][1] = f16x2_rest(b1, y[2 * k + 1], y[2 * k + 5]);
         }
       }
     }
   }
-  const bool tree = p.tree != nullptr;
-  uint64_t mask[NH];
-#pragma unroll
-  for (int u = 0; u < NH; ++u) mask[u] = tree && rok[u] ? __ldg(p.tree + qrow[u]) : 0ull;
 
-  float o[D / 8][4];  // column tile 8 g + i: dimensions 64 g + 8 n + i
+  const Kv4Masks km;
+  float o[NT][D / 16][4];  // row tile 4 g + q: dimensions 64 g + 8 r + 2 q (+ 1: the second half), rows 2 j, 2 j + 1
+  float m[NT][2], l[NT][2], om[NT][2][NG];  // reference of the weights, their sum, sum of weight * (least + 8 step)
+  int eo[NT][2];                            // exponent of the largest step seen
+  auto reset = [&]() {
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[NH], l[NH], om[NH][NG];
-  int eo[NH];
+    for (int u = 0; u < NT; ++u) {
 #pragma unroll
-  for (int u = 0; u < NH; ++u) {
-    m[u] = -INFINITY;
-    l[u] = 0.f;
-    eo[u] = -112;
+      for (int i = 0; i < D / 16; ++i) o[u][i][0] = o[u][i][1] = o[u][i][2] = o[u][i][3] = 0.f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) om[u][g] = 0.f;
-  }
+      for (int b = 0; b < 2; ++b) {
+        m[u][b] = -INFINITY;
+        l[u][b] = 0.f;
+        eo[u][b] = -112;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) om[u][b][g] = 0.f;
+      }
+    }
+  };
+  reset();
 
-  bool ok = true;
   for (int i = 0; i < nst; ++i) {
     const int st = i % KA_ST;
-    // the stage read in the step before is free once all row tiles have read it
+    // the stage read before is free once all row tiles have read it
     if (rt == 0 && lane == 0 && i > 0 && issued < nst &&
         wd_wait(&empty[kg][(i - 1) % KA_ST], (uint32_t)((i - 1) / KA_ST) & 1u, 0x805, abrt))
       issue(issued++);
     __syncwarp();
-    if (!__all_sync(0xffffffffu, wd_wait(&full[kg][st], (uint32_t)(i / KA_ST) & 1u, 0x804, abrt))) {
-      ok = false;
-      break;
-    }
-    const int j0 = lo + i * KA_STEP;
-    if (j0 < my_end) {
-      const uint8_t *sk = ring + st * Stage::BYTES;
-      const uint32_t *skp = reinterpret_cast<const uint32_t *>(sk + Stage::CB);
+    if (!__all_sync(0xffffffffu, wd_wait(&full[kg][st], (uint32_t)(i / KA_ST) & 1u, 0x804, abrt))) break;
+#pragma unroll 1
+    for (int hs = 0; hs < KA_SLOTS; hs += KA_STEP) {
+      const int j0 = lo + i * KA_SLOTS + hs;
+      if (j0 >= my_end) break;
+      const uint8_t *sk = ring + st * Stage::BYTES + hs * (D / 2);
+      const uint32_t *skp = reinterpret_cast<const uint32_t *>(ring + st * Stage::BYTES + Stage::CB) + hs * NG;
       const uint8_t *sv = sk + Stage::CB + Stage::PB;
-      const uint32_t *svp = reinterpret_cast<const uint32_t *>(sv + Stage::CB);
-      // ---- scores: sc[u][2 t + k], column tile t, this lane's slot kv4_key(2 j + k) of its eight
-      float sc[NH][8];
+      const uint32_t *svp = skp + (Stage::CB + Stage::PB) / 4;
+      // ---- scores in the queries' unit: sc[u][2 a + k][b], slot 16 a + 8 k + kv4_key(r), row 2 j + b
+      float sc[NT][4][2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        uint32_t w[NW];
-        const uint8_t *kr = sk + (8 * t + kv4_key(r)) * (D / 2) + j * (D / 8);
-        if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(kr);
-          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2 *>(kr);
-          w[0] = v.x; w[1] = v.y;
+      for (int a = 0; a < 2; ++a) {
+        uint32_t w[2][NW];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint8_t *kr = sk + (16 * a + 8 * k + kv4_key(r)) * (D / 2) + j * (D / 8);
+          if constexpr (D == 128) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(kr);
+            w[k][0] = v.x; w[k][1] = v.y; w[k][2] = v.z; w[k][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(kr);
+            w[k][0] = v.x; w[k][1] = v.y;
+          }
         }
-        float acc[NG][4];
+        float acc[NT][NG][4];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
+        for (int q = 0; q < 2 * NW; ++q) {
+          const uint32_t w0 = (q & 1) ? w[0][q / 2] >> 8 : w[0][q / 2], w1 = (q & 1) ? w[1][q / 2] >> 8 : w[1][q / 2];
+          const uint32_t a0 = kv4_kcode<SPLIT, 0>(km, w0), a1 = kv4_kcode<SPLIT, 0>(km, w1);
+          const uint32_t a2 = kv4_kcode<SPLIT, 1>(km, w0), a3 = kv4_kcode<SPLIT, 1>(km, w1);
 #pragma unroll
-        for (int q = 0; q < NW; ++q) {
-          const uint32_t y = w[q] >> 8;
-          mma_f16(acc[q * NG / NW], qa[2 * q], w[q] & 0x000F000Fu, w[q] & 0x00F000F0u);
-          mma_f16(acc[q * NG / NW], qa[2 * q + 1], y & 0x000F000Fu, y & 0x00F000F0u);
+          for (int u = 0; u < NT; ++u) {
+            float (&d)[4] = acc[u][q * NG / (2 * NW)];
+            if (q % (2 * NW / NG) == 0) mma_f16_first(d, a0, a1, a2, a3, qb[u][0][q][0], qb[u][0][q][1]);
+            else mma_f16(d, a0, a1, a2, a3, qb[u][0][q][0], qb[u][0][q][1]);
+            if constexpr (SPLIT) mma_f16(d, a0, a1, a2, a3, qb[u][1][q][0], qb[u][1][q][1]);
+          }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t *pr = skp + (8 * t + kv4_key(2 * j + k)) * NG;
-#pragma unroll
-          for (int u = 0; u < NH; ++u) sc[u][2 * t + k] = 0.f;
+          uint32_t pp[NG];
+          kv4_params<NG>(skp + (16 * a + 8 * k + kv4_key(r)) * NG, pp);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const uint32_t pp = pr[g];
+            const float sg = kv4_step(pp[g]), lg = SPLIT ? fmaf(8.f, sg, kv4_least(pp[g])) : kv4_least(pp[g]);
 #pragma unroll
-            for (int u = 0; u < NH; ++u) {
-              const float a = SPLIT ? acc[g][k] + acc[g][2 + k] : acc[g][2 * u + k];
-              sc[u][2 * t + k] = fmaf(a, kv4_step(pp) * fq[u][g], fmaf(kv4_least(pp), qs[u][g], sc[u][2 * t + k]));
-            }
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                float &x = sc[u][2 * a + k][b];
+                x = fmaf(acc[u][g][2 * k + b], sg, g == 0 ? lg * qs[u][b][g] : fmaf(lg, qs[u][b][g], x));
+              }
           }
         }
       }
-      // ---- what each row sees of the step; the values' steps, theirs to be kept within fp16
+      // ---- the values' params of this lane's slots; what each row sees of the step
       const bool whole = j0 + KA_STEP <= prefix;
-      float stp[8][NG], lst[8][NG];
+      float sg[4][NG], lg[4][NG];
+      float sx[NT][2];
+      {
+        float a = 0.f;
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const uint32_t *pr = svp + (8 * (t >> 1) + kv4_key(2 * j + (t & 1))) * NG;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t pp = pr[g];
-          stp[t][g] = kv4_step(pp);
-          lst[t][g] = fmaf(8.f, stp[t][g], kv4_least(pp));
-        }
-      }
-      uint32_t vis[NH];
-#pragma unroll
-      for (int u = 0; u < NH; ++u) {
-        vis[u] = 0xFFu;
-        if (!whole) {
-          vis[u] = 0u;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            if (rok[u] && kv4_sees(j0 + 8 * (t >> 1) + kv4_key(2 * j + (t & 1)), prefix, p.n, qi[u], tree, mask[u]))
-              vis[u] |= 1u << t;
-            else
-              sc[u][t] = -INFINITY;
-          }
-        }
-      }
-      float f[NH];
-      bool change = false;
-      float al[NH];
-#pragma unroll
-      for (int u = 0; u < NH; ++u) {
-        float mx = sc[u][0], sx = 0.f;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          mx = fmaxf(mx, sc[u][t]);
+        for (int t = 0; t < 4; ++t) {
+          uint32_t pp[NG];
+          kv4_params<NG>(svp + (8 * t + kv4_key(r)) * NG, pp);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const float a = fabsf(stp[t][g]);
-            if ((whole || (vis[u] >> t & 1u)) && a < INFINITY) sx = fmaxf(sx, a);
+            sg[t][g] = kv4_step(pp[g]);
+            lg[t][g] = fmaf(8.f, sg[t][g], kv4_least(pp[g]));
+            a = fmaxf(a, fabsf(sg[t][g]));  // (a NaN is passed over)
           }
         }
-        mx = fmaxf(quad_max(mx), m[u]);
-        const int e = max(kv4_exp(__float_as_uint(quad_max(sx))), eo[u]);
-        const bool ch = mx > m[u] || e > eo[u];
-        change |= ch;
-        // (nothing seen so far: any finite reference gives weights 0)
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        al[u] = m[u] == -INFINITY ? 0.f : ex2(m[u] - ref);
-        l[u] *= al[u];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) om[u][g] *= al[u];
-        al[u] *= __uint_as_float((uint32_t)(127 + max(eo[u] - e, -126)) << 23);
-        m[u] = mx;
-        eo[u] = e;
-        f[u] = kv4_up(e);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) sc[u][t] = ex2(sc[u][t] - ref);
+        for (int u = 0; u < NT; ++u) sx[u][0] = sx[u][1] = a;
       }
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            float a = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              if (rok[u][b] && kv4_sees(j0 + 8 * t + kv4_key(r), prefix, p.n, qi[u][b], tree, mask[u][b])) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                  a = fmaxf(a, fabsf(sg[t][g]));
+                  // what is not a number reaches the rows that see it, and (below) no other
+                  if (!(fabsf(lg[t][g]) < INFINITY)) om[u][b][g] += __uint_as_float(0x7FC00000u);
+                }
+              } else {
+                sc[u][t][b] = -INFINITY;
+              }
+            }
+            sx[u][b] = a;
+          }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            if (!(fabsf(lg[t][g]) < INFINITY)) sg[t][g] = lg[t][g] = 0.f;
+      }
+      // ---- references: a row's moves when its maximum is 2^8 above it (or a step is above all before)
+      bool change = false;
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float a = fmaxf(fmaxf(sc[u][0][b], sc[u][1][b]), fmaxf(sc[u][2][b], sc[u][3][b]));
+          change |= a * fq[u][b] > m[u][b] + KA_LAZY || kv4_exp(__float_as_uint(sx[u][b])) > eo[u][b];
+        }
       if (__any_sync(0xffffffffu, change)) {
 #pragma unroll
-        for (int t = 0; t < D / 8; ++t) {
-          o[t][0] *= al[0];
-          o[t][1] *= al[0];
-          o[t][2] *= al[NH - 1];
-          o[t][3] *= al[NH - 1];
-        }
-      }
-      // ---- values, 16 slots an MMA step: slots of column tiles 2 a (first eight) and 2 a + 1
+        for (int u = 0; u < NT; ++u) {
+          float al[2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        uint32_t pa[NG][4];
+          for (int b = 0; b < 2; ++b) {
+            const float mx =
+                col_max(fmaxf(fmaxf(sc[u][0][b], sc[u][1][b]), fmaxf(sc[u][2][b], sc[u][3][b]))) * fq[u][b];
+            const int e = max(kv4_exp(__float_as_uint(col_max(sx[u][b]))), eo[u][b]);
+            const float mn = mx > m[u][b] + KA_LAZY ? mx : m[u][b];
+            al[b] = mn == m[u][b] ? 1.f : ex2(m[u][b] - mn);  // (from -inf: 0)
+            l[u][b] *= al[b];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
+            for (int g = 0; g < NG; ++g) om[u][b][g] *= al[b];
+            al[b] *= kv4_pow2(max(eo[u][b] - e, -126));
+            m[u][b] = mn;
+            eo[u][b] = e;
+          }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int t = 4 * a + 2 * hf;
-#pragma unroll
-            for (int u = 0; u < NH; ++u) {
-              float x0 = sc[u][t] * f[u] * stp[t][g], x1 = sc[u][t + 1] * f[u] * stp[t + 1][g];
-              float y0 = sc[u][t] * lst[t][g], y1 = sc[u][t + 1] * lst[t + 1][g];
-              if (!whole) {  // (a stale step may be NaN)
-                if (!(vis[u] >> t & 1u)) x0 = y0 = 0.f;
-                if (!(vis[u] >> (t + 1) & 1u)) x1 = y1 = 0.f;
-              }
-              om[u][g] += y0 + y1;
-              const uint32_t hi = f16x2(x0, x1);
-              if (SPLIT) {
-                pa[g][2 * hf] = hi;
-                pa[g][2 * hf + 1] = f16x2_rest(hi, x0, x1);
-              } else {
-                pa[g][2 * hf + u] = hi;
-                if (!H2) pa[g][2 * hf + 1] = 0u;
-              }
-            }
+          for (int t = 0; t < D / 16; ++t) {
+            o[u][t][0] *= al[0];
+            o[u][t][1] *= al[1];
+            o[u][t][2] *= al[0];
+            o[u][t][3] *= al[1];
           }
         }
+      }
+      // ---- weights (at most 2^8; with a step below 2^(eo + 1), times f, below 2^15), then 16 slots an MMA step
 #pragma unroll
-        for (int u = 0; u < NH; ++u) l[u] += (sc[u][4 * a] + sc[u][4 * a + 1]) + (sc[u][4 * a + 2] + sc[u][4 * a + 3]);
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float ref = m[u][b] == -INFINITY ? 0.f : m[u][b];  // (nothing seen so far: weights 0)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) sc[u][t][b] = ex2(fmaf(sc[u][t][b], fq[u][b], -ref));
+          l[u][b] += (sc[u][0][b] + sc[u][1][b]) + (sc[u][2][b] + sc[u][3][b]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) om[u][b][g] = fmaf(sc[u][t][b], lg[t][g], om[u][b][g]);
+          const float f = kv4_pow2(6 - eo[u][b]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) sc[u][t][b] *= f;
+        }
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
         uint32_t vw[4][NG];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -607,68 +687,84 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
+          uint32_t pb[NT][NS][2];
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float x0 = sc[u][2 * a + k][0] * sg[2 * a + k][g], x1 = sc[u][2 * a + k][1] * sg[2 * a + k][g];
+              const uint32_t hi = f16x2(x0, x1);
+              pb[u][0][k] = transpose8(hi);
+              if constexpr (SPLIT) pb[u][1][k] = transpose8(f16x2_rest(hi, x0, x1));
+            }
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {  // nibbles 0-3, 4-7 of the word
             uint32_t b0 = __byte_perm(vw[0][g], vw[1][g], hf ? 0x7632 : 0x5410);
             uint32_t b1 = __byte_perm(vw[2][g], vw[3][g], hf ? 0x7632 : 0x5410);
-            mma_f16(o[8 * g + 4 * hf], pa[g], kv4_mid<0>(b0), kv4_mid<0>(b1));
-            mma_f16(o[8 * g + 4 * hf + 1], pa[g], kv4_mid<1>(b0), kv4_mid<1>(b1));
-            b0 >>= 8;
-            b1 >>= 8;
-            mma_f16(o[8 * g + 4 * hf + 2], pa[g], kv4_mid<0>(b0), kv4_mid<0>(b1));
-            mma_f16(o[8 * g + 4 * hf + 3], pa[g], kv4_mid<1>(b0), kv4_mid<1>(b1));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t a0 = kv4_mid<0>(km, b0), a1 = kv4_mid<1>(km, b0), a2 = kv4_mid<0>(km, b1), a3 = kv4_mid<1>(km, b1);
+#pragma unroll
+              for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < NS; ++e) mma_f16(o[u][4 * g + 2 * hf + q], a0, a1, a2, a3, pb[u][e][0], pb[u][e][1]);
+              b0 >>= 8;
+              b1 >>= 8;
+            }
           }
         }
       }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive1(&empty[kg][st]);
+    const int j1 = lo + (i + 1) * KA_SLOTS;
+    if ((j1 % p.ck != 0 && i + 1 < nst) || (j1 - 1) / p.ck * p.ck >= my_end) continue;
+
+    // ---- the sub-chunk's (m, l, o): lane (r, j) holds dimensions 64 g + 8 r .. + 7 of rows 2 j, 2 j + 1
+    const int c = (j1 - 1) / p.ck;
+    const bool single = p.nsub == 1;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float lsum = col_sum(l[u][b]);
+        float oms[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) oms[g] = col_sum(om[u][b][g]);
+        if (!rok[u][b]) continue;
+        const int R = tile * RT + 8 * u + 2 * j + b;
+        const float dn = kv4_pow2(eo[u][b] - 6);
+        const int64_t pr = (((int64_t)s * p.c.kvh + h) * p.nsub + c) * p.R + R;
+        const int64_t od = (((int64_t)s * p.n + qi[u][b]) * p.heads + h * p.rep + R % p.rep) * D;
+        if (!single && r == 0) p.part_ml[pr] = make_float2(m[u][b], lsum);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float v[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            v[q] = fmaf(o[u][4 * g + q / 2][2 * (q & 1) + b], (q & 1) ? dn * 0.0625f : dn, oms[g]);
+            if (single) v[q] = lsum == 0.f ? 0.f : v[q] / lsum;  // (as the merge of one sub-chunk)
+          }
+          const int d = 64 * g + 8 * r;
+          if (!single || p.dtype == LBX_F32) {
+            float *dst = single ? reinterpret_cast<float *>(p.out) + od + d : p.part_o + pr * D + d;
+            reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              w[q] = (uint32_t)f32_to_bf16(v[2 * q]) | (uint32_t)f32_to_bf16(v[2 * q + 1]) << 16;
+            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.out) + od + d) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    reset();
   }
   if (rt == 0 && lane == 0 && *abrt) {  // copies in flight land before shared memory is given up
     int none = 0;
     for (int i = max(0, issued - KA_ST); i < issued; ++i)
       wd_wait(&full[kg][i % KA_ST], (uint32_t)(i / KA_ST) & 1u, 0x806, &none);
-  }
-  if (!ok || my_end <= lo) return;
-
-  // ---- this row's (m, l, o): lane (r, j) holds dimensions 64 g + 16 j .. + 15
-  const bool single = p.nsub == 1;
-#pragma unroll
-  for (int u = 0; u < NH; ++u) {
-    const float lsum = quad_sum(l[u]);
-    float oms[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) oms[g] = quad_sum(om[u][g]);
-    if (!rok[u]) continue;
-    const int R = tile * RT + r + 8 * u;
-    const float dn = kv4_down(eo[u]);
-    const int64_t pr = (((int64_t)s * p.c.kvh + h) * p.nsub + c) * p.R + R;
-    if (!single && j == 0) p.part_ml[pr] = make_float2(m[u], lsum);
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = SPLIT ? o[8 * g + i][k] + o[8 * g + i][2 + k] : o[8 * g + i][2 * u + k];
-          v[i] = fmaf(a, (i & 1) ? dn * 0.0625f : dn, oms[g]);
-          if (single) v[i] = lsum == 0.f ? 0.f : v[i] / lsum;  // (as the merge of one sub-chunk)
-        }
-        const int d = 64 * g + 8 * (2 * j + k);
-        if (!single || p.dtype == LBX_F32) {
-          float *dst = single ? reinterpret_cast<float *>(p.out) + (qrow[u] * p.heads + qh[u]) * D + d : p.part_o + pr * D + d;
-          reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-          uint16_t *dst = reinterpret_cast<uint16_t *>(p.out) + (qrow[u] * p.heads + qh[u]) * D + d;
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | (uint32_t)f32_to_bf16(v[2 * i + 1]) << 16;
-          *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
   }
 }
 
@@ -865,9 +961,10 @@ static int kv4_attn_launch(Kv4AttnParams p, void *ws, bool pdl, cudaStream_t str
   static DevCache<int> attr;
   int unused = 0;
   int rc = attr.get(unused, [](int &) {
-    cudaError_t e = allow_max_smem(kv4_attn_kernel<D, true, false>);
-    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, false>);
-    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, true>);
+    cudaError_t e = allow_max_smem(kv4_attn_kernel<D, true, 1>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, true, 2>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, 1>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, 2>);
     return cuda_status(e, "kv4_attn smem attribute");
   });
   if (rc) return rc;
@@ -876,23 +973,28 @@ static int kv4_attn_launch(Kv4AttnParams p, void *ws, bool pdl, cudaStream_t str
     p.i0 = i0;
     p.R = nt * p.rep;
     p.nsub = (p.max_prefix + (p.tree ? p.n : i0 + nt) + p.ck - 1) / p.ck;
-    const bool h2 = !split && p.R > 8;
-    p.ntile = (p.R + (h2 ? 15 : 7)) / (h2 ? 16 : 8);
+    const bool two = p.R > 8;  // column tiles a warp: two share the unpacked codes
+    p.ntile = (p.R + (two ? 15 : 7)) / (two ? 16 : 8);
     // row tiles a block, evenly; the warps left take further sub-chunks
     const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
     p.rw = (p.ntile + groups - 1) / groups;
-    p.kw = std::min(KA_WARPS / p.rw, p.nsub);
+    // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
+    // queries' fragments (1500 instructions) are made once for all of them
+    const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
+    p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (36 * device_sm_count())));
+    const int runs = (p.nsub + p.cpw - 1) / p.cpw;
+    p.kw = std::min(KA_WARPS / p.rw, runs);
     p.part_ml = reinterpret_cast<float2 *>(ws);
     const int64_t rows = (int64_t)p.c.n_seq * p.c.kvh * p.nsub * p.R;
     p.part_o = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(ws) + ((rows * 8 + 255) & ~(int64_t)255));
-    const int64_t gx = (int64_t)((p.nsub + p.kw - 1) / p.kw) * ((p.ntile + p.rw - 1) / p.rw);
+    const int64_t gx = (int64_t)((runs + p.kw - 1) / p.kw) * ((p.ntile + p.rw - 1) / p.rw);
     LBX_CHECK_SUP(gx <= 0x7fffffff && p.c.kvh <= 65535 && p.c.n_seq <= 65535, "too many heads, sequences or rows");
     const dim3 grid((unsigned)gx, p.c.kvh, p.c.n_seq), block(32 * p.kw * p.rw);
     const size_t smem = (size_t)p.kw * KA_ST * Kv4Stage<D>::BYTES;
     const bool dep = pdl || i0 > 0;  // (every kernel here waits for the one before it)
-    const cudaError_t e = split ? launch(kv4_attn_kernel<D, true, false>, grid, block, smem, stream, dep, p)
-                          : h2  ? launch(kv4_attn_kernel<D, false, true>, grid, block, smem, stream, dep, p)
-                                : launch(kv4_attn_kernel<D, false, false>, grid, block, smem, stream, dep, p);
+    auto go = [&](auto kern) { return launch(kern, grid, block, smem, stream, dep, p); };
+    const cudaError_t e = split ? (two ? go(kv4_attn_kernel<D, true, 2>) : go(kv4_attn_kernel<D, true, 1>))
+                                : (two ? go(kv4_attn_kernel<D, false, 2>) : go(kv4_attn_kernel<D, false, 1>));
     rc = cuda_status(e, "kv4_attn launch");
     if (rc) return rc;
     if (p.nsub > 1) {
