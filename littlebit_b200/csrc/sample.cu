@@ -3,6 +3,8 @@
 // softmax(draft / T); draft i is accepted while u_i < min(1, p_i(d_i) /
 // max(q_i(d_i), 1e-10)); then argmax_v r_v / e_v with r the positive part of
 // p_a - q_a, or p_k.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace lbx {
@@ -21,127 +23,293 @@ struct AcceptParams {
   int64_t *next;
 };
 
-// (NaN counts as -inf)
-LBX_DEV float logit_at(const void *p, int dtype, int64_t i) {
-  const float x = load_act(p, dtype, i);
-  return x == x ? x : -INFINITY;
+// One cluster of AC_C blocks a sequence, each with a slice of the vocabulary, in one
+// launch: the statistics of all rows at once (a warp takes 1024 logits of one
+// row at a time, eight 16-byte loads a lane in flight), joined over the cluster's shared
+// memory; every block then makes the same decisions and takes its slice of the
+// drawing.  All rows are read before the first decision is known: deciding row
+// by row would read fewer of them and wait for the cluster once a draft.
+// Bound by memory for many sequences, by three round trips to it and two cluster barriers
+// for one.
+constexpr int AC_T = 256;    // threads
+constexpr int AC_C = 8;      // blocks a sequence
+constexpr int AC_SUB = 16;   // parts of a row's slice at most
+constexpr int AC_Q = 8;      // quads of logits a lane loads together
+constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
+
+// Logits 4 q .. 4 q + 3 of a row of V (NaN and what is past V count as -inf).
+// VEC: the row starts on 16 (fp32) or 8 (bf16) bytes.
+template <int DT>
+LBX_DEV bool ac_aligned(const void *row) { return (reinterpret_cast<uintptr_t>(row) & (DT == LBX_F32 ? 15u : 7u)) == 0; }
+template <int DT>
+LBX_DEV float4 ac_quad(const void *row, bool vec, int q, int V) {
+  float v[4];
+  if (vec && 4 * q + 3 < V) {
+    if constexpr (DT == LBX_F32) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(row) + q);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row) + q);
+      v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xFFFF0000u);
+      v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 4 * q + i < V ? load_act(row, DT, 4 * (int64_t)q + i) : -INFINITY;
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
-// weight of a logit against its row's maximum m: exp((x - m) / T), 1 at the
-// maximum (an infinite one too), 0 for -inf
-LBX_DEV float logit_weight(float x, float m, float T) {
-  return x == m ? 1.f : expf((x - m) / T);
+LBX_DEV float ac_num(float x) { return x == x ? x : -INFINITY; }
+LBX_DEV float ac_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// weight of a logit against its row's maximum m: 2^((x - m) c), c = log2(e) / T;
+// 1 at the maximum (an infinite one too)
+LBX_DEV float ac_weight(float x, float m, float c) { return x == m ? 1.f : ac_ex2((x - m) * c); }
+// the larger value first, then the lower index
+LBX_DEV uint64_t ac_key(float x, uint32_t i) {
+  const uint32_t b = __float_as_uint(x);
+  return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
+}
+LBX_DEV uint64_t warp_max64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor_sync(0xffffffffu, (unsigned long long)v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+// (maximum, sum of weights against it) of two parts of a row
+LBX_DEV float2 ac_join(float2 a, float2 b, float c) {
+  const float m = fmaxf(a.x, b.x);
+  if (m == -INFINITY) return make_float2(m, 0.f);
+  return make_float2(m, a.y * ac_weight(a.x, m, c) + b.y * ac_weight(b.x, m, c));
 }
 
-constexpr int AC_THREADS = 512;
-
-__global__ void __launch_bounds__(AC_THREADS) accept_simple_kernel(const __grid_constant__ AcceptParams p) {
-  __shared__ float rf[AC_THREADS / 32];
-  __shared__ unsigned long long ru[AC_THREADS / 32];
-  const int s = blockIdx.x, tid = threadIdx.x, V = p.vocab;
-  const float T = p.temps ? p.temps[s] : p.temperature;
+template <int DT>
+__global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__ AcceptParams p) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cl = cg::this_cluster();
+  constexpr int ES = DT == LBX_F32 ? 4 : 2;
+  __shared__ uint64_t part[AC_ROWS][AC_SUB];  // of this block's slices: (max, sum) pairs, or keys (greedy)
+  __shared__ uint64_t mine[AC_ROWS], tot[AC_ROWS];
+  __shared__ uint64_t best[2][AC_C];          // every block's, in the first block
+  __shared__ uint64_t wbest[AC_T / 32];
+  __shared__ int rejected;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int s = blockIdx.x / AC_C, rank = (int)cl.block_rank(), V = p.vocab;
+  pdl_trigger();
+  pdl_wait();
+  const float T = p.temps ? __ldg(p.temps + s) : p.temperature;
   const bool greedy = !(T > 0.f);
-  auto bmax = [&](float v) {
-    v = warp_max(v);
-    __syncthreads();
-    if ((tid & 31) == 0) rf[tid >> 5] = v;
-    __syncthreads();
-    float m = rf[0];
-    for (int i = 1; i < AC_THREADS / 32; ++i) m = fmaxf(m, rf[i]);
-    return m;
-  };
-  auto bsum = [&](float v) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((tid & 31) == 0) rf[tid >> 5] = v;
-    __syncthreads();
-    float m = rf[0];
-    for (int i = 1; i < AC_THREADS / 32; ++i) m += rf[i];
-    return m;
-  };
-  // largest value first, then the lowest index; values >= 0
-  auto bbest = [&](unsigned long long v) {
-    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((tid & 31) == 0) ru[tid >> 5] = v;
-    __syncthreads();
-    unsigned long long m = ru[0];
-    for (int i = 1; i < AC_THREADS / 32; ++i) m = max(m, ru[i]);
-    return m;
-  };
-  auto first_max = [&](const void *row, int64_t off, float m) {
-    unsigned long long b = 0;
-    for (int v = tid; v < V; v += AC_THREADS)
-      if (m > -INFINITY && logit_at(row, p.dtype, off + v) == m) b = max(b, (unsigned long long)(0xffffffffu - v));
-    return bbest(b);
-  };
-  // (max, sum of weights, first maximum's index) of a row; sum 0: no probability
-  auto stats = [&](const void *row, int64_t off, float &m, float &l, int &at) {
-    float x = -INFINITY;
-    for (int v = tid; v < V; v += AC_THREADS) x = fmaxf(x, logit_at(row, p.dtype, off + v));
-    m = bmax(x);
-    at = -1;
-    if (m == -INFINITY) {
-      l = 0.f;
-      return;
-    }
-    if (greedy) {
-      l = 1.f;
-      at = (int)(0xffffffffu - (unsigned)first_max(row, off, m));
-      return;
-    }
-    float t = 0.f;
-    for (int v = tid; v < V; v += AC_THREADS) t += logit_weight(logit_at(row, p.dtype, off + v), m, T);
-    l = bsum(t);
-  };
-  auto prob = [&](const void *row, int64_t off, int v, float m, float l, int at) {
-    if (!(l > 0.f)) return 0.f;
-    if (greedy) return v == at ? 1.f : 0.f;
-    return logit_weight(logit_at(row, p.dtype, off + v), m, T) / l;
-  };
+  const float c = 1.4426950408889634f / T;
   int nd = p.k;
   if (p.n_draft) {
-    nd = p.n_draft[s];
+    nd = __ldg(p.n_draft + s);
     if (nd < 0 || nd > p.k) {
-      if (tid == 0) atomicCAS(&g_lbx_device_error, 0, 0x812);
+      if (rank == 0 && tid == 0) atomicCAS(&g_lbx_device_error, 0, 0x812);
       nd = min(max(nd, 0), p.k);
     }
   }
-  int a = 0;
-  float pm = 0.f, pl = 0.f, qm = 0.f, ql = 0.f;
-  int pa = -1, qa = -1;
-  int64_t po = 0, qo = 0;
-  int64_t d = -1;
-  for (;; ++a) {
-    po = s * p.target_seq + a * p.target_row;
-    stats(p.target, po, pm, pl, pa);
-    if (a >= nd) break;
-    d = p.tokens[s * p.tokens_ld + a];
-    const bool in = d >= 0 && d < V;
-    if (!in && tid == 0) atomicCAS(&g_lbx_device_error, 0, 0x811);
-    const float pd = in ? prob(p.target, po, (int)d, pm, pl, pa) : 0.f;
-    float qd = 1.f;
-    if (p.draft) {
-      qo = s * p.draft_seq + a * p.draft_row;
-      stats(p.draft, qo, qm, ql, qa);
-      qd = in ? prob(p.draft, qo, (int)d, qm, ql, qa) : 0.f;
+  const bool has_q = p.draft != nullptr && !greedy;
+  // rows 0 .. nd: the target's; nd + 1 ..: the drafts'
+  const int nrow = nd + 1 + (has_q ? nd : 0);
+  auto row_at = [&](int r) {
+    return r <= nd ? reinterpret_cast<const uint8_t *>(p.target) + (s * p.target_seq + r * p.target_row) * ES
+                   : reinterpret_cast<const uint8_t *>(p.draft) + (s * p.draft_seq + (r - nd - 1) * p.draft_row) * ES;
+  };
+  // this block's quads, and their parts (AC_SUB at most, a multiple of a warp's batch)
+  const int nq = (V + 3) / 4, per = (nq + AC_C - 1) / AC_C;
+  const int q0 = min(nq, rank * per), q1 = min(nq, q0 + per);
+  const int len = ((per + AC_SUB - 1) / AC_SUB + 32 * AC_Q - 1) / (32 * AC_Q) * (32 * AC_Q);
+  const int nsub = (per + len - 1) / len;
+
+  // what a decision needs besides the rows' statistics, on its way meanwhile
+  int64_t tok = -1;
+  float tl = -INFINITY, dl = -INFINITY, uu = 2.f;
+  if (tid < nd) {
+    tok = __ldg(p.tokens + s * p.tokens_ld + tid);
+    uu = __ldg(p.u + s * p.u_ld + tid);
+    if (tok >= 0 && tok < V) {
+      tl = ac_num(load_act(row_at(tid), DT, tok));
+      if (has_q) dl = ac_num(load_act(row_at(nd + 1 + tid), DT, tok));
+    } else if (rank == 0) {
+      atomicCAS(&g_lbx_device_error, 0, 0x811);
     }
-    if (!(p.u[s * p.u_ld + a] < fminf(pd / fmaxf(qd, 1e-10f), 1.f))) break;
   }
-  unsigned long long best = 0;
-  for (int pass = a < nd ? 0 : 1; pass < 2 && best == 0; ++pass) {
-    unsigned long long b = 0;
-    for (int v = tid; v < V; v += AC_THREADS) {
-      float r = prob(p.target, po, v, pm, pl, pa);
-      if (pass == 0) r -= p.draft ? prob(p.draft, qo, v, qm, ql, qa) : (v == d ? 1.f : 0.f);
-      if (!(r > 0.f)) continue;
-      const float sc = r / p.e[s * p.e_ld + v];
-      b = max(b, (unsigned long long)__float_as_uint(sc) << 32 | (0xffffffffu - v));
+
+  // ---- statistics of every row's slice
+  for (int t = warp; t < nrow * nsub; t += AC_T / 32) {
+    const int r = t / nsub, sub = t - r * nsub;
+    const uint8_t *row = row_at(r);
+    const bool vec = ac_aligned<DT>(row);
+    const int b0 = q0 + sub * len, b1 = min(q1, b0 + len);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    uint64_t key = 0;
+    for (int b = b0; b < b1; b += 32 * AC_Q) {
+      float4 x[AC_Q];
+#pragma unroll
+      for (int i = 0; i < AC_Q; ++i) {
+        const int q = b + 32 * i + lane;
+        x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (q < b1) x[i] = ac_quad<DT>(row, vec, q, V);
+      }
+      if (greedy) {
+#pragma unroll
+        for (int i = 0; i < AC_Q; ++i) {
+          const float v[4] = {ac_num(x[i].x), ac_num(x[i].y), ac_num(x[i].z), ac_num(x[i].w)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t k = v[e] > -INFINITY ? ac_key(v[e], (uint32_t)(4 * (b + 32 * i + lane) + e)) : 0ull;
+            key = k > key ? k : key;
+          }
+        }
+        continue;
+      }
+      float m = ml.x;  // (fmaxf passes a NaN over)
+#pragma unroll
+      for (int i = 0; i < AC_Q; ++i) m = fmaxf(m, fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w)));
+      if (m == -INFINITY) continue;
+      float l = ml.y * ac_weight(ml.x, m, c);
+#pragma unroll
+      for (int i = 0; i < AC_Q; ++i)
+        l += (ac_weight(ac_num(x[i].x), m, c) + ac_weight(ac_num(x[i].y), m, c)) +
+             (ac_weight(ac_num(x[i].z), m, c) + ac_weight(ac_num(x[i].w), m, c));
+      ml = make_float2(m, l);
     }
-    best = bbest(b);
+    if (greedy) {
+      key = warp_max64(key);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        ml = ac_join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o)), c);
+      key = (uint64_t)__float_as_uint(ml.x) << 32 | __float_as_uint(ml.y);
+    }
+    if (lane == 0) part[r][sub] = key;
   }
-  if (tid == 0) {
+  auto pair = [](uint64_t v) { return make_float2(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v)); };
+  auto join = [&](uint64_t a, uint64_t b) {
+    if (greedy) return a > b ? a : b;
+    const float2 r = ac_join(pair(a), pair(b), c);
+    return (uint64_t)__float_as_uint(r.x) << 32 | __float_as_uint(r.y);
+  };
+  __syncthreads();
+  for (int r = tid; r < nrow; r += AC_T) {
+    uint64_t a = part[r][0];
+    for (int i = 1; i < nsub; ++i) a = join(a, part[r][i]);
+    mine[r] = a;
+  }
+  cl.sync();
+  for (int r = tid; r < nrow; r += AC_T) {
+    uint64_t v[AC_C];
+#pragma unroll
+    for (int i = 0; i < AC_C; ++i) v[i] = *cl.map_shared_rank(&mine[r], i);
+    uint64_t a = v[0];
+#pragma unroll
+    for (int i = 1; i < AC_C; ++i) a = join(a, v[i]);  // (the same order in every block)
+    tot[r] = a;
+  }
+  if (tid == 0) rejected = nd;
+  __syncthreads();
+
+  // ---- decisions (the same in every block)
+  auto first_of = [](uint64_t k) { return k ? (int64_t)(0xFFFFFFFFu - (uint32_t)k) : -1; };
+  auto prob = [&](float x, int r) {
+    const float2 ml = pair(tot[r]);
+    return ml.y > 0.f && x > -INFINITY ? ac_weight(x, ml.x, c) / ml.y : 0.f;
+  };
+  if (tid < nd) {
+    bool ok;
+    if (greedy) {
+      ok = first_of(tot[tid]) == tok && tok >= 0 && uu < 1.f;
+    } else {
+      const float qd = !has_q ? 1.f : prob(dl, nd + 1 + tid);
+      ok = uu < fminf(prob(tl, tid) / fmaxf(qd, 1e-10f), 1.f);
+    }
+    if (!ok) atomicMin(&rejected, tid);
+  }
+  __syncthreads();
+  const int a = rejected;
+  int64_t next = -1;
+  if (greedy) {
+    next = first_of(tot[a]);
+  } else {
+    // ---- the token after them: the largest r_v / e_v of this block's slice
+    const float2 pm = pair(tot[a]);
+    const bool cut = a < nd, q = cut && has_q;
+    const float2 qm = q ? pair(tot[nd + 1 + a]) : make_float2(0.f, 0.f);
+    const float pi = pm.y > 0.f ? 1.f / pm.y : 0.f, qi = qm.y > 0.f ? 1.f / qm.y : 0.f;
+    const uint8_t *prow = row_at(a), *qrow = q ? row_at(nd + 1 + a) : prow;
+    const bool pv = ac_aligned<DT>(prow), qv = ac_aligned<DT>(qrow);
+    const float *er = p.e + s * p.e_ld;
+    const bool ev = ac_aligned<LBX_F32>(er);
+    int64_t dtok = -1;
+    if (cut && !p.draft) dtok = __ldg(p.tokens + s * p.tokens_ld + a);
+    uint64_t got = 0;
+    for (int pass = cut ? 0 : 1; pass < 2; ++pass) {
+      uint64_t key = 0;
+      const bool less = pass == 0;
+      constexpr int NB = 2;
+      for (int b = q0 + tid; b < q1; b += NB * AC_T) {
+        float4 x[NB], y[NB], z[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int k = b + i * AC_T;
+          x[i] = y[i] = z[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (k < q1) {
+            x[i] = ac_quad<DT>(prow, pv, k, V);
+            if (q && less) y[i] = ac_quad<DT>(qrow, qv, k, V);
+            z[i] = ac_quad<LBX_F32>(er, ev, k, V);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const float xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+          const float zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = 4 * (b + i * AC_T) + e;
+            const float xv = ac_num(xs[e]);
+            // (products rounded on their own: equal rows leave exactly nothing)
+            float r = xv > -INFINITY ? __fmul_rn(ac_weight(xv, pm.x, c), pi) : 0.f;
+            if (less) {
+              if (q) {
+                const float yv = ac_num(ys[e]);
+                if (yv > -INFINITY) r = __fsub_rn(r, __fmul_rn(ac_weight(yv, qm.x, c), qi));
+              } else if (v == dtok) {
+                r -= 1.f;
+              }
+            }
+            if (r > 0.f) {
+              const uint64_t k = (uint64_t)__float_as_uint(r / zs[e]) << 32 | (0xFFFFFFFFu - (uint32_t)v);
+              key = k > key ? k : key;
+            }
+          }
+        }
+      }
+      key = warp_max64(key);
+      if (lane == 0) wbest[warp] = key;
+      __syncthreads();
+      if (tid == 0) {
+        for (int i = 1; i < AC_T / 32; ++i) key = wbest[i] > key ? wbest[i] : key;
+        *cl.map_shared_rank(&best[pass][rank], 0) = key;
+      }
+      cl.sync();
+#pragma unroll
+      for (int i = 0; i < AC_C; ++i) {
+        const uint64_t k = *cl.map_shared_rank(&best[pass][i], 0);
+        got = k > got ? k : got;
+      }
+      if (got) break;  // (else p and q are equal, nothing is left over, and the token comes from p)
+    }
+    next = first_of(got);
+  }
+  cl.sync();  // (no block leaves while another reads its shared memory)
+  if (rank == 0 && tid == 0) {
     p.accepted[s] = a;
-    p.next[s] = best ? (int64_t)(0xffffffffu - (unsigned)best) : -1;
+    p.next[s] = next;
   }
 }
 
@@ -181,6 +349,20 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   p.e_ld = a->e_ld;
   p.accepted = a->accepted;
   p.next = a->next;
-  accept_simple_kernel<<<a->n_seq, AC_THREADS, 0, stream>>>(p);
-  return cuda_status(cudaGetLastError(), "accept_sampled launch");
+  LBX_CHECK_SUP((int64_t)a->n_seq * AC_C <= 0x7fffffff, "too many sequences");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a->n_seq * AC_C);
+  cfg.blockDim = dim3(AC_T);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = AC_C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a->use_pdl ? 2 : 1;
+  return cuda_status(a->dtype == LBX_F32 ? cudaLaunchKernelEx(&cfg, accept_kernel<LBX_F32>, p)
+                                         : cudaLaunchKernelEx(&cfg, accept_kernel<LBX_BF16>, p),
+                     "accept_sampled launch");
 }
