@@ -4,6 +4,7 @@
 // dimensions, (step, least) in bf16; a value is least + step * code.
 // See include/lbx.h for the layout.
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "tcgen05.cuh"
 
@@ -28,66 +29,79 @@ struct Kv4View {
 
 struct Kv4AppendParams {
   Kv4View c;
-  int n, max_start, dtype;
+  int n, max_start, rows;  // tokens of a sequence, their starts' bound, tokens in all
+  int vec;                 // inputs on 16 (fp32) or 8 (bf16) bytes
   const int32_t *start;
   const void *k; const void *v; int64_t ld;
   const float2 *rope;
 };
 
-// One warp a (token, head, key or value).  Lane l holds dimensions 2l, 2l+1 of
-// each group of 64 after the rotation.
-template <int D>
+// A row (one token's key or value of one head) is D / 4 lanes of four dimensions:
+// both members of a rotation pair are D / 8 lanes apart, a group of 64 is 16
+// lanes, two lanes make a word of codes.  ROWS rows a warp at once, so that a
+// prompt's loads are in flight together (2048 tokens x 8 heads: 18.5 us with one row
+// through shared memory, 8.9 with four).
+constexpr int KP_MANY = 4;
+template <int D, int ROWS, int DT>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4AppendParams p) {
-  constexpr int NG = D / KV4_G;
-  __shared__ __align__(16) float sx[8][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + warp;
-  const int64_t per = (int64_t)p.c.n_seq * p.n * p.c.kvh;
+  constexpr int LPR = D / 4, NG = D / KV4_G, RPW = 32 / LPR;  // lanes a row, rows a warp and pass
+  const int lane = threadIdx.x & 31, l = lane % LPR, g = l / 16;
+  const uint32_t heads = (uint32_t)p.c.kvh, per = (uint32_t)p.rows * heads;  // (token, head) rows
+  const bool value = blockIdx.y == 1;
+  const uint32_t w0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (ROWS * RPW) + lane / LPR;
   pdl_trigger();
   pdl_wait();
-  if (item >= 2 * per) return;
-  const bool value = item >= per;
-  const int64_t it = value ? item - per : item;
-  const int h = (int)(it % p.c.kvh);
-  const int64_t row = it / p.c.kvh;  // token row
-  const int s = (int)(row / p.n), i = (int)(row - (int64_t)s * p.n);
-  const int st = p.start ? p.start[s] : p.max_start;
-  if (st < 0 || st > p.max_start) {
-    if (lane == 0) atomicCAS(&g_lbx_device_error, 0, 0x801);
-    return;
-  }
-  const void *src = value ? p.v : p.k;
-  const int64_t off = row * p.ld + (int64_t)h * D;
-  float *x = sx[warp];
+  float x[ROWS][4];
+  float4 cs[ROWS][2];
+  uint32_t row[ROWS], h[ROWS];
+  bool ok[ROWS];
 #pragma unroll
-  for (int e = lane; e < D; e += 32) x[e] = load_act(src, p.dtype, off + e);
-  __syncwarp();
-  if (!value && p.rope) {
-    float y1[D / 64], y2[D / 64];
+  for (int u = 0; u < ROWS; ++u) {
+    const uint32_t it = w0 + u * RPW;
+    ok[u] = it < per;
+    row[u] = ok[u] ? it / heads : 0;
+    h[u] = ok[u] ? it - row[u] * heads : 0;
+    const void *src = value ? p.v : p.k;
+    const int64_t off = (int64_t)row[u] * p.ld + (int64_t)h[u] * D + 4 * l;
+    if (p.vec) {
+      if constexpr (DT == LBX_F32) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(src) + off));
+        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(src) + off));
+        x[u][0] = __uint_as_float(v.x << 16); x[u][1] = __uint_as_float(v.x & 0xFFFF0000u);
+        x[u][2] = __uint_as_float(v.y << 16); x[u][3] = __uint_as_float(v.y & 0xFFFF0000u);
+      }
+    } else {
 #pragma unroll
-    for (int u = 0; u < D / 64; ++u) {
-      const int j = lane + 32 * u;
-      const float2 cs = p.rope[row * (D / 2) + j];
-      const float x1 = x[j], x2 = x[j + D / 2];
-      y1[u] = __fsub_rn(__fmul_rn(x1, cs.x), __fmul_rn(x2, cs.y));
-      y2[u] = __fadd_rn(__fmul_rn(x2, cs.x), __fmul_rn(x1, cs.y));
+      for (int i = 0; i < 4; ++i) x[u][i] = load_act(src, DT, off + i);
     }
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u) {
-      const int j = lane + 32 * u;
-      x[j] = y1[u];
-      x[j + D / 2] = y2[u];
+    if (!value && p.rope) {
+      const float4 *c = reinterpret_cast<const float4 *>(p.rope + (int64_t)row[u] * (D / 2) + 4 * (l % (LPR / 2)));
+      cs[u][0] = __ldg(c);
+      cs[u][1] = __ldg(c + 1);
     }
-    __syncwarp();
   }
-  const int64_t slot = ((int64_t)s * p.c.kvh + h) * p.c.max_seq + st + i;
-  uint32_t *words = reinterpret_cast<uint32_t *>((value ? p.c.vc : p.c.kc) + slot * (D / 2));
-  uint32_t *par = (value ? p.c.vp : p.c.kp) + slot * NG;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const float a = x[64 * g + 2 * lane], b = x[64 * g + 2 * lane + 1];
-    const bool fin = __all_sync(0xffffffffu, fabsf(a) < INFINITY && fabsf(b) < INFINITY);
-    const float lo = -warp_max(fmaxf(-a, -b)), hi = warp_max(fmaxf(a, b));
+  for (int u = 0; u < ROWS; ++u) {
+    if (!value && p.rope) {
+      const float c[4] = {cs[u][0].x, cs[u][0].z, cs[u][1].x, cs[u][1].z}, s[4] = {cs[u][0].y, cs[u][0].w, cs[u][1].y, cs[u][1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = __shfl_xor_sync(0xffffffffu, x[u][i], LPR / 2);
+        x[u][i] = l < LPR / 2 ? __fsub_rn(__fmul_rn(x[u][i], c[i]), __fmul_rn(y, s[i]))
+                              : __fadd_rn(__fmul_rn(x[u][i], c[i]), __fmul_rn(y, s[i]));
+      }
+    }
+    float lo = fminf(fminf(x[u][0], x[u][1]), fminf(x[u][2], x[u][3]));
+    float hi = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
+    bool fin = fabsf(x[u][0]) < INFINITY && fabsf(x[u][1]) < INFINITY && fabsf(x[u][2]) < INFINITY && fabsf(x[u][3]) < INFINITY;
+    fin = (__ballot_sync(0xffffffffu, !fin) & (0xFFFFu << (lane & 16))) == 0u;
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
     uint16_t sb = f32_to_bf16(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
     uint16_t lb = f32_to_bf16(lo);
     float step = bf16_to_f32(sb);
@@ -101,19 +115,25 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
       step = 0.f;
     }
     const float inv = step > 0.f ? __fdiv_rn(1.0f, step) : 0.f;
-    auto code = [&](float y) {
-      if (!(step > 0.f)) return 0u;
-      return (uint32_t)__float2int_rn(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(y, least), inv)), 0.f), 15.f));
-    };
-    // 8 codes of a block: lanes 4r .. 4r+3
-    uint32_t w = (code(a) | code(b) << 4) << (8 * (lane & 3));
-    w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    w |= __shfl_xor_sync(0xffffffffu, w, 2);
-    if ((lane & 3) == 0) {
-      const int blk = 8 * g + (lane >> 2);
-      words[value ? kv4_word<D, true>(blk) : kv4_word<D, false>(blk)] = w;
+    uint32_t w = 0;
+    if (step > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w |= (uint32_t)__float2int_rn(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[u][i], least), inv)), 0.f), 15.f)) << (4 * i);
     }
-    if (lane == 0) par[g] = (uint32_t)sb | (uint32_t)lb << 16;
+    w |= __shfl_xor_sync(0xffffffffu, w, 1) << 16;  // (the even lane's: its codes below, its neighbour's above)
+    if (!ok[u]) continue;
+    const int s = (int)(row[u] / (uint32_t)p.n), i = (int)(row[u] - (uint32_t)s * (uint32_t)p.n);
+    const int st = p.start ? __ldg(p.start + s) : p.max_start;
+    if (st < 0 || st > p.max_start) {
+      if (l == 0) atomicCAS(&g_lbx_device_error, 0, 0x801);
+      continue;
+    }
+    const int64_t slot = ((int64_t)s * p.c.kvh + h[u]) * p.c.max_seq + st + i;
+    const int b = l / 2;
+    if (!(l & 1))
+      reinterpret_cast<uint32_t *>((value ? p.c.vc : p.c.kc) + slot * (D / 2))[value ? kv4_word<D, true>(b) : kv4_word<D, false>(b)] = w;
+    if (l % 16 == 0) (value ? p.c.vp : p.c.kp)[slot * NG + g] = (uint32_t)sb | (uint32_t)lb << 16;
   }
 }
 
@@ -124,23 +144,19 @@ struct Kv4ReadParams {
   float *out[2];
 };
 
-// one thread a block of eight dimensions of one (sequence, head, token), keys then values
+// one thread a block of eight dimensions: (slot, block) along x, head, (sequence, keys or values)
 template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4ReadParams p) {
-  constexpr int NB = D / 8;
-  const bool value = blockIdx.y == 1;
-  float *out = p.out[blockIdx.y];
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (!out || e >= (int64_t)p.c.n_seq * p.c.kvh * p.n * NB) return;
-  const int b = (int)(e % NB);
-  const int64_t r = e / NB;  // (sequence, head, token)
-  const int64_t sh = r / p.n;
-  const int i = (int)(r - sh * p.n), s = (int)(sh / p.c.kvh);
-  const int st = p.start ? p.start[s] : p.max_start;
-  const bool ok = st >= 0 && st <= p.max_start;
-  if (!ok) atomicCAS(&g_lbx_device_error, 0, 0x802);
+  constexpr uint32_t NB = D / 8;
+  const bool value = blockIdx.z & 1;
+  float *out = p.out[value];
+  const uint32_t e = blockIdx.x * 256 + threadIdx.x, i = e / NB, b = e % NB;
+  if (!out || i >= (uint32_t)p.n) return;
+  const int s = blockIdx.z >> 1;
+  const int64_t sh = (int64_t)s * p.c.kvh + blockIdx.y;
+  const int st = p.start ? __ldg(p.start + s) : p.max_start;
   float v[8];
-  if (ok) {
+  if (st >= 0 && st <= p.max_start) {
     const int64_t slot = sh * p.c.max_seq + st + i;
     const uint32_t *words = reinterpret_cast<const uint32_t *>((value ? p.c.vc : p.c.kc) + slot * (D / 2));
     const uint32_t w = words[value ? kv4_word<D, true>(b) : kv4_word<D, false>(b)];
@@ -149,10 +165,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
     for (int t = 0; t < 8; ++t)
       v[t] = __fadd_rn(kv4_least(par), __fmul_rn(kv4_step(par), (float)((w >> (4 * t)) & 15u)));
   } else {
+    atomicCAS(&g_lbx_device_error, 0, 0x802);
 #pragma unroll
     for (int t = 0; t < 8; ++t) v[t] = __uint_as_float(0x7FC00000u);
   }
-  float4 *o = reinterpret_cast<float4 *>(out + r * D + 8 * b);
+  float4 *o = reinterpret_cast<float4 *>(out + (sh * p.n + i) * D + 8 * b);
   o[0] = make_float4(v[0], v[1], v[2], v[3]);
   o[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
@@ -898,18 +915,32 @@ extern "C" int lbx_kv4_append(const lbx_kv4_append_args *a, cudaStream_t stream)
   LBX_CHECK_ARG(a->kv_ld >= (int64_t)a->cache.kv_heads * a->cache.head_dim, "rows overlap");
   p.n = a->n;
   p.max_start = a->max_start;
-  p.dtype = a->dtype;
   p.start = a->start;
   p.k = a->k_new;
   p.v = a->v_new;
   p.ld = a->kv_ld;
   p.rope = reinterpret_cast<const float2 *>(a->rope_cs);
-  const int64_t items = 2ll * a->cache.n_seq * a->n * a->cache.kv_heads;
-  LBX_CHECK_SUP((items + 7) / 8 <= 0x7fffffff, "too many rows");
-  const dim3 grid((unsigned)((items + 7) / 8));
-  const cudaError_t e = a->cache.head_dim == 128
-                            ? launch(kv4_append_kernel<128>, grid, dim3(256), 0, stream, a->use_pdl != 0, p)
-                            : launch(kv4_append_kernel<64>, grid, dim3(256), 0, stream, a->use_pdl != 0, p);
+  LBX_CHECK_ARG(aligned16(a->rope_cs), "rope_cs must be 16-byte aligned");
+  const int64_t rows = (int64_t)a->cache.n_seq * a->n, items = rows * a->cache.kv_heads;
+  LBX_CHECK_SUP(items <= 0x3fffffff, "too many rows");
+  p.rows = (int)rows;
+  const int es = a->dtype == LBX_F32 ? 4 : 2;
+  p.vec = ((reinterpret_cast<uintptr_t>(a->k_new) | reinterpret_cast<uintptr_t>(a->v_new)) & (uintptr_t)(4 * es - 1)) == 0 &&
+          a->kv_ld % 4 == 0;
+  const int d = a->cache.head_dim, rpw = 128 / d;
+  // several rows a warp once single ones would fill the SMs twice over
+  const bool many = items > (int64_t)rpw * 64 * device_sm_count();
+  const int64_t blk = 8 * rpw * (many ? KP_MANY : 1);
+  const dim3 grid((unsigned)((items + blk - 1) / blk), 2);
+  auto go = [&](auto kern) { return launch(kern, grid, dim3(256), 0, stream, a->use_pdl != 0, p); };
+  auto pick = [&](auto dd, auto dt) {
+    constexpr int D = decltype(dd)::value, DT = decltype(dt)::value;
+    return many ? go(kv4_append_kernel<D, KP_MANY, DT>) : go(kv4_append_kernel<D, 1, DT>);
+  };
+  using F = std::integral_constant<int, LBX_F32>;
+  using B = std::integral_constant<int, LBX_BF16>;
+  const cudaError_t e = d == 128 ? (es == 4 ? pick(std::integral_constant<int, 128>{}, F{}) : pick(std::integral_constant<int, 128>{}, B{}))
+                                 : (es == 4 ? pick(std::integral_constant<int, 64>{}, F{}) : pick(std::integral_constant<int, 64>{}, B{}));
   return cuda_status(e, "kv4_append launch");
 }
 
@@ -928,9 +959,9 @@ extern "C" int lbx_kv4_read(const lbx_kv4_cache *c, const int32_t *start, int32_
   p.start = start;
   p.out[0] = k;
   p.out[1] = v;
-  const int64_t items = (int64_t)c->n_seq * c->kv_heads * n * (c->head_dim / 8);
-  LBX_CHECK_SUP((items + 255) / 256 <= 0x7fffffff, "too many rows");
-  const dim3 grid((unsigned)((items + 255) / 256), 2);
+  const int64_t items = (int64_t)n * (c->head_dim / 8);
+  LBX_CHECK_SUP(items <= 0x7fffffff && c->kv_heads <= 65535 && c->n_seq <= 32767, "too many rows");
+  const dim3 grid((unsigned)((items + 255) / 256), c->kv_heads, 2 * c->n_seq);
   if (c->head_dim == 128)
     kv4_read_kernel<128><<<grid, 256, 0, stream>>>(p);
   else

@@ -24,54 +24,55 @@ struct AcceptParams {
 };
 
 // One cluster of AC_C blocks a sequence, each with a slice of the vocabulary, in one
-// launch: the statistics of all rows at once (a warp takes 1024 logits of one
-// row at a time, eight 16-byte loads a lane in flight), joined over the cluster's shared
+// launch: the statistics of all rows at once (a warp takes 512 logits of one
+// row at a time, four 16-byte loads a lane in flight), joined over the cluster's shared
 // memory; every block then makes the same decisions and takes its slice of the
 // drawing.  All rows are read before the first decision is known: deciding row
 // by row would read fewer of them and wait for the cluster once a draft.
 // Bound by memory for many sequences, by three round trips to it and two cluster barriers
 // for one.
-constexpr int AC_T = 256;    // threads
+constexpr int AC_MANY = 16;  // sequences from which blocks have 256 threads (four fill an SM) instead of 1024
 constexpr int AC_C = 8;      // blocks a sequence
-constexpr int AC_SUB = 16;   // parts of a row's slice at most
-constexpr int AC_Q = 8;      // quads of logits a lane loads together
+constexpr int AC_Q = 4;      // quads of logits a lane loads together
 constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
+// Scaled logits y = x * log2(e) / T stay within +-AC_TOP, NaN at the bottom: weights
+// 2^(y - top) then need no case of their own for infinities, and 36 instructions a
+// logit (selects turned into branches) became 7.
+constexpr float AC_TOP = 3e38f;
+constexpr float AC_COLD = 1e-30f;  // temperatures up to here take the maximum
 
-// Logits 4 q .. 4 q + 3 of a row of V (NaN and what is past V count as -inf).
-// VEC: the row starts on 16 (fp32) or 8 (bf16) bytes.
+// does a row start on 16 (fp32) or 8 (bf16) bytes
 template <int DT>
 LBX_DEV bool ac_aligned(const void *row) { return (reinterpret_cast<uintptr_t>(row) & (DT == LBX_F32 ? 15u : 7u)) == 0; }
+// four logits (what is past V: -inf)
+template <int DT>
+LBX_DEV float4 ac_quad_full(const void *row, int q) {
+  if constexpr (DT == LBX_F32) {
+    return __ldg(reinterpret_cast<const float4 *>(row) + q);
+  } else {
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row) + q);
+    return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xFFFF0000u), __uint_as_float(x.y << 16),
+                       __uint_as_float(x.y & 0xFFFF0000u));
+  }
+}
 template <int DT>
 LBX_DEV float4 ac_quad(const void *row, bool vec, int q, int V) {
+  if (vec && 4 * q + 3 < V) return ac_quad_full<DT>(row, q);
   float v[4];
-  if (vec && 4 * q + 3 < V) {
-    if constexpr (DT == LBX_F32) {
-      const float4 x = __ldg(reinterpret_cast<const float4 *>(row) + q);
-      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else {
-      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row) + q);
-      v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xFFFF0000u);
-      v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xFFFF0000u);
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 4 * q + i < V ? load_act(row, DT, 4 * (int64_t)q + i) : -INFINITY;
-  }
+  for (int i = 0; i < 4; ++i) v[i] = 4 * q + i < V ? load_act(row, DT, 4 * (int64_t)q + i) : -INFINITY;
   return make_float4(v[0], v[1], v[2], v[3]);
 }
-LBX_DEV float ac_num(float x) { return x == x ? x : -INFINITY; }
+LBX_DEV float ac_scaled(float x, float c) { return fminf(fmaxf(x * c, -AC_TOP), AC_TOP); }
 LBX_DEV float ac_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// weight of a logit against its row's maximum m: 2^((x - m) c), c = log2(e) / T;
-// 1 at the maximum (an infinite one too)
-LBX_DEV float ac_weight(float x, float m, float c) { return x == m ? 1.f : ac_ex2((x - m) * c); }
-// the larger value first, then the lower index
+// the larger value first, then the lower index; 0 for -inf and NaN
 LBX_DEV uint64_t ac_key(float x, uint32_t i) {
   const uint32_t b = __float_as_uint(x);
-  return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
+  return x > -INFINITY ? (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i) : 0ull;
 }
 LBX_DEV uint64_t warp_max64(uint64_t v) {
 #pragma unroll
@@ -81,19 +82,21 @@ LBX_DEV uint64_t warp_max64(uint64_t v) {
   }
   return v;
 }
-// (maximum, sum of weights against it) of two parts of a row
-LBX_DEV float2 ac_join(float2 a, float2 b, float c) {
+// (top, sum of weights against it) of two parts of a row; a part of nothing: (-AC_TOP, 0)
+LBX_DEV float2 ac_join(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) return make_float2(m, 0.f);
-  return make_float2(m, a.y * ac_weight(a.x, m, c) + b.y * ac_weight(b.x, m, c));
+  return make_float2(m, a.y * ac_ex2(a.x - m) + b.y * ac_ex2(b.x - m));
 }
+LBX_DEV uint64_t ac_pack(float2 v) { return (uint64_t)__float_as_uint(v.x) << 32 | __float_as_uint(v.y); }
+LBX_DEV float2 ac_pair(uint64_t v) { return make_float2(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v)); }
 
-template <int DT>
-__global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__ AcceptParams p) {
+template <int DT, int AC_T>
+__global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_constant__ AcceptParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   constexpr int ES = DT == LBX_F32 ? 4 : 2;
-  __shared__ uint64_t part[AC_ROWS][AC_SUB];  // of this block's slices: (max, sum) pairs, or keys (greedy)
+  constexpr int NWARP = AC_T / 32;
+  __shared__ uint64_t part[AC_ROWS][NWARP];  // each warp's share of a row: (top, sum) pairs, or keys (greedy)
   __shared__ uint64_t mine[AC_ROWS], tot[AC_ROWS];
   __shared__ uint64_t best[2][AC_C];          // every block's, in the first block
   __shared__ uint64_t wbest[AC_T / 32];
@@ -103,8 +106,9 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
   pdl_trigger();
   pdl_wait();
   const float T = p.temps ? __ldg(p.temps + s) : p.temperature;
-  const bool greedy = !(T > 0.f);
+  const bool greedy = !(T > AC_COLD);
   const float c = 1.4426950408889634f / T;
+  const uint64_t none = greedy ? 0ull : ac_pack(make_float2(-AC_TOP, 0.f));
   int nd = p.k;
   if (p.n_draft) {
     nd = __ldg(p.n_draft + s);
@@ -120,11 +124,10 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
     return r <= nd ? reinterpret_cast<const uint8_t *>(p.target) + (s * p.target_seq + r * p.target_row) * ES
                    : reinterpret_cast<const uint8_t *>(p.draft) + (s * p.draft_seq + (r - nd - 1) * p.draft_row) * ES;
   };
-  // this block's quads, and their parts (AC_SUB at most, a multiple of a warp's batch)
+  // this block's quads, in batches of 32 lanes x AC_Q
+  constexpr int BQ = 32 * AC_Q;
   const int nq = (V + 3) / 4, per = (nq + AC_C - 1) / AC_C;
-  const int q0 = min(nq, rank * per), q1 = min(nq, q0 + per);
-  const int len = ((per + AC_SUB - 1) / AC_SUB + 32 * AC_Q - 1) / (32 * AC_Q) * (32 * AC_Q);
-  const int nsub = (per + len - 1) / len;
+  const int q0 = min(nq, rank * per), q1 = min(nq, q0 + per), nb = (per + BQ - 1) / BQ;
 
   // what a decision needs besides the rows' statistics, on its way meanwhile
   int64_t tok = -1;
@@ -133,72 +136,101 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
     tok = __ldg(p.tokens + s * p.tokens_ld + tid);
     uu = __ldg(p.u + s * p.u_ld + tid);
     if (tok >= 0 && tok < V) {
-      tl = ac_num(load_act(row_at(tid), DT, tok));
-      if (has_q) dl = ac_num(load_act(row_at(nd + 1 + tid), DT, tok));
+      tl = load_act(row_at(tid), DT, tok);
+      if (has_q) dl = load_act(row_at(nd + 1 + tid), DT, tok);
     } else if (rank == 0) {
       atomicCAS(&g_lbx_device_error, 0, 0x811);
     }
   }
 
-  // ---- statistics of every row's slice
-  for (int t = warp; t < nrow * nsub; t += AC_T / 32) {
-    const int r = t / nsub, sub = t - r * nsub;
-    const uint8_t *row = row_at(r);
-    const bool vec = ac_aligned<DT>(row);
-    const int b0 = q0 + sub * len, b1 = min(q1, b0 + len);
-    float2 ml = make_float2(-INFINITY, 0.f);
+  // ---- statistics of every row's slice: the (row, batch) items dealt evenly to the
+  // warps, the next item's loads under way while one is worked on
+  for (int i = tid; i < nrow * NWARP; i += AC_T) (&part[0][0])[i] = none;
+  __syncthreads();
+  {
+    const int items = nrow * nb;
+    int it = (int)((int64_t)items * warp / NWARP);
+    const int end = (int)((int64_t)items * (warp + 1) / NWARP);
+    int r = it / nb, b = it - r * nb;
+    float m = -AC_TOP, l = 0.f;
     uint64_t key = 0;
-    for (int b = b0; b < b1; b += 32 * AC_Q) {
-      float4 x[AC_Q];
+    auto load = [&](float4 (&x)[AC_Q], int r, int b) {
+      const uint8_t *row = row_at(r);
+      const bool vec = ac_aligned<DT>(row);
+      const int q = q0 + b * BQ;
+      if (vec && q + BQ <= q1 && 4 * (q + BQ) <= V) {
 #pragma unroll
-      for (int i = 0; i < AC_Q; ++i) {
-        const int q = b + 32 * i + lane;
-        x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (q < b1) x[i] = ac_quad<DT>(row, vec, q, V);
+        for (int i = 0; i < AC_Q; ++i) x[i] = ac_quad_full<DT>(row, q + 32 * i + lane);
+      } else {
+#pragma unroll
+        for (int i = 0; i < AC_Q; ++i) {
+          x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (q + 32 * i + lane < q1) x[i] = ac_quad<DT>(row, vec, q + 32 * i + lane, V);
+        }
       }
+    };
+    // works on x, item (r, b), with item it + 1 on its way into y
+    auto work = [&](float4 (&x)[AC_Q], float4 (&y)[AC_Q]) {
+      const int b2 = b + 1 < nb ? b + 1 : 0, r2 = b2 ? r : r + 1;
+      if (it + 1 < end) load(y, r2, b2);
       if (greedy) {
 #pragma unroll
         for (int i = 0; i < AC_Q; ++i) {
-          const float v[4] = {ac_num(x[i].x), ac_num(x[i].y), ac_num(x[i].z), ac_num(x[i].w)};
+          const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint64_t k = v[e] > -INFINITY ? ac_key(v[e], (uint32_t)(4 * (b + 32 * i + lane) + e)) : 0ull;
+            const uint64_t k = ac_key(v[e], (uint32_t)(4 * (q0 + b * BQ + 32 * i + lane) + e));
             key = k > key ? k : key;
           }
         }
-        continue;
+      } else {
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < AC_Q; ++i) {
+          x[i] = make_float4(ac_scaled(x[i].x, c), ac_scaled(x[i].y, c), ac_scaled(x[i].z, c), ac_scaled(x[i].w, c));
+          mn = fmaxf(mn, fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w)));
+        }
+        l *= ac_ex2(m - mn);
+        m = mn;
+        // (a top still at the bottom: nothing but -inf so far, whose weights of 1 the rows' totals drop)
+#pragma unroll
+        for (int i = 0; i < AC_Q; ++i)
+          l += (ac_ex2(x[i].x - m) + ac_ex2(x[i].y - m)) + (ac_ex2(x[i].z - m) + ac_ex2(x[i].w - m));
       }
-      float m = ml.x;  // (fmaxf passes a NaN over)
+      if (r2 != r || it + 1 >= end) {
+        if (greedy) {
+          key = warp_max64(key);
+        } else {
+          float2 ml = make_float2(m, m > -AC_TOP ? l : 0.f);
 #pragma unroll
-      for (int i = 0; i < AC_Q; ++i) m = fmaxf(m, fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w)));
-      if (m == -INFINITY) continue;
-      float l = ml.y * ac_weight(ml.x, m, c);
-#pragma unroll
-      for (int i = 0; i < AC_Q; ++i)
-        l += (ac_weight(ac_num(x[i].x), m, c) + ac_weight(ac_num(x[i].y), m, c)) +
-             (ac_weight(ac_num(x[i].z), m, c) + ac_weight(ac_num(x[i].w), m, c));
-      ml = make_float2(m, l);
+          for (int o = 16; o > 0; o >>= 1)
+            ml = ac_join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o)));
+          key = ac_pack(ml);
+        }
+        if (lane == 0) part[r][warp] = key;
+        key = 0;
+        m = -AC_TOP;
+        l = 0.f;
+      }
+      r = r2;
+      b = b2;
+      ++it;
+    };
+    float4 x[AC_Q], y[AC_Q];
+    if (it < end) load(x, r, b);
+    while (it < end) {
+      work(x, y);
+      if (it < end) work(y, x);
     }
-    if (greedy) {
-      key = warp_max64(key);
-    } else {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        ml = ac_join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o)), c);
-      key = (uint64_t)__float_as_uint(ml.x) << 32 | __float_as_uint(ml.y);
-    }
-    if (lane == 0) part[r][sub] = key;
   }
-  auto pair = [](uint64_t v) { return make_float2(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v)); };
   auto join = [&](uint64_t a, uint64_t b) {
     if (greedy) return a > b ? a : b;
-    const float2 r = ac_join(pair(a), pair(b), c);
-    return (uint64_t)__float_as_uint(r.x) << 32 | __float_as_uint(r.y);
+    return ac_pack(ac_join(ac_pair(a), ac_pair(b)));
   };
   __syncthreads();
   for (int r = tid; r < nrow; r += AC_T) {
     uint64_t a = part[r][0];
-    for (int i = 1; i < nsub; ++i) a = join(a, part[r][i]);
+    for (int i = 1; i < NWARP; ++i) a = join(a, part[r][i]);
     mine[r] = a;
   }
   cl.sync();
@@ -217,8 +249,8 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
   // ---- decisions (the same in every block)
   auto first_of = [](uint64_t k) { return k ? (int64_t)(0xFFFFFFFFu - (uint32_t)k) : -1; };
   auto prob = [&](float x, int r) {
-    const float2 ml = pair(tot[r]);
-    return ml.y > 0.f && x > -INFINITY ? ac_weight(x, ml.x, c) / ml.y : 0.f;
+    const float2 ml = ac_pair(tot[r]);
+    return ml.y > 0.f ? ac_ex2(ac_scaled(x, c) - ml.x) / ml.y : 0.f;
   };
   if (tid < nd) {
     bool ok;
@@ -237,9 +269,9 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
     next = first_of(tot[a]);
   } else {
     // ---- the token after them: the largest r_v / e_v of this block's slice
-    const float2 pm = pair(tot[a]);
+    const float2 pm = ac_pair(tot[a]);
     const bool cut = a < nd, q = cut && has_q;
-    const float2 qm = q ? pair(tot[nd + 1 + a]) : make_float2(0.f, 0.f);
+    const float2 qm = q ? ac_pair(tot[nd + 1 + a]) : make_float2(0.f, 0.f);
     const float pi = pm.y > 0.f ? 1.f / pm.y : 0.f, qi = qm.y > 0.f ? 1.f / qm.y : 0.f;
     const uint8_t *prow = row_at(a), *qrow = q ? row_at(nd + 1 + a) : prow;
     const bool pv = ac_aligned<DT>(prow), qv = ac_aligned<DT>(qrow);
@@ -251,7 +283,7 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
     for (int pass = cut ? 0 : 1; pass < 2; ++pass) {
       uint64_t key = 0;
       const bool less = pass == 0;
-      constexpr int NB = 2;
+      constexpr int NB = AC_T == 256 ? 2 : 1;
       for (int b = q0 + tid; b < q1; b += NB * AC_T) {
         float4 x[NB], y[NB], z[NB];
 #pragma unroll
@@ -271,16 +303,11 @@ __global__ void __launch_bounds__(AC_T, 3) accept_kernel(const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int v = 4 * (b + i * AC_T) + e;
-            const float xv = ac_num(xs[e]);
             // (products rounded on their own: equal rows leave exactly nothing)
-            float r = xv > -INFINITY ? __fmul_rn(ac_weight(xv, pm.x, c), pi) : 0.f;
+            float r = __fmul_rn(ac_ex2(ac_scaled(xs[e], c) - pm.x), pi);
             if (less) {
-              if (q) {
-                const float yv = ac_num(ys[e]);
-                if (yv > -INFINITY) r = __fsub_rn(r, __fmul_rn(ac_weight(yv, qm.x, c), qi));
-              } else if (v == dtok) {
-                r -= 1.f;
-              }
+              if (q) r = __fsub_rn(r, __fmul_rn(ac_ex2(ac_scaled(ys[e], c) - qm.x), qi));
+              else if (v == dtok) r -= 1.f;
             }
             if (r > 0.f) {
               const uint64_t k = (uint64_t)__float_as_uint(r / zs[e]) << 32 | (0xFFFFFFFFu - (uint32_t)v);
@@ -352,7 +379,8 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   LBX_CHECK_SUP((int64_t)a->n_seq * AC_C <= 0x7fffffff, "too many sequences");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a->n_seq * AC_C);
-  cfg.blockDim = dim3(AC_T);
+  const bool many = a->n_seq >= AC_MANY;
+  cfg.blockDim = dim3(many ? 256 : 1024);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -362,7 +390,8 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a->use_pdl ? 2 : 1;
-  return cuda_status(a->dtype == LBX_F32 ? cudaLaunchKernelEx(&cfg, accept_kernel<LBX_F32>, p)
-                                         : cudaLaunchKernelEx(&cfg, accept_kernel<LBX_BF16>, p),
+  auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, p); };
+  return cuda_status(a->dtype == LBX_F32 ? (many ? go(accept_kernel<LBX_F32, 256>) : go(accept_kernel<LBX_F32, 1024>))
+                                         : (many ? go(accept_kernel<LBX_BF16, 256>) : go(accept_kernel<LBX_BF16, 1024>)),
                      "accept_sampled launch");
 }

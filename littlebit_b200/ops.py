@@ -541,7 +541,13 @@ def accept_greedy_tree(cand: torch.Tensor, node_argmax: torch.Tensor,
 # ---------------------------------------------------------------------------
 # 8-bit integer product (scales for each token and each channel)
 # ---------------------------------------------------------------------------
-def _rows(name: str, t: torch.Tensor, dtypes=(torch.float32, torch.bfloat16)) -> torch.Tensor:
+_FLOATS = (torch.float32, torch.bfloat16)
+_DTYPE = {torch.float32: L.LBX_F32, torch.bfloat16: L.LBX_BF16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _rows(name: str, t: torch.Tensor, dtypes=_FLOATS) -> torch.Tensor:
     """A 2-D CUDA tensor whose rows are contiguous (any row stride that does not overlap)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
@@ -549,6 +555,8 @@ def _rows(name: str, t: torch.Tensor, dtypes=(torch.float32, torch.bfloat16)) ->
         raise RuntimeError(f"{name} must be a CUDA tensor (the B200 library has no CPU path)")
     if t.dtype not in dtypes:
         raise RuntimeError(f"{name} has type {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if t.is_contiguous() and t.dim() == 2:
+        return t
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise RuntimeError(f"{name} must be 2-D with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
     return t
@@ -558,35 +566,42 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
+def _vec(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, index: int) -> int:
+    """Address of a contiguous tensor of n values on device ``index``."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != dtype or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+        raise RuntimeError(f"{name} must hold {n} contiguous {dtype} values on cuda:{index}, got {tuple(t.shape)} "
+                           f"{t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
 class _on:
-    """Makes a tensor's device current for a call where it is not."""
-    __slots__ = ("dev", "prev")
+    """Makes a device current for a call where it is not; gives its current stream."""
+    __slots__ = ("index", "prev")
 
-    def __init__(self, dev: torch.device):
-        self.dev, self.prev = dev.index, None
+    def __init__(self, index: int):
+        self.index, self.prev = index, None
 
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.dev:
+    def __enter__(self) -> int:
+        cur = torch._C._cuda_getDevice()
+        if cur != self.index:
             self.prev = cur
-            torch.cuda.set_device(self.dev)
-        return ctypes.c_void_p(torch.cuda.current_stream(self.dev).cuda_stream)
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.prev is not None:
             torch.cuda.set_device(self.prev)
 
 
-def _stream_ws(device: torch.device, tag: str, stream: ctypes.c_void_p, nbytes: int) -> torch.Tensor:
+def _stream_ws(index: int, tag: str, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of one operator on one stream (calls on different streams never share it)."""
-    return workspace(device, f"{tag}/{stream.value or 0}").get(nbytes)
-
-
-def _vec(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    _cuda(name, t)
-    if t.dtype != dtype or t.numel() != n or t.device != device:
-        raise RuntimeError(f"{name} must hold {n} {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t
+    key = (index, tag, stream)
+    ws = _WS.get(key)
+    if ws is None:
+        ws = _WS[key] = Workspace(torch.device("cuda", index))
+    return ws.get(nbytes)
 
 
 def quantize_tokens(x: torch.Tensor):
@@ -599,8 +614,9 @@ def quantize_tokens(x: torch.Tensor):
     ld = -(-k // 16) * 16
     q = torch.empty(m, ld, dtype=torch.int8, device=x.device)[:, :k]
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    with _on(x.device) as st:
-        L.check(lib().lbx_quant_tokens(_p(x), _dt(x), _ld(x), m, k, _p(q), ld, _p(scale), st), "quantize_tokens")
+    with _on(x.get_device()) as st:
+        L.check(lib().lbx_quant_tokens(x.data_ptr(), _DTYPE[x.dtype], _ld(x), m, k, q.data_ptr(), ld,
+                                       scale.data_ptr(), st), "quantize_tokens")
     return q, scale
 
 
@@ -615,26 +631,27 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     Result type: ``out_dtype``, else x's."""
     _rows("x", x)
     _rows("weight", weight, (torch.int8,))
-    (m, k), n = x.shape, weight.shape[0]
-    if weight.shape[1] != k:
-        raise RuntimeError(f"x has {k} features, weight {weight.shape[1]}")
-    dev = x.device
-    if weight.device != dev:
+    (m, k), (n, kw) = x.shape, weight.shape
+    if kw != k:
+        raise RuntimeError(f"x has {k} features, weight {kw}")
+    dev = x.get_device()
+    if weight.get_device() != dev:
         raise RuntimeError("x and weight must be on one device")
-    _vec("weight_scale", weight_scale, n, torch.float32, dev)
-    if bias is not None:
-        _vec("bias", bias, n, torch.float32, dev)
     if out is None:
-        out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=dev)
+        out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=x.device)
     else:
         _rows("out", out)
-        if tuple(out.shape) != (m, n) or out.device != dev or (out_dtype is not None and out.dtype != out_dtype):
-            raise RuntimeError(f"out must be [{m}, {n}] on {dev}")
-    a = L.Int8Args(m, n, k, _dt(x), _dt(out), 0, x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight),
-                   weight_scale.data_ptr(), _p(bias), out.data_ptr(), _ld(out))
+        if tuple(out.shape) != (m, n) or out.get_device() != dev or (out_dtype is not None and out.dtype != out_dtype):
+            raise RuntimeError(f"out must be [{m}, {n}] on cuda:{dev}")
+    if out.dtype not in _FLOATS:
+        raise RuntimeError(f"unsupported result type {out.dtype} (float32 or bfloat16)")
+    a = L.Int8Args(m, n, k, _DTYPE[x.dtype], _DTYPE[out.dtype], 0, x.data_ptr(), _ld(x), weight.data_ptr(),
+                   _ld(weight), _vec("weight_scale", weight_scale, n, torch.float32, dev),
+                   None if bias is None else _vec("bias", bias, n, torch.float32, dev), out.data_ptr(), _ld(out))
     with _on(dev) as st:
-        ws = _stream_ws(dev, "int8", st, int(lib().lbx_linear_int8_workspace_size(m, n, k)))
-        L.check(lib().lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
+        c = lib()
+        ws = _stream_ws(dev, "int8", st, c.lbx_linear_int8_workspace_size(m, n, k))
+        L.check(c.lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
     return out
 
 
@@ -701,17 +718,18 @@ class Kv4Cache:
         kc, kp, vc, vp = self.k_codes, self.k_params, self.v_codes, self.v_params
         for nm, t, ty in (("k_codes", kc, torch.uint8), ("v_codes", vc, torch.uint8),
                           ("k_params", kp, torch.bfloat16), ("v_params", vp, torch.bfloat16)):
-            _cuda(nm, t)
-            if t.dtype != ty:
-                raise RuntimeError(f"{nm} must be {ty}")
-            if t.device != kc.device:
-                raise RuntimeError("cache tensors must be on one device")
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == ty and t.is_contiguous()):
+                raise RuntimeError(f"{nm} must be a contiguous {ty} CUDA tensor (the B200 library has no CPU path)")
+        index = kc.get_device()
+        if not index == kp.get_device() == vc.get_device() == vp.get_device():
+            raise RuntimeError("cache tensors must be on one device")
         if kc.dim() != 4 or kp.dim() != 5:
             raise RuntimeError("codes must be 4-D and params 5-D")
         S, H, T, D2 = kc.shape
-        if vc.shape != kc.shape or vp.shape != kp.shape or tuple(kp.shape) != (S, H, T, 2 * D2 // KV4_GROUP, 2):
+        if vc.shape != kc.shape or vp.shape != kp.shape or kp.shape != (S, H, T, 2 * D2 // KV4_GROUP, 2):
             raise RuntimeError(f"cache shapes do not fit together: {tuple(kc.shape)} {tuple(kp.shape)} "
                                f"{tuple(vc.shape)} {tuple(vp.shape)}")
+        object.__setattr__(self, "index", index)
         object.__setattr__(self, "_struct", L.Kv4Cache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(),
                                                        S, H, T, 2 * D2))
 
@@ -720,17 +738,11 @@ class Kv4Cache:
         return self._struct
 
 
-def _rope_arg(rope_cs: Optional[torch.Tensor], rows: int, d: int, device) -> Optional[int]:
-    if rope_cs is None:
-        return None
-    return _vec("rope_cs", rope_cs, rows * d, torch.float32, device).data_ptr()
-
-
-def _start_arg(name: str, start, n_seq: int, bound: int, device):
-    """(device pointer or None, host bound) of per-sequence slot counts: an int for all,
+def _start_arg(name: str, start, n_seq: int, bound: Optional[int], max_seq: int, index: int):
+    """(device address or None, host bound) of per-sequence slot counts: an int for all,
     or a device int32 [n_seq] with its host-side upper bound."""
     if isinstance(start, torch.Tensor):
-        return _vec(name, start, n_seq, torch.int32, device).data_ptr(), int(bound)
+        return _vec(name, start, n_seq, torch.int32, index), max_seq if bound is None else int(bound)
     return None, int(start)
 
 
@@ -742,31 +754,32 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start,
     k_new / v_new [S * n, kv_heads * head_dim], float32 or bfloat16, sequence by
     sequence.  ``start``: first slot, an int for every sequence, or a device int32
     [S] bounded by ``max_start``."""
-    c = cache.struct()
+    c, dev = cache.struct(), cache.index
     _rows("k_new", k_new)
     _rows("v_new", v_new, (k_new.dtype,))
-    dev = cache.k_codes.device
-    if v_new.shape != k_new.shape or k_new.shape[1] != c.kv_heads * c.head_dim or k_new.shape[0] % c.n_seq:
+    rows, width = k_new.shape
+    if v_new.shape != k_new.shape or width != c.kv_heads * c.head_dim or rows % c.n_seq:
         raise RuntimeError(f"k_new / v_new must be [{c.n_seq} * n, {c.kv_heads * c.head_dim}], got "
                            f"{tuple(k_new.shape)} and {tuple(v_new.shape)}")
-    if k_new.device != dev or v_new.device != dev:
+    if k_new.get_device() != dev or v_new.get_device() != dev:
         raise RuntimeError("k_new, v_new and the cache must be on one device")
-    if k_new.shape[0] > 1 and v_new.stride(0) != k_new.stride(0):
+    ld = _ld(k_new)
+    if rows > 1 and _ld(v_new) != ld:
         raise RuntimeError("k_new and v_new must have one row stride")
-    sp, bound = _start_arg("start", start, c.n_seq, max_start if max_start is not None else c.max_seq, dev)
-    a = L.Kv4AppendArgs(c, k_new.shape[0] // c.n_seq, bound, _dt(k_new), 0, sp, k_new.data_ptr(), v_new.data_ptr(),
-                        _ld(k_new), _rope_arg(rope_cs, k_new.shape[0], c.head_dim, dev))
+    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq, dev)
+    rope = None if rope_cs is None else _vec("rope_cs", rope_cs, rows * c.head_dim, torch.float32, dev)
+    a = L.Kv4AppendArgs(c, rows // c.n_seq, bound, _DTYPE[k_new.dtype], 0, sp, k_new.data_ptr(), v_new.data_ptr(), ld,
+                        rope)
     with _on(dev) as st:
         L.check(lib().lbx_kv4_append(ctypes.byref(a), st), "kv4_append")
 
 
 def kv4_read(cache: Kv4Cache, start, max_start: Optional[int], n: int):
     """The values of n slots of every sequence: (k, v) float32 [S, kv_heads, n, head_dim]."""
-    c = cache.struct()
-    dev = cache.k_codes.device
-    sp, bound = _start_arg("start", start, c.n_seq, max_start if max_start is not None else c.max_seq, dev)
-    k = torch.empty(c.n_seq, c.kv_heads, n, c.head_dim, dtype=torch.float32, device=dev)
-    v = torch.empty_like(k)
+    c, dev = cache.struct(), cache.index
+    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq, dev)
+    kv = torch.empty(2, c.n_seq, c.kv_heads, n, c.head_dim, dtype=torch.float32, device=cache.k_codes.device)
+    k, v = kv.unbind(0)
     with _on(dev) as st:
         L.check(lib().lbx_kv4_read(ctypes.byref(c), sp, bound, n, k.data_ptr(), v.data_ptr(), st), "kv4_read")
     return k, v
@@ -783,28 +796,27 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional
     bounded by ``max_prefix``.  A query sees its sequence's cached slots and the
     new ones up to itself, or those of its ``tree_mask`` bits (int64 [S * n], n <= 64).
     A query that sees nothing gives zeros.  Result: q's shape and type."""
-    c = cache.struct()
+    c, dev = cache.struct(), cache.index
     _rows("q", q)
-    dev = cache.k_codes.device
-    if q.device != dev:
+    rows, width = q.shape
+    if q.get_device() != dev:
         raise RuntimeError("q and the cache must be on one device")
-    if q.shape[0] == 0 or q.shape[0] % c.n_seq or q.shape[1] != heads * c.head_dim:
+    if rows == 0 or rows % c.n_seq or width != heads * c.head_dim:
         raise RuntimeError(f"q must be [{c.n_seq} * n, {heads * c.head_dim}], got {tuple(q.shape)}")
-    pp, bound = _start_arg("prefix", prefix, c.n_seq, max_prefix if max_prefix is not None else c.max_seq, dev)
-    tm = None
-    if tree_mask is not None:
-        tm = _vec("tree_mask", tree_mask, q.shape[0], torch.int64, dev).data_ptr()
+    pp, bound = _start_arg("prefix", prefix, c.n_seq, max_prefix, c.max_seq, dev)
+    rope = None if rope_cs is None else _vec("rope_cs", rope_cs, rows * c.head_dim, torch.float32, dev)
+    tm = None if tree_mask is None else _vec("tree_mask", tree_mask, rows, torch.int64, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _cuda("out", out)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise RuntimeError(f"out must have q's shape, type and device")
-    a = L.Kv4AttnArgs(c, q.shape[0] // c.n_seq, heads, bound, _dt(q), 0, float(scale), pp, q.data_ptr(), _ld(q),
-                      _rope_arg(rope_cs, q.shape[0], c.head_dim, dev), tm, out.data_ptr())
+        out = torch.empty((rows, width), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous, with q's shape, type and device")
+    a = L.Kv4AttnArgs(c, rows // c.n_seq, heads, bound, _DTYPE[q.dtype], 0, scale, pp, q.data_ptr(), _ld(q), rope, tm,
+                      out.data_ptr())
     with _on(dev) as st:
-        ws = _stream_ws(dev, "kv4", st, max(1, int(lib().lbx_kv4_attn_workspace_size(ctypes.byref(a)))))
-        L.check(lib().lbx_kv4_attn(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "attention_kv4")
+        cl = lib()
+        ref = ctypes.byref(a)
+        ws = _stream_ws(dev, "kv4", st, cl.lbx_kv4_attn_workspace_size(ref) or 1)
+        L.check(cl.lbx_kv4_attn(ref, ws.data_ptr(), ws.numel(), st), "attention_kv4")
     return out
 
 
@@ -824,48 +836,38 @@ def accept_sampled(tokens: Optional[torch.Tensor], target_logits: torch.Tensor, 
     with fewer drafts.  With k = 0 (tokens, draft_logits and u None or empty) it
     draws next from softmax(target_logits[:, 0] / temperature)."""
     t = target_logits
-    if t.dim() != 3 or not t.is_cuda:
-        raise RuntimeError("target_logits must be a CUDA tensor [S, k + 1, V]")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 3 or t.dtype not in _FLOATS:
+        raise RuntimeError("target_logits must be a float32 or bfloat16 CUDA tensor [S, k + 1, V]")
     S, k1, V = t.shape
-    k, dev, dt = k1 - 1, t.device, _dt(t)
+    k, dev = k1 - 1, t.get_device()
     if k < 0 or V < 1:
         raise RuntimeError("target_logits must be [S, k + 1, V] with V >= 1")
 
     def plane(name, x, shape, dtype):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.device != dev:
-            raise RuntimeError(f"{name} must be a tensor on {dev}")
-        if tuple(x.shape) != shape or x.dtype != dtype:
+        if not isinstance(x, torch.Tensor) or x.get_device() != dev:
+            raise RuntimeError(f"{name} must be a tensor on cuda:{dev}")
+        if x.shape != shape or x.dtype != dtype:
             raise RuntimeError(f"{name} must be {shape} {dtype}, got {tuple(x.shape)} {x.dtype}")
-        if x.shape[-1] > 1 and x.stride(-1) != 1:
+        st = x.stride()
+        if st[-1] != 1 and shape[-1] > 1:
             raise RuntimeError(f"{name} must be contiguous along its last dimension")
-        return x
+        return x.data_ptr(), *st[:-1]
 
-    plane("target_logits", t, (S, k1, V), t.dtype)
-    plane("e", e, (S, V), torch.float32)
+    tp = plane("target_logits", t, (S, k1, V), t.dtype)
+    ep = plane("e", e, (S, V), torch.float32)
+    tk, up, dp, nd, temps = (None, 0), (None, 0), (None, 0, 0), None, None
     if k:
-        plane("tokens", tokens, (S, k), torch.int64)
-        plane("u", u, (S, k), torch.float32)
+        tk = plane("tokens", tokens, (S, k), torch.int64)
+        up = plane("u", u, (S, k), torch.float32)
         if draft_logits is not None:
-            plane("draft_logits", draft_logits, (S, k, V), t.dtype)
-    d = draft_logits if k else None
-    a = L.AcceptArgs()
-    a.n_seq, a.k, a.vocab, a.dtype = S, k, V, dt
-    if isinstance(temperature, torch.Tensor):
-        a.temps = _vec("temperature", temperature, S, torch.float32, dev).data_ptr()
-    else:
-        a.temperature = float(temperature)
-    if k:
-        a.tokens, a.tokens_ld = tokens.data_ptr(), tokens.stride(0)
-        a.u, a.u_ld = u.data_ptr(), u.stride(0)
+            dp = plane("draft_logits", draft_logits, (S, k, V), t.dtype)
         if n_draft is not None:
-            a.n_draft = _vec("n_draft", n_draft, S, torch.int32, dev).data_ptr()
-    a.target, a.target_seq, a.target_row = t.data_ptr(), t.stride(0), t.stride(1)
-    if d is not None:
-        a.draft, a.draft_seq, a.draft_row = d.data_ptr(), d.stride(0), d.stride(1)
-    a.e, a.e_ld = e.data_ptr(), e.stride(0)
-    res = torch.empty(2, S, dtype=torch.int64, device=dev)
-    a.accepted = res.data_ptr()
-    a.next = res.data_ptr() + 8 * S
+            nd = _vec("n_draft", n_draft, S, torch.int32, dev)
+    if isinstance(temperature, torch.Tensor):
+        temps, temperature = _vec("temperature", temperature, S, torch.float32, dev), 0.0
+    res = torch.empty((2, S), dtype=torch.int64, device=t.device)
+    rp = res.data_ptr()
+    a = L.AcceptArgs(S, k, V, _DTYPE[t.dtype], 0, temperature, temps, *tk, nd, *tp, *dp, *up, *ep, rp, rp + 8 * S)
     with _on(dev) as st:
         L.check(lib().lbx_accept_sampled(ctypes.byref(a), st), "accept_sampled")
-    return res[0], res[1]
+    return res.unbind(0)
