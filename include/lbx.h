@@ -347,6 +347,11 @@ typedef struct lbx_model {
   const lbx_layer *layers; /* host array [n_layers] */
   int32_t exec_mode;       /* LBX_EXEC_*: how lbx_forward runs a step */
   int32_t _pad2;
+  const struct lbx_kv4_cache *kv4; /* host array [n_layers]: keys and values are held
+                                    * in 4 bits (lbx_kv4_append, lbx_kv4_attn) and the
+                                    * layers' bf16 caches are not used; each has the
+                                    * step's n_seq, and the model's kv_heads, max_seq and
+                                    * head_dim.  NULL: bf16 caches.  Kernel path only.  */
 } lbx_model;
 
 /* lbx_forward execution: the kernel path launches one grid per op (chained

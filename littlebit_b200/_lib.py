@@ -68,6 +68,13 @@ class Layer(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", c_void_p), ("k_params", c_void_p), ("v_codes", c_void_p), ("v_params", c_void_p),
+        ("n_seq", c_int32), ("kv_heads", c_int32), ("max_seq", c_int32), ("head_dim", c_int32),
+    ]
+
+
 class Model(ctypes.Structure):
     _fields_ = [
         ("n_layers", c_int32), ("hidden", c_int32), ("intermediate", c_int32),
@@ -77,7 +84,7 @@ class Model(ctypes.Structure):
         ("use_pdl", c_int32),
         ("embed", c_void_p), ("final_norm", c_void_p), ("lm_head", c_void_p),
         ("layers", POINTER(Layer)),
-        ("exec_mode", c_int32), ("_pad2", c_int32),
+        ("exec_mode", c_int32), ("_pad2", c_int32), ("kv4", POINTER(Kv4Cache)),
     ]
 
 
@@ -86,13 +93,6 @@ class Int8Args(ctypes.Structure):
         ("m", c_int32), ("n", c_int32), ("k", c_int32), ("x_dtype", c_int32), ("y_dtype", c_int32),
         ("use_pdl", c_int32), ("x", c_void_p), ("x_ld", c_int64), ("w", c_void_p), ("w_ld", c_int64),
         ("w_scale", c_void_p), ("bias", c_void_p), ("y", c_void_p), ("y_ld", c_int64),
-    ]
-
-
-class Kv4Cache(ctypes.Structure):
-    _fields_ = [
-        ("k_codes", c_void_p), ("k_params", c_void_p), ("v_codes", c_void_p), ("v_params", c_void_p),
-        ("n_seq", c_int32), ("kv_heads", c_int32), ("max_seq", c_int32), ("head_dim", c_int32),
     ]
 
 

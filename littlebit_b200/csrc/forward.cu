@@ -23,10 +23,38 @@ constexpr int FWD_MAX_SEQ = 64;     // independent sequences per multi-sequence 
 
 struct FwdLayout {
   size_t tk, sw, x, q, kk, vv, att, gate, up, pos, rope, lin, attn, lm, total;
-  size_t lin_bytes, attn_bytes, lm_bytes;
+  size_t kv4;
+  size_t lin_bytes, attn_bytes, lm_bytes, kv4_bytes;
 };
 
 static size_t al(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// the 4-bit attention of a step of n tokens at layer l
+static lbx_kv4_attn_args kv4_attn_args(const lbx_model *m, int l, int n, int max_prefix) {
+  lbx_kv4_attn_args a = {};
+  a.cache = m->kv4[l];
+  a.n = n;
+  a.heads = m->heads;
+  a.max_prefix = max_prefix;
+  a.dtype = LBX_F32;
+  a.use_pdl = m->use_pdl;
+  a.scale = m->attn_scale;
+  a.q_ld = (int64_t)m->heads * m->head_dim;
+  return a;
+}
+
+// the caches of a step of S sequences fit the model
+static int kv4_check(const lbx_model *m, int S) {
+  for (int l = 0; m->kv4 && l < m->n_layers; ++l) {
+    const lbx_kv4_cache &c = m->kv4[l];
+    LBX_CHECK_ARG(c.n_seq == S && c.kv_heads == m->kv_heads && c.max_seq == m->max_seq && c.head_dim == m->head_dim,
+                  "the 4-bit cache of layer %d does not fit the model and the step's sequences", l);
+    Kv4View v;
+    const int rc = kv4_view(c, v);
+    if (rc) return rc;
+  }
+  return LBX_OK;
+}
 
 // n tokens of each of S sequences (S = 1: one sequence)
 static FwdLayout fwd_layout(const lbx_model *m, int n, int S = 1) {
@@ -67,8 +95,13 @@ static FwdLayout fwd_layout(const lbx_model *m, int n, int S = 1) {
   aa.kv_heads = m->kv_heads;
   aa.head_dim = m->head_dim;
   aa.prefix_len = m->max_seq - n;
-  L.attn_bytes = attn_partial_bytes(&aa, nullptr);
+  L.attn_bytes = m->kv4 ? 0 : attn_partial_bytes(&aa, nullptr);
   L.attn = take(L.attn_bytes);
+  if (m->kv4) {
+    lbx_kv4_attn_args ka = kv4_attn_args(m, 0, n, m->max_seq - n);
+    L.kv4_bytes = lbx_kv4_attn_workspace_size(&ka);
+  }
+  L.kv4 = take(L.kv4_bytes);
   L.lm_bytes = lbx_lmhead_workspace_size(T, m->vocab);
   L.lm = take(L.lm_bytes);
   L.total = off;
@@ -190,34 +223,58 @@ static int forward_chunk(const lbx_model *m, const int64_t *tokens, int32_t n, i
     rc = lbx_linear_verify(ly.proj + 0, &a, lin, L.lin_bytes, stream);
     if (rc) return rc;
     // attention with RoPE and KV write
-    lbx_attn_args aa = {};
-    aa.n = n;
-    aa.heads = m->heads;
-    aa.kv_heads = m->kv_heads;
-    aa.head_dim = m->head_dim;
-    aa.max_seq = m->max_seq;
-    aa.prefix_len = start;
-    aa.prefix_dev = start_dev;
-    aa.scale = m->attn_scale;
-    aa.theta = m->rope_theta;
-    aa.use_pdl = pdl;
-    aa.q = q;
-    aa.k_new = kk;
-    aa.v_new = vv;
-    aa.pos = pos;
-    aa.tree_mask = tree_mask;
-    aa.rope_cs = rope;
-    aa.k_cache = ly.k_cache;
-    aa.v_cache = ly.v_cache;
-    aa.out = att;
-    if (S > 1) {
-      aa.n_seq = S;
-      aa.prefix_seq = start_seq;
-      aa.cache_seq_stride = seq_stride;
-      aa.prefix_dev = nullptr;
+    if (m->kv4) {
+      lbx_kv4_append_args ap = {};
+      ap.cache = m->kv4[l];
+      ap.n = n;
+      ap.max_start = start;
+      ap.dtype = LBX_F32;
+      ap.use_pdl = pdl;
+      ap.start = S > 1 ? start_seq : start_dev;
+      ap.k_new = kk;
+      ap.v_new = vv;
+      ap.kv_ld = (int64_t)m->kv_heads * m->head_dim;
+      ap.rope_cs = rope;
+      rc = lbx_kv4_append(&ap, stream);
+      if (rc) return rc;
+      lbx_kv4_attn_args ka = kv4_attn_args(m, l, n, start);
+      ka.prefix = ap.start;
+      ka.q = q;
+      ka.rope_cs = rope;
+      ka.tree_mask = tree_mask;
+      ka.out = att;
+      rc = lbx_kv4_attn(&ka, w + L.kv4, L.kv4_bytes, stream);
+      if (rc) return rc;
+    } else {
+      lbx_attn_args aa = {};
+      aa.n = n;
+      aa.heads = m->heads;
+      aa.kv_heads = m->kv_heads;
+      aa.head_dim = m->head_dim;
+      aa.max_seq = m->max_seq;
+      aa.prefix_len = start;
+      aa.prefix_dev = start_dev;
+      aa.scale = m->attn_scale;
+      aa.theta = m->rope_theta;
+      aa.use_pdl = pdl;
+      aa.q = q;
+      aa.k_new = kk;
+      aa.v_new = vv;
+      aa.pos = pos;
+      aa.tree_mask = tree_mask;
+      aa.rope_cs = rope;
+      aa.k_cache = ly.k_cache;
+      aa.v_cache = ly.v_cache;
+      aa.out = att;
+      if (S > 1) {
+        aa.n_seq = S;
+        aa.prefix_seq = start_seq;
+        aa.cache_seq_stride = seq_stride;
+        aa.prefix_dev = nullptr;
+      }
+      rc = attn_launch(&aa, attn_part, attn_tk, stream);
+      if (rc) return rc;
     }
-    rc = attn_launch(&aa, attn_part, attn_tk, stream);
-    if (rc) return rc;
     // x += o(att)
     lbx_linear_args o = {};
     o.exec = a.exec;
@@ -503,6 +560,8 @@ extern "C" int lbx_forward_multi(const lbx_model *m, const int64_t *tokens, int3
   LBX_CHECK_ARG(m->embed && m->final_norm, "embed/final_norm required");
   LBX_CHECK_ARG(!(logits || argmax_out) || m->lm_head, "lm_head required for logits/argmax");
   LBX_CHECK_SUP(m->exec_mode != LBX_EXEC_PROGRAM, "multi-sequence steps run on the kernel path");
+  const int kc = kv4_check(m, n_seq);
+  if (kc) return kc;
   const size_t need = fwd_layout(m, n, n_seq).total;
   LBX_CHECK_ARG(ws && ws_bytes >= need, "workspace too small (%zu < %zu)", ws_bytes, need);
   return forward_chunk(m, tokens, n, max_start, nullptr, pos, tree_mask, hidden_out, logits, argmax_out, ws,
@@ -522,6 +581,9 @@ extern "C" int lbx_forward(const lbx_model *m, const int64_t *tokens, int32_t n,
   LBX_CHECK_ARG(!(logits || argmax_out) || m->lm_head, "lm_head required for logits/argmax");
   LBX_CHECK_ARG(n <= FWD_MAX_TOKENS || (!tree_mask && !start_dev),
                 "more than %d tokens only as a causal run at a host-given start", FWD_MAX_TOKENS);
+  LBX_CHECK_SUP(!m->kv4 || m->exec_mode != LBX_EXEC_PROGRAM, "a 4-bit cache runs on the kernel path");
+  const int kc = kv4_check(m, 1);
+  if (kc) return kc;
   const size_t need = fwd_layout(m, n < FWD_MAX_TOKENS ? n : FWD_MAX_TOKENS).total;
   LBX_CHECK_ARG(ws && ws_bytes >= need, "workspace too small (%zu < %zu)", ws_bytes, need);
   LBX_CHECK_ARG(m->exec_mode >= LBX_EXEC_AUTO && m->exec_mode <= LBX_EXEC_PROGRAM, "bad exec_mode");

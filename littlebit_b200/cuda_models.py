@@ -72,10 +72,8 @@ def _branch0_view(dec: LittleBitDecoder, max_seq: int) -> LittleBitDecoder:
         v.layers.append({"ln1": ly["ln1"], "ln2": ly["ln2"],
                          "projs": [PackedLinear(p.in_features, p.out_features, p.branches[:1], p.bias)
                                    for p in ly["projs"]]})
-    s = dec.shape
-    kvs = (s.num_key_value_heads, max_seq, s.head_dim)
-    v.k_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dec.device) for _ in v.layers]
-    v.v_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dec.device) for _ in v.layers]
+    v.kv_bits = dec.kv_bits
+    v._alloc_cache()
     v._build_struct()
     v._ws = torch.zeros(0, dtype=torch.uint8, device=dec.device)
     v._ws_n = 0
@@ -101,6 +99,8 @@ class _Unit:
             self.dec.step(tokens[a:b], start + a, **kw)
 
     def kv_move(self, src: torch.Tensor, dst: torch.Tensor):
+        if self.dec.kv_bits != 16:
+            raise RuntimeError("tree verification moves cache rows, which needs a bf16 cache (kv_bits=16)")
         s = self.dec.shape
         L.check(lib().lbx_kv_move(_p(self.kc_ptrs), _p(self.vc_ptrs), len(self.dec.layers),
                                   s.num_key_value_heads, self.dec.max_seq, s.head_dim, _p(src), _p(dst),

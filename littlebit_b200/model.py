@@ -32,7 +32,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from . import _lib as L
-from .ops import Branch, PackedLinear, _p, _stream, lib
+from .ops import Branch, Kv4Cache, PackedLinear, _p, _stream, lib
 
 PROJ_NAMES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
@@ -105,13 +105,18 @@ class LittleBitDecoder:
     def __init__(self, shape: DecoderShape, state: Dict[str, torch.Tensor], device="cuda",
                  max_seq: int = 4096, include_residual: bool = True, use_pdl: bool = True,
                  lm_head: Optional[torch.Tensor] = None, embed: Optional[torch.Tensor] = None,
-                 exec_mode: int = L.LBX_EXEC_AUTO):
+                 exec_mode: int = L.LBX_EXEC_AUTO, kv_bits: int = 16):
         """``exec_mode``: LBX_EXEC_AUTO / LBX_EXEC_KERNELS launch one grid per
         op; LBX_EXEC_PROGRAM runs a step of up to 16 tokens as one persistent
-        cooperative program (same numerics)."""
+        cooperative program (same numerics).  ``kv_bits``: 16 holds keys and values
+        in bf16, 4 in 4-bit codes (ops.Kv4Cache; head_dim 64 or 128, max_seq rounded
+        up to a multiple of 64, kernel path)."""
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 4 or 16")
         self.shape = shape
         self.device = torch.device(device)
-        self.max_seq = int(max_seq)
+        self.kv_bits = kv_bits
+        self.max_seq = -(-int(max_seq) // 64) * 64 if kv_bits == 4 else int(max_seq)
         self.use_pdl = use_pdl
         self.exec_mode = exec_mode
         dev = self.device
@@ -141,12 +146,21 @@ class LittleBitDecoder:
                 "ln2": _f32(state[f"{pre}.post_attention_layernorm.weight"], dev),
                 "projs": projs,
             })
-        kvs = (shape.num_key_value_heads, self.max_seq, shape.head_dim)
-        self.k_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dev) for _ in self.layers]
-        self.v_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dev) for _ in self.layers]
+        self._alloc_cache()
         self._build_struct()
         self._ws = torch.zeros(0, dtype=torch.uint8, device=dev)
         self._ws_n = 0
+
+    def _alloc_cache(self):
+        """This decoder's own cache: bf16 [kv_heads, max_seq, head_dim] a layer, or 4-bit."""
+        s, dev = self.shape, self.device
+        self.k_cache, self.v_cache, self.kv4 = [], [], []
+        if self.kv_bits == 4:
+            self.kv4 = [Kv4Cache.empty(1, s.num_key_value_heads, self.max_seq, s.head_dim, dev) for _ in self.layers]
+            return
+        kvs = (s.num_key_value_heads, self.max_seq, s.head_dim)
+        self.k_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dev) for _ in self.layers]
+        self.v_cache = [torch.zeros(kvs, dtype=torch.bfloat16, device=dev) for _ in self.layers]
 
     # ---- native descriptors -------------------------------------------------
     def _build_struct(self):
@@ -158,8 +172,9 @@ class LittleBitDecoder:
             c.ln2 = _p(ly["ln2"])
             for j, pr in enumerate(ly["projs"]):
                 c.proj[j] = pr.proj
-            c.k_cache = _p(self.k_cache[i])
-            c.v_cache = _p(self.v_cache[i])
+            if self.kv_bits == 16:
+                c.k_cache = _p(self.k_cache[i])
+                c.v_cache = _p(self.v_cache[i])
         m = L.Model()
         m.n_layers = len(self.layers)
         m.hidden = s.hidden_size
@@ -178,6 +193,9 @@ class LittleBitDecoder:
         m.final_norm = _p(self.final_norm)
         m.lm_head = _p(self.lm_head)
         m.layers = ctypes.cast(self._layer_arr, ctypes.POINTER(L.Layer))
+        if self.kv4:
+            self._kv4_arr = (L.Kv4Cache * len(self.kv4))(*[c.struct() for c in self.kv4])
+            m.kv4 = ctypes.cast(self._kv4_arr, ctypes.POINTER(L.Kv4Cache))
         self._model = m
 
     def workspace(self, n: int) -> torch.Tensor:
