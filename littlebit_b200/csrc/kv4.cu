@@ -40,7 +40,7 @@ struct Kv4AppendParams {
 // both members of a rotation pair are D / 8 lanes apart, a group of 64 is 16
 // lanes, two lanes make a word of codes.  ROWS rows a warp at once, so that a
 // prompt's loads are in flight together (2048 tokens x 8 heads: 18.5 us with one row
-// through shared memory, 8.9 with four).
+// through shared memory, 13.7 with four in registers).
 constexpr int KP_MANY = 4;
 template <int D, int ROWS, int DT>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4AppendParams p) {
@@ -185,23 +185,28 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 //   q . k = sum_g [ step_g (sum_{d in g} q_d (c_d - 8)) + (least_g + 8 step_g) (sum_{d in g} q_d) ]
 //   o_d   = sum_j (p_j step_jg) (c_jd - 8) + sum_j p_j (least_jg + 8 step_jg)
 //
-// only the queries and p * step are rounded to fp16; they are brought to
-// [2^14, 2^15) by a power of two first (a query by its group's largest, p * step by the
-// largest step the row has seen).  A pair of codes becomes fp16 by two logic
-// operations at most and one exact subtraction.  Codes are centred because the
-// tensor cores round their sums towards zero, and sums of one sign drift: 4e-5 of the
-// result at 4000 slots, 6e-4 at 130 000, against 3e-7 and 5e-6.  The keys of bfloat16 calls
-// (64 terms a sum, drift 1e-6) keep c: in the low bits of a 16-bit lane it IS the
-// fp16 subnormal c * 2^-24, which the tensor cores multiply exactly.  Nibbles 1 and 3 are left
-// at 16 times their value.
+// only the queries and p * step are rounded to fp16; they are brought up by a power of
+// two first (a query by its row's largest, p * step by the largest step the row has seen).
+// The tensor cores round their sums towards zero, and over thousands of slots
+// that showed (4e-5 of the result at 4000 slots, 6e-4 at 130 000), so a sum on them
+// never runs longer than 64 dimensions or 32 slots, small terms first, and the rest is
+// ordinary additions.  float32 calls centre their codes (a pair of codes is two logic
+// operations at most and one exact subtraction): 3e-7 and 5e-6.  bfloat16 calls keep c: in
+// the low bits of a 16-bit lane it IS the fp16 subnormal c * 2^-24, which the tensor cores
+// multiply exactly.  Nibbles 1 and 3 are left at 16 times their value.
 // Codes are the A operand (16 slots x 16 dimensions of the keys, 16 dimensions x 16
 // slots of the values) and query rows the columns of B, eight to a column tile, so that
-// a decode step's few rows waste half a tile at most, the running sums take
-// D / 16 x 4 registers a column tile, and NT column tiles share the unpacked codes.
-// The weights reach B's layout by one 8 x 8 transposition (movmatrix) a tile.
-// (Rows as A measured 500 instructions per 16 slots, half of them moves and masks; this
-// form is half that, which is what bounds the kernel: 6.5 TB/s is 400 issue slots per 16
-// slots of 128-wide keys and values.)
+// a decode step's few rows waste half a tile at most and the running sums take 4
+// registers for 16 dimensions.  The weights reach B's layout by one 8 x 8 transposition
+// (movmatrix) a tile.  (Rows as A measured 500 instructions per 16 slots, half of them moves
+// and masks, and 206 us where this form takes 161; two column tiles a warp share the
+// unpacked codes but halve the warps: 341 us against 285 for five tiles.)
+//
+// What bounds it is issue: 330 (bf16) to 450 (float32) instructions per 16 slots and warp at
+// half an instruction a cycle, where 6.5 TB/s would be 400 cycles per 16 slots of
+// 128-wide keys and values.  Neither more warps (queries' fragments in shared memory, 16
+// a multiprocessor: 193 us for 161) nor longer steps (64 slots, 255 registers: 163) change that.
+//
 // float32 calls (SPLIT) take each query and weight in two fp16 terms, 22 bits;
 // bfloat16 ones in one, 11 bits against the result's 8.
 //
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 constexpr int KA_STEP = 32;     // slots a step of the softmax
 constexpr int KA_SLOTS = 64;    // slots a stage of the ring
 constexpr int KA_ST = 2;        // stages
-constexpr float KA_LAZY = 8.f;  // a row's reference moves when its maximum is 2^8 above it
+constexpr float KA_LAZY = 8.f;  // a row's reference moves when its maximum is 2^8 above it: o is rescaled once or twice a sub-chunk
 constexpr int KA_WARPS = 4;     // warps a block at most
 
 struct Kv4AttnParams {
@@ -374,10 +379,11 @@ LBX_DEV void kv4_load_q(const Kv4AttnParams &p, int64_t row, int hq, int j, bool
   for (int i = 0; i < D / 4; ++i) x[i] *= p.scale;
 }
 
-template <int D, bool SPLIT, int NT>
-__global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+template <int D, bool SPLIT>
+__global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int NG = D / KV4_G, NW = D / 32, NS = SPLIT ? 2 : 1;
-  constexpr int RT = 8 * NT;  // query rows a tile
+  constexpr int RT = 8;              // query rows a tile
+  constexpr int NK = KA_STEP / 8;    // slots of a step that a lane holds the weights of
   using Stage = Kv4Stage<D>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[KA_WARPS][KA_ST], empty[KA_WARPS][KA_ST];
@@ -444,23 +450,20 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   if (rt == 0 && lane == 0)
     for (; issued < KA_ST && issued < nst; ++issued) issue(issued);
 
-  // ---- the queries' fragments: lane (r, j) makes its dimensions of row r of each
-  // column tile; as accumulator columns it owns rows 2 j and 2 j + 1
-  uint32_t qb[NT][NS][2 * NW][2];
-  float fq[NT][2], qs[NT][2][NG];  // the queries' unit, and their sums in it
-  int qi[NT][2];                   // token index of the rows
-  bool rok[NT][2];
+  // ---- the queries' fragments: lane (r, j) makes its dimensions of row r; as
+  // accumulator columns it owns rows 2 j and 2 j + 1
+  uint32_t qb[NS][2 * NW][2];
+  float fq[2], qs[2][NG];  // the queries' unit, and their sums in it
+  int qi[2];               // token index of the rows
+  bool rok[2];
   const bool tree = p.tree != nullptr;
-  uint64_t mask[NT][2];
+  uint64_t mask[2];
   const int64_t qrow0 = (int64_t)s * p.n + p.i0;
-#pragma unroll
-  for (int u = 0; u < NT; ++u) {
+  {
     float x[D / 4];
-    {
-      const int R = tile * RT + 8 * u + r;
-      const bool ok = live_tile && R < p.R;
-      kv4_load_q<D>(p, qrow0 + (ok ? R / p.rep : 0), h * p.rep + (ok ? R % p.rep : 0), j, ok, x);
-    }
+    const int Rr = tile * RT + r;
+    const bool ok = live_tile && Rr < p.R;
+    kv4_load_q<D>(p, qrow0 + (ok ? Rr / p.rep : 0), h * p.rep + (ok ? Rr % p.rep : 0), j, ok, x);
     float mq = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) mq = fmaxf(mq, fabsf(x[i]));
@@ -478,13 +481,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
     for (int b = 0; b < 2; ++b) {  // (from the lanes that made rows 2 j + b)
       const int src = 4 * (2 * j + b);
-      fq[u][b] = __shfl_sync(0xffffffffu, unit, src);
+      fq[b] = __shfl_sync(0xffffffffu, unit, src);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) qs[u][b][g] = __shfl_sync(0xffffffffu, sum[g], src);
-      const int R = tile * RT + 8 * u + 2 * j + b;
-      rok[u][b] = live_tile && R < p.R;
-      qi[u][b] = p.i0 + (rok[u][b] ? R / p.rep : 0);
-      mask[u][b] = tree && rok[u][b] ? __ldg(p.tree + (int64_t)s * p.n + qi[u][b]) : 0ull;
+      for (int g = 0; g < NG; ++g) qs[b][g] = __shfl_sync(0xffffffffu, sum[g], src);
+      const int R = tile * RT + 2 * j + b;
+      rok[b] = live_tile && R < p.R;
+      qi[b] = p.i0 + (rok[b] ? R / p.rep : 0);
+      mask[b] = tree && rok[b] ? __ldg(p.tree + (int64_t)s * p.n + qi[b]) : 0ull;
     }
 #pragma unroll
     for (int t = 0; t < NW; ++t) {
@@ -494,33 +497,32 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
       for (int k = 0; k < 2; ++k) {  // (k step 2t + k: dimensions 2k, 2k+4 and 2k+1, 2k+5 of the block)
         const uint32_t b0 = f16x2(y[2 * k], y[2 * k + 4]), b1 = f16x2(y[2 * k + 1], y[2 * k + 5]);
-        qb[u][0][2 * t + k][0] = b0;
-        qb[u][0][2 * t + k][1] = b1;
+        qb[0][2 * t + k][0] = b0;
+        qb[0][2 * t + k][1] = b1;
         if constexpr (SPLIT) {
-          qb[u][1][2 * t + k][0] = f16x2_rest(b0, y[2 * k], y[2 * k + 4]);
-          qb[u][1][2 * t + k][1] = f16x2_rest(b1, y[2 * k + 1], y[2 * k + 5]);
+          qb[1][2 * t + k][0] = f16x2_rest(b0, y[2 * k], y[2 * k + 4]);
+          qb[1][2 * t + k][1] = f16x2_rest(b1, y[2 * k + 1], y[2 * k + 5]);
         }
       }
     }
   }
 
   const Kv4Masks km;
-  float o[NT][D / 16][4];  // row tile 4 g + q: dimensions 64 g + 8 r + 2 q (+ 1: the second half), rows 2 j, 2 j + 1
-  float m[NT][2], l[NT][2], om[NT][2][NG];  // reference of the weights, their sum, sum of weight * (least + 8 step)
-  int eo[NT][2];                            // exponent of the largest step seen
+  float o[D / 16][4];  // row tile 4 g + q: dimensions 64 g + 8 r + 2 q (+ 1: the second half), rows 2 j, 2 j + 1
+  float m[2], l[2], om[2][NG];  // reference of the weights, their sum, sum of weight * (least + 8 step)
+  int eo[2];                    // exponent of the largest step seen
+  float lim[2];                 // 2^(eo + 1)
   auto reset = [&]() {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
+    for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) o[u][i][0] = o[u][i][1] = o[u][i][2] = o[u][i][3] = 0.f;
+    for (int b = 0; b < 2; ++b) {
+      m[b] = -INFINITY;
+      l[b] = 0.f;
+      eo[b] = -112;
+      lim[b] = kv4_pow2(-111);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        m[u][b] = -INFINITY;
-        l[u][b] = 0.f;
-        eo[u][b] = -112;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) om[u][b][g] = 0.f;
-      }
+      for (int g = 0; g < NG; ++g) om[b][g] = 0.f;
     }
   };
   reset();
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       issue(issued++);
     __syncwarp();
     if (!__all_sync(0xffffffffu, wd_wait(&full[kg][st], (uint32_t)(i / KA_ST) & 1u, 0x804, abrt))) break;
-#pragma unroll 1
+#pragma unroll 1  // (two steps of code do not fit the instruction cache as well as one: 285 us a pass became 311)
     for (int hs = 0; hs < KA_SLOTS; hs += KA_STEP) {
       const int j0 = lo + i * KA_SLOTS + hs;
       if (j0 >= my_end) break;
@@ -541,10 +543,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       const uint32_t *skp = reinterpret_cast<const uint32_t *>(ring + st * Stage::BYTES + Stage::CB) + hs * NG;
       const uint8_t *sv = sk + Stage::CB + Stage::PB;
       const uint32_t *svp = skp + (Stage::CB + Stage::PB) / 4;
-      // ---- scores in the queries' unit: sc[u][2 a + k][b], slot 16 a + 8 k + kv4_key(r), row 2 j + b
-      float sc[NT][4][2];
+      // ---- scores in the queries' unit: sc[2 a + k][b], slot 16 a + 8 k + kv4_key(r), row 2 j + b
+      float sc[NK][2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int a = 0; a < NK / 2; ++a) {
         uint32_t w[2][NW];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -557,19 +559,28 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
             w[k][0] = v.x; w[k][1] = v.y;
           }
         }
-        float acc[NT][NG][4];
+        float acc[NG][4];
 #pragma unroll
-        for (int q = 0; q < 2 * NW; ++q) {
-          const uint32_t w0 = (q & 1) ? w[0][q / 2] >> 8 : w[0][q / 2], w1 = (q & 1) ? w[1][q / 2] >> 8 : w[1][q / 2];
-          const uint32_t a0 = kv4_kcode<SPLIT, 0>(km, w0), a1 = kv4_kcode<SPLIT, 0>(km, w1);
-          const uint32_t a2 = kv4_kcode<SPLIT, 1>(km, w0), a3 = kv4_kcode<SPLIT, 1>(km, w1);
+        for (int g = 0; g < NG; ++g) {
+          constexpr int KS = 2 * NW / NG;  // k steps of a group
+          uint32_t f[KS][4];
 #pragma unroll
-          for (int u = 0; u < NT; ++u) {
-            float (&d)[4] = acc[u][q * NG / (2 * NW)];
-            if (q % (2 * NW / NG) == 0) mma_f16_first(d, a0, a1, a2, a3, qb[u][0][q][0], qb[u][0][q][1]);
-            else mma_f16(d, a0, a1, a2, a3, qb[u][0][q][0], qb[u][0][q][1]);
-            if constexpr (SPLIT) mma_f16(d, a0, a1, a2, a3, qb[u][1][q][0], qb[u][1][q][1]);
+          for (int q = 0; q < KS; ++q) {
+            const int wi = (g * KS + q) / 2;
+            const uint32_t w0 = (q & 1) ? w[0][wi] >> 8 : w[0][wi], w1 = (q & 1) ? w[1][wi] >> 8 : w[1][wi];
+            f[q][0] = kv4_kcode<SPLIT, 0>(km, w0);
+            f[q][1] = kv4_kcode<SPLIT, 0>(km, w1);
+            f[q][2] = kv4_kcode<SPLIT, 1>(km, w0);
+            f[q][3] = kv4_kcode<SPLIT, 1>(km, w1);
           }
+#pragma unroll
+          for (int e = NS - 1; e >= 0; --e)  // (the small terms first)
+#pragma unroll
+            for (int q = 0; q < KS; ++q) {
+              const uint32_t(&b)[2] = qb[e][g * KS + q];
+              if (e == NS - 1 && q == 0) mma_f16_first(acc[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
+              else mma_f16(acc[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
+            }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -579,155 +590,151 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           for (int g = 0; g < NG; ++g) {
             const float sg = kv4_step(pp[g]), lg = SPLIT ? fmaf(8.f, sg, kv4_least(pp[g])) : kv4_least(pp[g]);
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                float &x = sc[u][2 * a + k][b];
-                x = fmaf(acc[u][g][2 * k + b], sg, g == 0 ? lg * qs[u][b][g] : fmaf(lg, qs[u][b][g], x));
-              }
+            for (int b = 0; b < 2; ++b) {
+              float &x = sc[2 * a + k][b];
+              x = fmaf(acc[g][2 * k + b], sg, g == 0 ? lg * qs[b][g] : fmaf(lg, qs[b][g], x));
+            }
           }
         }
       }
       // ---- the values' params of this lane's slots; what each row sees of the step
       const bool whole = j0 + KA_STEP <= prefix;
-      float sg[4][NG], lg[4][NG];
-      float sx[NT][2];
-      {
-        float a = 0.f;
+      float sg[NK][NG], lg[NK][NG];
+      float sx[2] = {0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          uint32_t pp[NG];
-          kv4_params<NG>(svp + (8 * t + kv4_key(r)) * NG, pp);
+      for (int t = 0; t < NK; ++t) {
+        uint32_t pp[NG];
+        kv4_params<NG>(svp + (8 * t + kv4_key(r)) * NG, pp);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            sg[t][g] = kv4_step(pp[g]);
-            lg[t][g] = fmaf(8.f, sg[t][g], kv4_least(pp[g]));
-            a = fmaxf(a, fabsf(sg[t][g]));  // (a NaN is passed over)
-          }
+        for (int g = 0; g < NG; ++g) {
+          sg[t][g] = kv4_step(pp[g]);
+          lg[t][g] = SPLIT ? fmaf(8.f, sg[t][g], kv4_least(pp[g])) : kv4_least(pp[g]);
+          sx[0] = fmaxf(sx[0], fabsf(sg[t][g]));  // (a NaN is passed over)
         }
-#pragma unroll
-        for (int u = 0; u < NT; ++u) sx[u][0] = sx[u][1] = a;
       }
+      sx[1] = sx[0];
       if (!whole) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int b = 0; b < 2; ++b) {
+          float a = 0.f;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            float a = 0.f;
+          for (int t = 0; t < NK; ++t) {
+            if (rok[b] && kv4_sees(j0 + 8 * t + kv4_key(r), prefix, p.n, qi[b], tree, mask[b])) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              if (rok[u][b] && kv4_sees(j0 + 8 * t + kv4_key(r), prefix, p.n, qi[u][b], tree, mask[u][b])) {
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                  a = fmaxf(a, fabsf(sg[t][g]));
-                  // what is not a number reaches the rows that see it, and (below) no other
-                  if (!(fabsf(lg[t][g]) < INFINITY)) om[u][b][g] += __uint_as_float(0x7FC00000u);
-                }
-              } else {
-                sc[u][t][b] = -INFINITY;
+              for (int g = 0; g < NG; ++g) {
+                a = fmaxf(a, fabsf(sg[t][g]));
+                // what is not a number reaches the rows that see it, and (below) no other
+                if (!(fabsf(lg[t][g]) < INFINITY)) om[b][g] += __uint_as_float(0x7FC00000u);
               }
+            } else {
+              sc[t][b] = -INFINITY;
             }
-            sx[u][b] = a;
           }
+          sx[b] = a;
+        }
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < NK; ++t)
 #pragma unroll
           for (int g = 0; g < NG; ++g)
             if (!(fabsf(lg[t][g]) < INFINITY)) sg[t][g] = lg[t][g] = 0.f;
       }
       // ---- references: a row's moves when its maximum is 2^8 above it (or a step is above all before)
+      float mx[2];
       bool change = false;
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+      for (int b = 0; b < 2; ++b) {
+        mx[b] = sc[0][b];
+#pragma unroll
+        for (int t = 1; t < NK; ++t) mx[b] = fmaxf(mx[b], sc[t][b]);
+        change |= mx[b] * fq[b] > m[b] + KA_LAZY || sx[b] >= lim[b];
+      }
+      if (__any_sync(0xffffffffu, change)) {
+        float al[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float a = fmaxf(fmaxf(sc[u][0][b], sc[u][1][b]), fmaxf(sc[u][2][b], sc[u][3][b]));
-          change |= a * fq[u][b] > m[u][b] + KA_LAZY || kv4_exp(__float_as_uint(sx[u][b])) > eo[u][b];
+          const float top = col_max(mx[b]) * fq[b];
+          const int e = max(kv4_exp(__float_as_uint(col_max(sx[b]))), eo[b]);
+          const float mn = top > m[b] + KA_LAZY ? top : m[b];
+          al[b] = mn == m[b] ? 1.f : ex2(m[b] - mn);  // (from -inf: 0)
+          l[b] *= al[b];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) om[b][g] *= al[b];
+          al[b] *= kv4_pow2(max(eo[b] - e, -126));
+          m[b] = mn;
+          eo[b] = e;
+          lim[b] = kv4_pow2(e + 1);
         }
-      if (__any_sync(0xffffffffu, change)) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          float al[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float mx =
-                col_max(fmaxf(fmaxf(sc[u][0][b], sc[u][1][b]), fmaxf(sc[u][2][b], sc[u][3][b]))) * fq[u][b];
-            const int e = max(kv4_exp(__float_as_uint(col_max(sx[u][b]))), eo[u][b]);
-            const float mn = mx > m[u][b] + KA_LAZY ? mx : m[u][b];
-            al[b] = mn == m[u][b] ? 1.f : ex2(m[u][b] - mn);  // (from -inf: 0)
-            l[u][b] *= al[b];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) om[u][b][g] *= al[b];
-            al[b] *= kv4_pow2(max(eo[u][b] - e, -126));
-            m[u][b] = mn;
-            eo[u][b] = e;
-          }
-#pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            o[u][t][0] *= al[0];
-            o[u][t][1] *= al[1];
-            o[u][t][2] *= al[0];
-            o[u][t][3] *= al[1];
-          }
+        for (int t = 0; t < D / 16; ++t) {
+          o[t][0] *= al[0];
+          o[t][1] *= al[1];
+          o[t][2] *= al[0];
+          o[t][3] *= al[1];
         }
       }
-      // ---- weights (at most 2^8; with a step below 2^(eo + 1), times f, below 2^15), then 16 slots an MMA step
+      // ---- weights (at most 2^8; with a step below 2^(eo + 1), times f, below 2^15)
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+      for (int b = 0; b < 2; ++b) {
+        const float ref = m[b] == -INFINITY ? 0.f : m[b];  // (nothing seen so far: weights 0)
+        const float f = kv4_pow2(6 - eo[b]);
+        float sum = 0.f;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float ref = m[u][b] == -INFINITY ? 0.f : m[u][b];  // (nothing seen so far: weights 0)
+        for (int t = 0; t < NK; ++t) {
+          const float w = ex2(fmaf(sc[t][b], fq[b], -ref));
+          sum += w;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) sc[u][t][b] = ex2(fmaf(sc[u][t][b], fq[u][b], -ref));
-          l[u][b] += (sc[u][0][b] + sc[u][1][b]) + (sc[u][2][b] + sc[u][3][b]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) om[u][b][g] = fmaf(sc[u][t][b], lg[t][g], om[u][b][g]);
-          const float f = kv4_pow2(6 - eo[u][b]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) sc[u][t][b] *= f;
+          for (int g = 0; g < NG; ++g) om[b][g] = fmaf(w, lg[t][g], om[b][g]);
+          sc[t][b] = w * f;
         }
+        l[b] += sum;
+      }
+      // ---- values: 16 slots an MMA, the step's 32 in one sum, which joins the running one by ordinary additions
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        uint32_t vw[4][NG];
+      for (int g = 0; g < NG; ++g) {
+        uint32_t pb[NK / 2][NS][2], vw[NK / 2][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t *vr = sv + (16 * a + 8 * (k >> 1) + kv4_key(2 * j + (k & 1))) * (D / 2) + r * (D / 16);
-          if constexpr (D == 128) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(vr);
-            vw[k][0] = v.x;
-            vw[k][1] = v.y;
-          } else {
-            vw[k][0] = *reinterpret_cast<const uint32_t *>(vr);
+        for (int a = 0; a < NK / 2; ++a) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x0 = sc[2 * a + k][0] * sg[2 * a + k][g], x1 = sc[2 * a + k][1] * sg[2 * a + k][g];
+            const uint32_t hi = f16x2(x0, x1);
+            pb[a][0][k] = transpose8(hi);
+            if constexpr (SPLIT) pb[a][1][k] = transpose8(f16x2_rest(hi, x0, x1));
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            vw[a][k] = *reinterpret_cast<const uint32_t *>(
+                sv + (16 * a + 8 * (k >> 1) + kv4_key(2 * j + (k & 1))) * (D / 2) + r * (D / 16) + 4 * g);
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          uint32_t pb[NT][NS][2];
+        for (int hf = 0; hf < 2; ++hf) {  // nibbles 0-3, 4-7 of the word
+          uint32_t v[NK / 2][2];
 #pragma unroll
-          for (int u = 0; u < NT; ++u)
+          for (int a = 0; a < NK / 2; ++a)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float x0 = sc[u][2 * a + k][0] * sg[2 * a + k][g], x1 = sc[u][2 * a + k][1] * sg[2 * a + k][g];
-              const uint32_t hi = f16x2(x0, x1);
-              pb[u][0][k] = transpose8(hi);
-              if constexpr (SPLIT) pb[u][1][k] = transpose8(f16x2_rest(hi, x0, x1));
+            for (int k = 0; k < 2; ++k) v[a][k] = __byte_perm(vw[a][2 * k], vw[a][2 * k + 1], hf ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float t[4];
+            uint32_t f[NK / 2][4];
+#pragma unroll
+            for (int a = 0; a < NK / 2; ++a) {
+              f[a][0] = kv4_kcode<SPLIT, 0>(km, v[a][0]);
+              f[a][1] = kv4_kcode<SPLIT, 1>(km, v[a][0]);
+              f[a][2] = kv4_kcode<SPLIT, 0>(km, v[a][1]);
+              f[a][3] = kv4_kcode<SPLIT, 1>(km, v[a][1]);
+              v[a][0] >>= 8;
+              v[a][1] >>= 8;
             }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {  // nibbles 0-3, 4-7 of the word
-            uint32_t b0 = __byte_perm(vw[0][g], vw[1][g], hf ? 0x7632 : 0x5410);
-            uint32_t b1 = __byte_perm(vw[2][g], vw[3][g], hf ? 0x7632 : 0x5410);
+            for (int e = NS - 1; e >= 0; --e)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint32_t a0 = kv4_mid<0>(km, b0), a1 = kv4_mid<1>(km, b0), a2 = kv4_mid<0>(km, b1), a3 = kv4_mid<1>(km, b1);
+              for (int a = 0; a < NK / 2; ++a) {
+                if (e == NS - 1 && a == 0) mma_f16_first(t, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
+                else mma_f16(t, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
+              }
 #pragma unroll
-              for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int e = 0; e < NS; ++e) mma_f16(o[u][4 * g + 2 * hf + q], a0, a1, a2, a3, pb[u][e][0], pb[u][e][1]);
-              b0 >>= 8;
-              b1 >>= 8;
-            }
+            for (int i = 0; i < 4; ++i) o[4 * g + 2 * hf + q][i] += t[i];
           }
         }
       }
@@ -735,47 +742,45 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     __syncwarp();
     if (lane == 0) mbar_arrive1(&empty[kg][st]);
     const int j1 = lo + (i + 1) * KA_SLOTS;
-    if ((j1 % p.ck != 0 && i + 1 < nst) || (j1 - 1) / p.ck * p.ck >= my_end) continue;
+    if (j1 % p.ck != 0 && i + 1 < nst) continue;
+    const int c = (j1 - 1) / p.ck;
+    if (c * p.ck >= my_end) continue;
 
     // ---- the sub-chunk's (m, l, o): lane (r, j) holds dimensions 64 g + 8 r .. + 7 of rows 2 j, 2 j + 1
-    const int c = (j1 - 1) / p.ck;
     const bool single = p.nsub == 1;
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
+    for (int b = 0; b < 2; ++b) {
+      const float lsum = col_sum(l[b]);
+      float oms[NG];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float lsum = col_sum(l[u][b]);
-        float oms[NG];
+      for (int g = 0; g < NG; ++g) oms[g] = col_sum(om[b][g]);
+      if (!rok[b]) continue;
+      const int R = tile * RT + 2 * j + b;
+      const float dn = kv4_pow2(eo[b] - 6) * (SPLIT ? 1.f : 16777216.f);
+      const int64_t pr = (((int64_t)s * p.c.kvh + h) * p.nsub + c) * p.R + R;
+      const int64_t od = (((int64_t)s * p.n + qi[b]) * p.heads + h * p.rep + R % p.rep) * D;
+      if (!single && r == 0) p.part_ml[pr] = make_float2(m[b], lsum);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) oms[g] = col_sum(om[u][b][g]);
-        if (!rok[u][b]) continue;
-        const int R = tile * RT + 8 * u + 2 * j + b;
-        const float dn = kv4_pow2(eo[u][b] - 6);
-        const int64_t pr = (((int64_t)s * p.c.kvh + h) * p.nsub + c) * p.R + R;
-        const int64_t od = (((int64_t)s * p.n + qi[u][b]) * p.heads + h * p.rep + R % p.rep) * D;
-        if (!single && r == 0) p.part_ml[pr] = make_float2(m[u][b], lsum);
+      for (int g = 0; g < NG; ++g) {
+        float v[8];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float v[8];
+        for (int q = 0; q < 8; ++q) {
+          v[q] = fmaf(o[4 * g + q / 2][2 * (q & 1) + b], (q & 1) ? dn * 0.0625f : dn, oms[g]);
+          if (single) v[q] = lsum == 0.f ? 0.f : v[q] / lsum;  // (as the merge of one sub-chunk)
+        }
+        const int d = 64 * g + 8 * r;
+        if (!single || p.dtype == LBX_F32) {
+          float *dst = single ? reinterpret_cast<float *>(p.out) + od + d : p.part_o + pr * D + d;
+          reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          uint32_t w[4];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            v[q] = fmaf(o[u][4 * g + q / 2][2 * (q & 1) + b], (q & 1) ? dn * 0.0625f : dn, oms[g]);
-            if (single) v[q] = lsum == 0.f ? 0.f : v[q] / lsum;  // (as the merge of one sub-chunk)
-          }
-          const int d = 64 * g + 8 * r;
-          if (!single || p.dtype == LBX_F32) {
-            float *dst = single ? reinterpret_cast<float *>(p.out) + od + d : p.part_o + pr * D + d;
-            reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              w[q] = (uint32_t)f32_to_bf16(v[2 * q]) | (uint32_t)f32_to_bf16(v[2 * q + 1]) << 16;
-            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.out) + od + d) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)f32_to_bf16(v[2 * q]) | (uint32_t)f32_to_bf16(v[2 * q + 1]) << 16;
+          *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.out) + od + d) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+    }
     reset();
   }
   if (rt == 0 && lane == 0 && *abrt) {  // copies in flight land before shared memory is given up
@@ -786,12 +791,12 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 }
 
 // Merge of the sub-chunks' (m, l, o), one block a query row: warp w adds sub-chunks
-// w, w + 4, ... in order, a lane D / 32 dimensions, then the warps in order.
-constexpr int KM_BATCH = 8;  // partial sums loaded together
+// w, w + 8, ... in order, a lane D / 32 dimensions, then the warps in order.
+constexpr int KM_WARPS = 8, KM_BATCH = 8;  // warps, and partial results a lane loads together
 template <int D>
-__global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ Kv4AttnParams p) {
+__global__ void __launch_bounds__(KM_WARPS * 32) kv4_merge_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int V = D / 32;
-  __shared__ float red[4], wo[4][D], wl[4];
+  __shared__ float red[KM_WARPS], wo[KM_WARPS][D], wl[KM_WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int R = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
   const int i = p.i0 + R / p.rep, hq = h * p.rep + R % p.rep;
@@ -801,22 +806,24 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
   const int end = prefix + (p.tree ? p.n : i + 1), ns = bad ? 0 : (end + p.ck - 1) / p.ck;
   const int64_t base = ((int64_t)s * p.c.kvh + h) * p.nsub * p.R + R;
   float mx = -INFINITY;
-  for (int c = tid; c < ns; c += 128) mx = fmaxf(mx, __ldcg(p.part_ml + base + (int64_t)c * p.R).x);
+  for (int c = tid; c < ns; c += KM_WARPS * 32) mx = fmaxf(mx, __ldcg(p.part_ml + base + (int64_t)c * p.R).x);
   mx = warp_max(mx);
   if (lane == 0) red[warp] = mx;
   __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+  for (int w = 0; w < KM_WARPS; ++w) mx = fmaxf(mx, red[w]);
   float o[V], l = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) o[v] = 0.f;
-  for (int c0 = warp; c0 < ns; c0 += 4 * KM_BATCH) {
+  for (int c0 = warp; c0 < ns; c0 += KM_WARPS * KM_BATCH) {
     float2 ml[KM_BATCH];
     float x[KM_BATCH][V];
 #pragma unroll
     for (int b = 0; b < KM_BATCH; ++b) {
-      const int c = c0 + 4 * b;
+      const int c = c0 + KM_WARPS * b;
       ml[b] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[b][v] = 0.f;
       if (c < ns) {
         const int64_t pr = base + (int64_t)c * p.R;
         ml[b] = __ldcg(p.part_ml + pr);
@@ -826,8 +833,8 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
     }
 #pragma unroll
     for (int b = 0; b < KM_BATCH; ++b) {
-      if (ml[b].x == -INFINITY && ml[b].y == 0.f) continue;  // (no sub-chunk, or one without a visible slot)
-      const float w = exp2f(ml[b].x - ref);
+      // (no sub-chunk, or nothing of it seen: nothing to add; a sum that is not a number stays one)
+      const float w = ml[b].x == -INFINITY ? 0.f : exp2f(ml[b].x - mx);
       l = fmaf(w, ml[b].y, l);
 #pragma unroll
       for (int v = 0; v < V; ++v) o[v] = fmaf(w, x[b][v], o[v]);
@@ -838,8 +845,12 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
   if (lane == 0) wl[warp] = l;
   __syncthreads();
   if (tid < D) {
-    const float lt = ((wl[0] + wl[1]) + wl[2]) + wl[3];
-    const float ot = ((wo[0][tid] + wo[1][tid]) + wo[2][tid]) + wo[3][tid];
+    float lt = 0.f, ot = 0.f;
+#pragma unroll
+    for (int w = 0; w < KM_WARPS; ++w) {
+      lt += wl[w];
+      ot += wo[w][tid];
+    }
     const float y = bad ? __uint_as_float(0x7FC00000u) : lt == 0.f ? 0.f : ot / lt;
     const int64_t d = (((int64_t)s * p.n + i) * p.heads + hq) * D + tid;
     if (p.dtype == LBX_F32) reinterpret_cast<float *>(p.out)[d] = y;
@@ -848,7 +859,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
 }
 
 // slots a sub-chunk: by the cache's size alone (a row's bits then do not depend
-// on the lengths a call is given), 32 sub-chunks of a full cache
+// on the lengths a call is given)
 static int kv4_sub_chunk(int max_seq) {
   int ck = 128;
   while (ck < 1024 && ck * 32 < max_seq) ck *= 2;
@@ -970,6 +981,26 @@ extern "C" int lbx_kv4_read(const lbx_kv4_cache *c, const int32_t *start, int32_
 }
 
 namespace lbx {
+// how a launch of nt tokens is cut
+static void kv4_cut(Kv4AttnParams &p, int i0, int nt) {
+  const int end = p.max_prefix + (p.tree ? p.n : i0 + nt);
+  p.ck = kv4_sub_chunk(p.c.max_seq);
+  p.i0 = i0;
+  p.R = nt * p.rep;
+  p.ntile = (p.R + 7) / 8;
+  p.nsub = (end + p.ck - 1) / p.ck;
+  // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
+  // queries' fragments (1500 instructions) are made once for all of them
+  const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
+  p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (48 * device_sm_count())));
+  // Row tiles a block, evenly (5 tiles, 64 sequences over 4000 slots: 469 us sharing the
+  // ring, 506 each with its own); with one sub-chunk a warp a tile has its own ring (5 tiles
+  // over 130 000 slots: 251 us, shared 285).  The warps left take further runs.
+  const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
+  p.rw = p.cpw == 1 ? 1 : (p.ntile + groups - 1) / groups;
+  p.kw = std::min(KA_WARPS / p.rw, (p.nsub + p.cpw - 1) / p.cpw);
+}
+
 // tokens a launch (its partial results stay within a gigabyte) and their bytes
 static int kv4_slice(const Kv4AttnParams &p, int D, int64_t &bytes) {
   const int ck = kv4_sub_chunk(p.c.max_seq), nsub = (p.max_prefix + p.n + ck - 1) / ck;
@@ -986,50 +1017,33 @@ static int kv4_slice(const Kv4AttnParams &p, int D, int64_t &bytes) {
 template <int D>
 static int kv4_attn_launch(Kv4AttnParams p, void *ws, bool pdl, cudaStream_t stream) {
   const bool split = p.dtype == LBX_F32;
-  p.ck = kv4_sub_chunk(p.c.max_seq);
   int64_t bytes = 0;
   const int sl = kv4_slice(p, D, bytes);
   static DevCache<int> attr;
   int unused = 0;
   int rc = attr.get(unused, [](int &) {
-    cudaError_t e = allow_max_smem(kv4_attn_kernel<D, true, 1>);
-    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, true, 2>);
-    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, 1>);
-    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false, 2>);
+    cudaError_t e = allow_max_smem(kv4_attn_kernel<D, true>);
+    if (e == cudaSuccess) e = allow_max_smem(kv4_attn_kernel<D, false>);
     return cuda_status(e, "kv4_attn smem attribute");
   });
   if (rc) return rc;
   for (int i0 = 0; i0 < p.n; i0 += sl) {
-    const int nt = std::min(sl, p.n - i0);
-    p.i0 = i0;
-    p.R = nt * p.rep;
-    p.nsub = (p.max_prefix + (p.tree ? p.n : i0 + nt) + p.ck - 1) / p.ck;
-    const bool two = p.R > 8;  // column tiles a warp: two share the unpacked codes
-    p.ntile = (p.R + (two ? 15 : 7)) / (two ? 16 : 8);
-    // row tiles a block, evenly; the warps left take further sub-chunks
-    const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
-    p.rw = (p.ntile + groups - 1) / groups;
-    // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
-    // queries' fragments (1500 instructions) are made once for all of them
-    const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
-    p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (36 * device_sm_count())));
-    const int runs = (p.nsub + p.cpw - 1) / p.cpw;
-    p.kw = std::min(KA_WARPS / p.rw, runs);
+    kv4_cut(p, i0, std::min(sl, p.n - i0));
     p.part_ml = reinterpret_cast<float2 *>(ws);
     const int64_t rows = (int64_t)p.c.n_seq * p.c.kvh * p.nsub * p.R;
     p.part_o = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(ws) + ((rows * 8 + 255) & ~(int64_t)255));
+    const int runs = (p.nsub + p.cpw - 1) / p.cpw;
     const int64_t gx = (int64_t)((runs + p.kw - 1) / p.kw) * ((p.ntile + p.rw - 1) / p.rw);
     LBX_CHECK_SUP(gx <= 0x7fffffff && p.c.kvh <= 65535 && p.c.n_seq <= 65535, "too many heads, sequences or rows");
     const dim3 grid((unsigned)gx, p.c.kvh, p.c.n_seq), block(32 * p.kw * p.rw);
     const size_t smem = (size_t)p.kw * KA_ST * Kv4Stage<D>::BYTES;
     const bool dep = pdl || i0 > 0;  // (every kernel here waits for the one before it)
-    auto go = [&](auto kern) { return launch(kern, grid, block, smem, stream, dep, p); };
-    const cudaError_t e = split ? (two ? go(kv4_attn_kernel<D, true, 2>) : go(kv4_attn_kernel<D, true, 1>))
-                                : (two ? go(kv4_attn_kernel<D, false, 2>) : go(kv4_attn_kernel<D, false, 1>));
-    rc = cuda_status(e, "kv4_attn launch");
+    rc = cuda_status(split ? launch(kv4_attn_kernel<D, true>, grid, block, smem, stream, dep, p)
+                           : launch(kv4_attn_kernel<D, false>, grid, block, smem, stream, dep, p),
+                     "kv4_attn launch");
     if (rc) return rc;
     if (p.nsub > 1) {
-      rc = cuda_status(launch(kv4_merge_kernel<D>, dim3(p.R, p.c.kvh, p.c.n_seq), dim3(128), 0, stream, true, p),
+      rc = cuda_status(launch(kv4_merge_kernel<D>, dim3(p.R, p.c.kvh, p.c.n_seq), dim3(KM_WARPS * 32), 0, stream, true, p),
                        "kv4_merge launch");
       if (rc) return rc;
     }
