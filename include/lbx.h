@@ -454,8 +454,9 @@ typedef struct lbx_int8_args {
 } lbx_int8_args;
 /* The sums are exact, so a token's bits depend neither on the other tokens of
  * the call nor on how the work is split.  The workspace must be zero-filled
- * once when it is allocated (split tiles add their integer partial sums there
- * and leave it at zero); calls sharing one are ordered on one stream. */
+ * once when it is allocated (it starts with the tickets of split tiles, which
+ * every call leaves at zero); calls sharing one are ordered on one stream.  A
+ * bounded wait that runs out records device error 0x821 .. 0x826. */
 size_t lbx_linear_int8_workspace_size(int32_t m, int32_t n, int32_t k);
 int lbx_linear_int8(const lbx_int8_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
 
@@ -527,7 +528,8 @@ typedef struct lbx_kv4_attn_args {
   const uint64_t *tree_mask; /* [n_seq * n] or NULL */
   void *out;
 } lbx_kv4_attn_args;
-/* Workspace: zero-filled once at allocation (it holds self-resetting tickets). */
+/* Workspace: any contents.  A bounded wait that runs out records device error
+ * 0x804 .. 0x806. */
 size_t lbx_kv4_attn_workspace_size(const lbx_kv4_attn_args *a /* host */);
 int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
 
@@ -540,8 +542,8 @@ int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_byte
  * a rejection (p_a where that is all zero) and p_k after none.  With e
  * exponentially distributed that is a draw from r.  k = 0 draws a token from
  * target_0: the sampler of the drafts themselves.  draft == NULL: the drafts
- * were not sampled (greedy or looked up), q_i is 1 at d_i.  T = 0: p and q are 1
- * at their first maximum.  A logit of -inf or NaN has probability 0; +inf
+ * were not sampled (greedy or looked up), q_i is 1 at d_i.  T = 0 (up to 1e-30): p
+ * and q are 1 at their first maximum.  A logit of -inf or NaN has probability 0; +inf
  * counts as the maximum, shared equally.  A row without any probability
  * rejects its draft, and gives the next token -1.  A draft outside the
  * vocabulary is rejected (device error 0x811), q_i then taken as it is.

@@ -229,6 +229,7 @@ struct Kv4AttnParams {
   int ck, nsub;        // slots a sub-chunk, sub-chunks of the longest sequence
   int kw, rw, ntile;   // warps' runs and row tiles a block, row tiles in all
   int cpw;             // sub-chunks a warp's run
+  int qvec;            // queries on 16 bytes
   float scale;         // times log2 e
   const int32_t *prefix;
   const void *q; int64_t q_ld;
@@ -359,16 +360,37 @@ LBX_DEV void kv4_load_q(const Kv4AttnParams &p, int64_t row, int hq, int j, bool
     const int b = D == 128 ? (t >> 1) * 8 + (t & 1) * 4 + j : t * 4 + j;
     const int64_t o = row * p.q_ld + (int64_t)hq * D + 8 * b;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[8 * t + i] = ok ? load_act(p.q, p.dtype, o + i) : 0.f;
+    for (int i = 0; i < 8; ++i) x[8 * t + i] = 0.f;
+    if (!ok) continue;
+    if (!p.qvec) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[8 * t + i] = load_act(p.q, p.dtype, o + i);
+    } else if (p.dtype == LBX_F32) {
+      const float4 *v = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.q) + o);
+      const float4 a = __ldg(v), c = __ldg(v + 1);
+      x[8 * t] = a.x; x[8 * t + 1] = a.y; x[8 * t + 2] = a.z; x[8 * t + 3] = a.w;
+      x[8 * t + 4] = c.x; x[8 * t + 5] = c.y; x[8 * t + 6] = c.z; x[8 * t + 7] = c.w;
+    } else {
+      const uint4 a = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) + o));
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[8 * t + 2 * i] = __uint_as_float(w[i] << 16);
+        x[8 * t + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
   }
   if (p.rope && ok) {
 #pragma unroll
     for (int t = 0; t < NW / 2; ++t) {
       const int b = t * 4 + j;  // (first half of the dimensions)
-      const float2 *cs = p.rope + row * (D / 2) + 8 * b;
+      const float4 *cs = reinterpret_cast<const float4 *>(p.rope + row * (D / 2) + 8 * b);
+      float4 cv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cv[i] = __ldg(cs + i);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 c = __ldg(cs + i);
+        const float2 c = (i & 1) ? make_float2(cv[i / 2].z, cv[i / 2].w) : make_float2(cv[i / 2].x, cv[i / 2].y);
         const float x1 = x[8 * t + i], x2 = x[8 * (t + NW / 2) + i];
         x[8 * t + i] = x1 * c.x - x2 * c.y;
         x[8 * (t + NW / 2) + i] = x2 * c.x + x1 * c.y;
@@ -905,6 +927,8 @@ static int kv4_attn_prep(const lbx_kv4_attn_args *a, Kv4AttnParams &p) {
   p.q = a->q;
   p.q_ld = a->q_ld;
   p.rope = reinterpret_cast<const float2 *>(a->rope_cs);
+  LBX_CHECK_ARG(aligned16(a->rope_cs), "rope_cs must be 16-byte aligned");
+  p.qvec = aligned16(a->q) && a->q_ld % (a->dtype == LBX_F32 ? 4 : 8) == 0;
   p.tree = a->tree_mask;
   p.out = a->out;
   return LBX_OK;
