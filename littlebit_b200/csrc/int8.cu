@@ -611,10 +611,10 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   p.ydt = a->y_dtype;
   p.part = reinterpret_cast<int32_t *>(b + W.part);
   p.ticket = reinterpret_cast<unsigned *>(b);
-  CUtensorMap tw, tw32, tx;
+  CUtensorMap tw, tw32 = {}, tx;  // (only the even deal copies 32 rows at a time)
   rc = i8_map(&tw, a->w, a->n, a->k, a->w_ld, 128);
   if (rc) return rc;
-  rc = i8_map(&tw32, a->w, a->n, a->k, a->w_ld, 32);
+  if (p.units) rc = i8_map(&tw32, a->w, a->n, a->k, a->w_ld, 32);
   if (rc) return rc;
   rc = i8_map(&tx, q, a->m, a->k, W.q_ld, p.BN);
   if (rc) return rc;

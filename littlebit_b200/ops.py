@@ -645,7 +645,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
             raise RuntimeError(f"out must be [{m}, {n}] on cuda:{dev}")
     if out.dtype not in _FLOATS:
         raise RuntimeError(f"unsupported result type {out.dtype} (float32 or bfloat16)")
-    a = L.Int8Args(m, n, k, _DTYPE[x.dtype], _DTYPE[out.dtype], 0, x.data_ptr(), _ld(x), weight.data_ptr(),
+    a = L.Int8Args(m, n, k, _DTYPE[x.dtype], _DTYPE[out.dtype], 1, x.data_ptr(), _ld(x), weight.data_ptr(),
                    _ld(weight), _vec("weight_scale", weight_scale, n, torch.float32, dev),
                    None if bias is None else _vec("bias", bias, n, torch.float32, dev), out.data_ptr(), _ld(out))
     with _on(dev) as st:
@@ -683,17 +683,32 @@ class Int8Linear:
 KV4_GROUP = 64
 
 
-@dataclass(frozen=True)
 class Kv4Cache:
     """Keys and values of S sequences in 4 bits: codes uint8 [S, kv_heads, max_seq,
     head_dim / 2] and, for each group of 64 dimensions, (step, least) bfloat16
     [S, kv_heads, max_seq, head_dim / 64, 2]; a value is least + step * code.
     The order of the codes is that of include/lbx.h; :func:`kv4_read` gives the
-    values back."""
-    k_codes: torch.Tensor
-    k_params: torch.Tensor
-    v_codes: torch.Tensor
-    v_params: torch.Tensor
+    values back.  A cache's tensors are fixed: its C descriptor is made once."""
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "index", "_struct")
+
+    def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor, v_params: torch.Tensor):
+        kc, kp, vc, vp = k_codes, k_params, v_codes, v_params
+        for t, ty in ((kc, torch.uint8), (vc, torch.uint8), (kp, torch.bfloat16), (vp, torch.bfloat16)):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is ty and t.is_contiguous()):
+                raise RuntimeError("codes must be contiguous uint8 CUDA tensors and params bfloat16 ones (the B200 "
+                                   "library has no CPU path)")
+        index = kc.get_device()
+        if not index == kp.get_device() == vc.get_device() == vp.get_device():
+            raise RuntimeError("cache tensors must be on one device")
+        shape, pshape = kc.shape, kp.shape
+        if len(shape) != 4 or len(pshape) != 5:
+            raise RuntimeError("codes must be 4-D and params 5-D")
+        S, H, T, D2 = shape
+        if vc.shape != shape or vp.shape != pshape or pshape != (S, H, T, 2 * D2 // KV4_GROUP, 2):
+            raise RuntimeError(f"cache shapes do not fit together: {tuple(kc.shape)} {tuple(kp.shape)} "
+                               f"{tuple(vc.shape)} {tuple(vp.shape)}")
+        self.k_codes, self.k_params, self.v_codes, self.v_params, self.index = kc, kp, vc, vp, index
+        self._struct = L.Kv4Cache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(), S, H, T, 2 * D2)
 
     @classmethod
     def empty(cls, n_seq: int, kv_heads: int, max_seq: int, head_dim: int, device="cuda") -> "Kv4Cache":
@@ -714,27 +729,8 @@ class Kv4Cache:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_params, self.v_codes, self.v_params))
 
-    def __post_init__(self):
-        kc, kp, vc, vp = self.k_codes, self.k_params, self.v_codes, self.v_params
-        for nm, t, ty in (("k_codes", kc, torch.uint8), ("v_codes", vc, torch.uint8),
-                          ("k_params", kp, torch.bfloat16), ("v_params", vp, torch.bfloat16)):
-            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == ty and t.is_contiguous()):
-                raise RuntimeError(f"{nm} must be a contiguous {ty} CUDA tensor (the B200 library has no CPU path)")
-        index = kc.get_device()
-        if not index == kp.get_device() == vc.get_device() == vp.get_device():
-            raise RuntimeError("cache tensors must be on one device")
-        if kc.dim() != 4 or kp.dim() != 5:
-            raise RuntimeError("codes must be 4-D and params 5-D")
-        S, H, T, D2 = kc.shape
-        if vc.shape != kc.shape or vp.shape != kp.shape or kp.shape != (S, H, T, 2 * D2 // KV4_GROUP, 2):
-            raise RuntimeError(f"cache shapes do not fit together: {tuple(kc.shape)} {tuple(kp.shape)} "
-                               f"{tuple(vc.shape)} {tuple(vp.shape)}")
-        object.__setattr__(self, "index", index)
-        object.__setattr__(self, "_struct", L.Kv4Cache(kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(),
-                                                       S, H, T, 2 * D2))
-
     def struct(self) -> L.Kv4Cache:
-        """The C descriptor (the tensors of a cache are fixed)."""
+        """The C descriptor."""
         return self._struct
 
 
@@ -768,7 +764,7 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start,
         raise RuntimeError("k_new and v_new must have one row stride")
     sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq, dev)
     rope = None if rope_cs is None else _vec("rope_cs", rope_cs, rows * c.head_dim, torch.float32, dev)
-    a = L.Kv4AppendArgs(c, rows // c.n_seq, bound, _DTYPE[k_new.dtype], 0, sp, k_new.data_ptr(), v_new.data_ptr(), ld,
+    a = L.Kv4AppendArgs(c, rows // c.n_seq, bound, _DTYPE[k_new.dtype], 1, sp, k_new.data_ptr(), v_new.data_ptr(), ld,
                         rope)
     with _on(dev) as st:
         L.check(lib().lbx_kv4_append(ctypes.byref(a), st), "kv4_append")
@@ -810,7 +806,7 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional
         out = torch.empty((rows, width), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise RuntimeError("out must be contiguous, with q's shape, type and device")
-    a = L.Kv4AttnArgs(c, rows // c.n_seq, heads, bound, _DTYPE[q.dtype], 0, scale, pp, q.data_ptr(), _ld(q), rope, tm,
+    a = L.Kv4AttnArgs(c, rows // c.n_seq, heads, bound, _DTYPE[q.dtype], 1, scale, pp, q.data_ptr(), _ld(q), rope, tm,
                       out.data_ptr())
     with _on(dev) as st:
         cl = lib()
@@ -846,7 +842,7 @@ def accept_sampled(tokens: Optional[torch.Tensor], target_logits: torch.Tensor, 
     def plane(name, x, shape, dtype):
         if not isinstance(x, torch.Tensor) or x.get_device() != dev:
             raise RuntimeError(f"{name} must be a tensor on cuda:{dev}")
-        if x.shape != shape or x.dtype != dtype:
+        if x.shape != shape or x.dtype is not dtype:
             raise RuntimeError(f"{name} must be {shape} {dtype}, got {tuple(x.shape)} {x.dtype}")
         st = x.stride()
         if st[-1] != 1 and shape[-1] > 1:
@@ -867,7 +863,7 @@ def accept_sampled(tokens: Optional[torch.Tensor], target_logits: torch.Tensor, 
         temps, temperature = _vec("temperature", temperature, S, torch.float32, dev), 0.0
     res = torch.empty((2, S), dtype=torch.int64, device=t.device)
     rp = res.data_ptr()
-    a = L.AcceptArgs(S, k, V, _DTYPE[t.dtype], 0, temperature, temps, *tk, nd, *tp, *dp, *up, *ep, rp, rp + 8 * S)
+    a = L.AcceptArgs(S, k, V, _DTYPE[t.dtype], 1, temperature, temps, *tk, nd, *tp, *dp, *up, *ep, rp, rp + 8 * S)
     with _on(dev) as st:
         L.check(lib().lbx_accept_sampled(ctypes.byref(a), st), "accept_sampled")
     return res.unbind(0)
