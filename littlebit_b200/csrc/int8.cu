@@ -209,14 +209,21 @@ LBX_DEV void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *b
       : "memory");
 }
 
-// results of 16 tokens from t on (nc of them in range) at channel ch.  The
-// tokens' scales are all loaded before the first store: a load behind a store
-// to memory that may be the same waits for its turn, and one such wait a token
-// (256 x 700 cycles a tile) held the whole kernel at a quarter of its rate.
-LBX_DEV void i8_store16(const I8Params &p, int64_t t, int nc, int ch, const int *acc, float wsc, float b, bool has_b) {
+// Results of 16 tokens from t on (nc of them in range) at channel ch; ts: the
+// tokens' scales, in shared memory since the piece began.  (A load from L2 behind a store
+// to memory that may be the same waits for its turn: one a token, 256 x 700 cycles a
+// tile, held the whole kernel at a quarter of its rate.)
+LBX_DEV void i8_store16(const I8Params &p, const float *ts, int64_t t, int nc, int ch, const int *acc, float wsc, float b,
+                        bool has_b) {
   float v[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = j < nc ? __ldcg(p.s + t + j) : 0.f;
+  for (int j = 0; j < 16; j += 4) {
+    const float4 s = *reinterpret_cast<const float4 *>(ts + j);
+    v[j] = s.x;
+    v[j + 1] = s.y;
+    v[j + 2] = s.z;
+    v[j + 3] = s.w;
+  }
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     v[j] = __int2float_rn(acc[j]) * v[j] * wsc;
@@ -235,6 +242,9 @@ LBX_DEV void i8_store16(const I8Params &p, int64_t t, int nc, int ch, const int 
   }
 }
 
+// ONE: one K block a stage (known, the copying and issuing threads have no inner
+// loops: each is one thread with some 500 cycles a block)
+template <bool ONE>
 __global__ void __launch_bounds__(I8_THREADS, 1)
     linear_int8_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tw32,
                        const __grid_constant__ CUtensorMap tx, const __grid_constant__ I8Params p) {
@@ -243,9 +253,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
   __shared__ __align__(8) uint64_t full[I8_MAXST], empty[I8_MAXST], tfull[2], tempty[2], drain;
   __shared__ uint32_t tbase;
   __shared__ int abort_flag, s_last;
+  __shared__ __align__(16) float tsc[2][256];  // the piece's token scales, and the next one's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
   // a stage: KS tiles of weights, then KS of tokens
-  const int abytes = 128 * I8_KB, bbytes = p.BN * I8_KB, stage = p.KS * (abytes + bbytes), boff = p.KS * abytes;
+  const int KS = ONE ? 1 : p.KS;
+  const int abytes = 128 * I8_KB, bbytes = p.BN * I8_KB, stage = KS * (abytes + bbytes), boff = KS * abytes;
   volatile int *abrt = &abort_flag;
   if (tid == 0) {
     for (int i = 0; i < p.ST; ++i) {
@@ -270,7 +282,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     // ---- copies.  The weights do not come from the kernel before this one:
     // the first stages' are on their way before its codes are waited for.
     auto load_w = [&](int st, const I8Piece &e, int kb) {
-      const int nk = min(p.KS, e.k1 - kb);
+      const int nk = min(KS, e.k1 - kb);
       mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * (e.rows * I8_KB + bbytes)));
       for (int i = 0; i < nk; ++i) {
         uint8_t *d = sm + st * stage + i * abytes;
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     {
       I8Pieces pre(p, cta);
       while (j < p.ST && pre.next(e))
-        for (int kb = e.k0; kb < e.k1 && j < p.ST; kb += p.KS) load_w(j++, e, kb);
+        for (int kb = e.k0; kb < e.k1 && j < p.ST; kb += KS) load_w(j++, e, kb);
     }
     const int npre = j;
     pdl_wait();
@@ -296,7 +308,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     j = 0;
     bool ok = true;
     while (ok && it.next(e)) {
-      for (int kb = e.k0; kb < e.k1; kb += p.KS, ++j) {
+      for (int kb = e.k0; kb < e.k1; kb += KS, ++j) {
         if (j >= npre) {
           if (!wd_wait(&empty[st], ph, 0x821, abrt)) {
             ok = false;
@@ -304,7 +316,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
           }
           load_w(st, e, kb);
         }
-        for (int i = 0; i < p.KS && kb + i < e.k1; ++i)
+        for (int i = 0; i < KS && kb + i < e.k1; ++i)
           tma_2d(sm + st * stage + boff + i * bbytes, &tx, (kb + i) * I8_KB, e.t0, &full[st]);
         if (++st == p.ST) {
           st = 0;
@@ -327,14 +339,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
       const uint32_t d = tmem + (uint32_t)(n & 1) * tbuf;
       if (n >= 2 && !wd_wait(&tempty[n & 1], (uint32_t)(n / 2 - 1) & 1u, 0x823, abrt)) break;
       tc_fence_after();
-      for (int kb = e.k0; kb < e.k1; kb += p.KS) {
+      for (int kb = e.k0; kb < e.k1; kb += KS) {
         if (!wd_wait(&full[st], ph, 0x824, abrt)) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint64_t a = sw128_desc(smem_u32(sm + st * stage)), b = sw128_desc(smem_u32(sm + st * stage + boff));
-        for (int i = 0; i < p.KS && kb + i < e.k1; ++i, a += abytes >> 4, b += bbytes >> 4) {
+        for (int i = 0; i < KS && kb + i < e.k1; ++i, a += abytes >> 4, b += bbytes >> 4) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)  // (32 bytes on: 2 in the descriptors' address units)
             umma_i8(d, a + 2 * q, b + 2 * q, p.idesc, kb + i > e.k0 || q > 0 ? 1u : 0u);
@@ -362,6 +374,9 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
     I8Piece e;
     int n = 0;
     while (it.next(e)) {
+      float *ts = tsc[n & 1];
+      for (int c = tid - 64; c < min(p.BN, p.m - e.t0); c += 128) ts[c] = __ldcg(p.s + e.t0 + c);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
       // (after a wait that gave up all four warps still go through the same
       // barriers: the pieces left then pass at once, and the call has failed)
       wd_wait(&tfull[n & 1], (uint32_t)(n / 2) & 1u, 0x826, abrt);
@@ -378,7 +393,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
         tmem_ld<16>(ta + c0, r);
         tmem_ld_wait();
         if (whole) {
-          if (cok) i8_store16(p, t0 + c0, nc - c0, ch, reinterpret_cast<const int *>(r), wsc, bs, hb);
+          if (cok) i8_store16(p, ts + c0, t0 + c0, nc - c0, ch, reinterpret_cast<const int *>(r), wsc, bs, hb);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
@@ -430,7 +445,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[j] += v[u][j];
         }
-        if (cok) i8_store16(p, t0 + c0, nc - c0, ch, acc, wsc, bs, hb);
+        if (cok) i8_store16(p, ts + c0, t0 + c0, nc - c0, ch, acc, wsc, bs, hb);
       }
     }
   }
@@ -592,7 +607,11 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   static DevCache<size_t> smax_cache;
   size_t smax = 0;
   int rc = smax_cache.get(smax, [](size_t &out) {
-    return cuda_status(allow_max_smem(linear_int8_kernel, &out), "linear_int8 smem attribute");
+    size_t o2 = 0;
+    cudaError_t e = allow_max_smem(linear_int8_kernel<true>, &out);
+    if (e == cudaSuccess) e = allow_max_smem(linear_int8_kernel<false>, &o2);
+    out = std::min(out, o2);
+    return cuda_status(e, "linear_int8 smem attribute");
   });
   if (rc) return rc;
   const int blk = (128 + p.BN) * I8_KB;
@@ -620,7 +639,8 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   if (rc) return rc;
   rc = quant_tokens_launch(a->x, a->x_dtype, a->x_ld, a->m, a->k, q, W.q_ld, s, a->use_pdl != 0, stream);
   if (rc) return rc;
-  return cuda_status(launch(linear_int8_kernel, dim3(p.G), dim3(I8_THREADS), (size_t)p.ST * stage + 1024, stream, true, tw,
-                            tw32, tx, p),
-                     "linear_int8 launch");
+  auto go = [&](auto kern) {
+    return launch(kern, dim3(p.G), dim3(I8_THREADS), (size_t)p.ST * stage + 1024, stream, true, tw, tw32, tx, p);
+  };
+  return cuda_status(p.KS == 1 ? go(linear_int8_kernel<true>) : go(linear_int8_kernel<false>), "linear_int8 launch");
 }

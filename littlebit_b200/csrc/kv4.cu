@@ -149,6 +149,7 @@ template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4ReadParams p) {
   constexpr uint32_t NB = D / 8;
   const bool value = blockIdx.z & 1;
+  pdl_wait();
   float *out = p.out[value];
   const uint32_t e = blockIdx.x * 256 + threadIdx.x, i = e / NB, b = e % NB;
   if (!out || i >= (uint32_t)p.n) return;
@@ -997,11 +998,10 @@ extern "C" int lbx_kv4_read(const lbx_kv4_cache *c, const int32_t *start, int32_
   const int64_t items = (int64_t)n * (c->head_dim / 8);
   LBX_CHECK_SUP(items <= 0x7fffffff && c->kv_heads <= 65535 && c->n_seq <= 32767, "too many rows");
   const dim3 grid((unsigned)((items + 255) / 256), c->kv_heads, 2 * c->n_seq);
-  if (c->head_dim == 128)
-    kv4_read_kernel<128><<<grid, 256, 0, stream>>>(p);
-  else
-    kv4_read_kernel<64><<<grid, 256, 0, stream>>>(p);
-  return cuda_status(cudaGetLastError(), "kv4_read launch");
+  // (the kernel waits for the one before it, so it may be launched while that runs)
+  return cuda_status(c->head_dim == 128 ? launch(kv4_read_kernel<128>, grid, dim3(256), 0, stream, true, p)
+                                        : launch(kv4_read_kernel<64>, grid, dim3(256), 0, stream, true, p),
+                     "kv4_read launch");
 }
 
 namespace lbx {

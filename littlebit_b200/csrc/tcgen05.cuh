@@ -113,11 +113,11 @@ LBX_DEV bool wd_wait(uint64_t *bar, uint32_t parity, int code, volatile int *abo
   uint64_t t0 = 0;
   for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 7u) == 0) {
+    if ((it & 7u) == 7) {  // (a wait that is soon over reads no clock)
       if (*abort) return false;
       uint64_t t;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (it == 0) t0 = t;
+      if (it == 7) t0 = t;
       else if (t - t0 > 1000000000ull) {
         *abort = 1;
         atomicCAS(&g_lbx_device_error, 0, code);
