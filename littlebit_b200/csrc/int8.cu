@@ -478,7 +478,11 @@ static I8Plan i8_plan(int m, int n, int k) {
   // at least), its bytes from L2 (37 a cycle and SM, measured with every SM
   // loading), its weights' share of memory (23.7 a cycle and SM, once for all token tiles).
   // A tile's results cost 20 cycles a token and 1000; a cut tile's parts go to
-  // L2 and back (40 bytes a cycle, 4000 cycles of latency).
+  // L2 and back (40 bytes a cycle, 12000 cycles of fences, tickets and latency), and
+  // CTAs that begin their rounds at different times share less in L2 (5 %).
+  // Both sides measured: 320 tokens x 32000 x 8192 103 us cut, 112 in rounds; 4096 x 28672
+  // x 8192 726 and 691; 128 x 4096 x 4096 30 and 24; 5 x 4096 x 28672 48 cut, 71 even; 16 x
+  // 4096 x 4096 24 and 19; 1 x 32000 x 4096 46 cut, 40 even.
   auto block = [&](int bn, int tm, int rows) {
     return std::max({324.0, 2.0 * bn, (rows + bn) * 128.0 / 37, rows * 128.0 / 23.7 / tm});
   };
@@ -508,7 +512,7 @@ static I8Plan i8_plan(int m, int n, int k) {
     if (take((double)((T + sms - 1) / sms) * tile)) set(T, 0, 1, 0);
     if (rb) {
       const double parts = 2 + (double)gr / (T - full);
-      if (take((double)(T / sms) * tile + (double)rb / gr * block(bn, tm, 128) + out + 4000 +
+      if (take((double)(T / sms) * tile * (tm > 1 ? 1.05 : 1) + (double)rb / gr * block(bn, tm, 128) + out + 12000 +
                parts * std::min(bn, m) * 512 / 40))
         set(full, rb, gr, 0);
     }
