@@ -38,103 +38,88 @@ struct Kv4AppendParams {
 
 // A row (one token's key or value of one head) is D / 4 lanes of four dimensions:
 // both members of a rotation pair are D / 8 lanes apart, a group of 64 is 16
-// lanes, two lanes make a word of codes.  ROWS rows a warp at once, so that a
-// prompt's loads are in flight together (2048 tokens x 8 heads: 18.5 us with one row
-// through shared memory, 13.7 with four in registers).
-constexpr int KP_MANY = 4;
-template <int D, int ROWS, int DT>
+// lanes, two lanes make a word of codes.  Bound by one round trip to memory (6.2 us for 64
+// rows) and, for a prompt, by instructions: 2048 tokens x 8 heads, 37 MB, 16.4 us.  (Several
+// rows a warp, their loads in flight together, 18.5 us, and 9.1 for the 64 rows.)
+template <int D, int DT>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4AppendParams p) {
-  constexpr int LPR = D / 4, NG = D / KV4_G, RPW = 32 / LPR;  // lanes a row, rows a warp and pass
+  constexpr int LPR = D / 4, NG = D / KV4_G, RPW = 32 / LPR;  // lanes a row, rows a warp
   const int lane = threadIdx.x & 31, l = lane % LPR, g = l / 16;
   const uint32_t heads = (uint32_t)p.c.kvh, per = (uint32_t)p.rows * heads;  // (token, head) rows
   const bool value = blockIdx.y == 1;
-  const uint32_t w0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (ROWS * RPW) + lane / LPR;
+  const uint32_t it = (blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW + lane / LPR;
+  const bool ok = it < per;
+  const uint32_t row = ok ? it / heads : 0, h = ok ? it - row * heads : 0;
+  const int s = (int)(row / (uint32_t)p.n), i = (int)(row - (uint32_t)s * (uint32_t)p.n);
   pdl_trigger();
   pdl_wait();
-  float x[ROWS][4];
-  float4 cs[ROWS][2];
-  uint32_t row[ROWS], h[ROWS];
-  bool ok[ROWS];
-#pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    const uint32_t it = w0 + u * RPW;
-    ok[u] = it < per;
-    row[u] = ok[u] ? it / heads : 0;
-    h[u] = ok[u] ? it - row[u] * heads : 0;
-    const void *src = value ? p.v : p.k;
-    const int64_t off = (int64_t)row[u] * p.ld + (int64_t)h[u] * D + 4 * l;
-    if (p.vec) {
-      if constexpr (DT == LBX_F32) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(src) + off));
-        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-      } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(src) + off));
-        x[u][0] = __uint_as_float(v.x << 16); x[u][1] = __uint_as_float(v.x & 0xFFFF0000u);
-        x[u][2] = __uint_as_float(v.y << 16); x[u][3] = __uint_as_float(v.y & 0xFFFF0000u);
-      }
+  const int st = p.start ? __ldg(p.start + s) : p.max_start;
+  float x[4];
+  const void *src = value ? p.v : p.k;
+  const int64_t off = (int64_t)row * p.ld + (int64_t)h * D + 4 * l;
+  if (p.vec) {
+    if constexpr (DT == LBX_F32) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(src) + off));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[u][i] = load_act(src, DT, off + i);
+      const uint2 v = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(src) + off));
+      x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xFFFF0000u);
     }
-    if (!value && p.rope) {
-      const float4 *c = reinterpret_cast<const float4 *>(p.rope + (int64_t)row[u] * (D / 2) + 4 * (l % (LPR / 2)));
-      cs[u][0] = __ldg(c);
-      cs[u][1] = __ldg(c + 1);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = load_act(src, DT, off + e);
+  }
+  if (!value && p.rope) {
+    const float4 *t = reinterpret_cast<const float4 *>(p.rope + (int64_t)row * (D / 2) + 4 * (l % (LPR / 2)));
+    const float4 c0 = __ldg(t), c1 = __ldg(t + 1);
+    const float c[4] = {c0.x, c0.z, c1.x, c1.z}, sn[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = __shfl_xor_sync(0xffffffffu, x[e], LPR / 2);
+      x[e] = l < LPR / 2 ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y, sn[e]))
+                         : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y, sn[e]));
     }
   }
+  float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+  float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  bool fin = fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY && fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY;
+  fin = (__ballot_sync(0xffffffffu, !fin) & (0xFFFFu << (lane & 16))) == 0u;
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    if (!value && p.rope) {
-      const float c[4] = {cs[u][0].x, cs[u][0].z, cs[u][1].x, cs[u][1].z}, s[4] = {cs[u][0].y, cs[u][0].w, cs[u][1].y, cs[u][1].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = __shfl_xor_sync(0xffffffffu, x[u][i], LPR / 2);
-        x[u][i] = l < LPR / 2 ? __fsub_rn(__fmul_rn(x[u][i], c[i]), __fmul_rn(y, s[i]))
-                              : __fadd_rn(__fmul_rn(x[u][i], c[i]), __fmul_rn(y, s[i]));
-      }
-    }
-    float lo = fminf(fminf(x[u][0], x[u][1]), fminf(x[u][2], x[u][3]));
-    float hi = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
-    bool fin = fabsf(x[u][0]) < INFINITY && fabsf(x[u][1]) < INFINITY && fabsf(x[u][2]) < INFINITY && fabsf(x[u][3]) < INFINITY;
-    fin = (__ballot_sync(0xffffffffu, !fin) & (0xFFFFu << (lane & 16))) == 0u;
-#pragma unroll
-    for (int o = 1; o < 16; o *= 2) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    uint16_t sb = f32_to_bf16(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-    uint16_t lb = f32_to_bf16(lo);
-    float step = bf16_to_f32(sb);
-    if (step < 1.1754943508222875e-38f) {
-      step = 0.f;
-      sb = 0;
-    }
-    const float least = bf16_to_f32(lb);
-    if (!fin || !(step < INFINITY) || !(fabsf(least) < INFINITY)) {
-      sb = lb = KV4_NAN;
-      step = 0.f;
-    }
-    const float inv = step > 0.f ? __fdiv_rn(1.0f, step) : 0.f;
-    uint32_t w = 0;
-    if (step > 0.f) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w |= (uint32_t)__float2int_rn(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[u][i], least), inv)), 0.f), 15.f)) << (4 * i);
-    }
-    w |= __shfl_xor_sync(0xffffffffu, w, 1) << 16;  // (the even lane's: its codes below, its neighbour's above)
-    if (!ok[u]) continue;
-    const int s = (int)(row[u] / (uint32_t)p.n), i = (int)(row[u] - (uint32_t)s * (uint32_t)p.n);
-    const int st = p.start ? __ldg(p.start + s) : p.max_start;
-    if (st < 0 || st > p.max_start) {
-      if (l == 0) atomicCAS(&g_lbx_device_error, 0, 0x801);
-      continue;
-    }
-    const int64_t slot = ((int64_t)s * p.c.kvh + h[u]) * p.c.max_seq + st + i;
-    const int b = l / 2;
-    if (!(l & 1))
-      reinterpret_cast<uint32_t *>((value ? p.c.vc : p.c.kc) + slot * (D / 2))[value ? kv4_word<D, true>(b) : kv4_word<D, false>(b)] = w;
-    if (l % 16 == 0) (value ? p.c.vp : p.c.kp)[slot * NG + g] = (uint32_t)sb | (uint32_t)lb << 16;
+  for (int o = 1; o < 16; o *= 2) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
+  uint16_t sb = f32_to_bf16(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+  uint16_t lb = f32_to_bf16(lo);
+  float step = bf16_to_f32(sb);
+  if (step < 1.1754943508222875e-38f) {
+    step = 0.f;
+    sb = 0;
+  }
+  const float least = bf16_to_f32(lb);
+  if (!fin || !(step < INFINITY) || !(fabsf(least) < INFINITY)) {
+    sb = lb = KV4_NAN;
+    step = 0.f;
+  }
+  const float inv = step > 0.f ? __fdiv_rn(1.0f, step) : 0.f;
+  uint32_t w = 0;
+  if (step > 0.f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w |= (uint32_t)__float2int_rn(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], least), inv)), 0.f), 15.f)) << (4 * e);
+  }
+  w |= __shfl_xor_sync(0xffffffffu, w, 1) << 16;  // (the even lane's: its codes below, its neighbour's above)
+  if (!ok) return;
+  if (st < 0 || st > p.max_start) {
+    if (l == 0) atomicCAS(&g_lbx_device_error, 0, 0x801);
+    return;
+  }
+  const int64_t slot = ((int64_t)s * p.c.kvh + h) * p.c.max_seq + st + i;
+  const int b = l / 2;
+  if (!(l & 1))
+    reinterpret_cast<uint32_t *>((value ? p.c.vc : p.c.kc) + slot * (D / 2))[value ? kv4_word<D, true>(b) : kv4_word<D, false>(b)] = w;
+  if (l % 16 == 0) (value ? p.c.vp : p.c.kp)[slot * NG + g] = (uint32_t)sb | (uint32_t)lb << 16;
 }
 
 struct Kv4ReadParams {
@@ -816,7 +801,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
 // Merge of the sub-chunks' (m, l, o), one block a query row: warp w adds sub-chunks
 // w, w + 8, ... in order, a lane D / 32 dimensions, then the warps in order.  Bound by the
 // round trips: prefix, then everything of 32 sub-chunks at once (their maxima with
-// them), 16 bytes a lane.  (4096 rows of 32 sub-chunks, 67 MB: 14 us after the attention, 36
+// them), 16 bytes a lane.  (4096 rows of 32 sub-chunks, 67 MB: 17.0 us by itself, 36.2
 // with the maxima fetched first and values four bytes at a time.)
 constexpr int KM_WARPS = 8, KM_BATCH = 4;  // warps, and partial results a lane loads together
 template <int D>
@@ -974,15 +959,12 @@ extern "C" int lbx_kv4_append(const lbx_kv4_append_args *a, cudaStream_t stream)
   const int es = a->dtype == LBX_F32 ? 4 : 2;
   p.vec = ((reinterpret_cast<uintptr_t>(a->k_new) | reinterpret_cast<uintptr_t>(a->v_new)) & (uintptr_t)(4 * es - 1)) == 0 &&
           a->kv_ld % 4 == 0;
-  const int d = a->cache.head_dim, rpw = 128 / d;
-  // several rows a warp once single ones would fill the SMs twice over
-  const bool many = items > (int64_t)rpw * 64 * device_sm_count();
-  const int64_t blk = 8 * rpw * (many ? KP_MANY : 1);
+  const int d = a->cache.head_dim, blk = 8 * (128 / d);  // (rows a block)
   const dim3 grid((unsigned)((items + blk - 1) / blk), 2);
   auto go = [&](auto kern) { return launch(kern, grid, dim3(256), 0, stream, a->use_pdl != 0, p); };
   auto pick = [&](auto dd, auto dt) {
     constexpr int D = decltype(dd)::value, DT = decltype(dt)::value;
-    return many ? go(kv4_append_kernel<D, KP_MANY, DT>) : go(kv4_append_kernel<D, 1, DT>);
+    return go(kv4_append_kernel<D, DT>);
   };
   using F = std::integral_constant<int, LBX_F32>;
   using B = std::integral_constant<int, LBX_BF16>;
