@@ -84,6 +84,25 @@ def test_rows_with_nan_or_infinity_stay_their_own():
     assert torch.equal(y[[0, 2, 3]], clean[[0, 2, 3]])
 
 
+# long sums and few tiles (or few past whole rounds of them): K is cut over the SMs and the parts are joined
+CUT = [(1, 20000, 700), (5, 28672, 500), (40, 16384, 1000), (130, 29990, 290), (300, 4992, 12631)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,n", CUT)
+def test_sums_joined_from_parts(m, k, n, dtype):
+    from littlebit_b200 import ops
+
+    x, w, ws, b = _case(m, k, n, dtype, True, k)
+    xd, wd, sd, bd = x.cuda(), w.cuda()[:, :k], ws.cuda(), b.cuda()
+    y = ops.linear_int8(xd, wd, sd, bd)
+    _check(y, x, w[:, :k], ws, b)
+    for _ in range(3):  # whichever part comes last
+        assert torch.equal(ops.linear_int8(xd, wd, sd, bd), y)
+    assert torch.equal(ops.linear_int8(xd[m - 1:], wd, sd, bd)[0], y[m - 1])
+    assert ops.device_error() == 0
+
+
 @pytest.mark.parametrize("m", [2, 16, 40, 130, 300])
 def test_a_token_does_not_depend_on_the_others(m):
     from littlebit_b200 import ops
