@@ -18,8 +18,9 @@ constexpr int Q8_MAXK = 131072;
 // One CTA a row: the absolute maximum, then the codes.  VEC: 16-byte loads, up to
 // Q8_NR of them held in registers from the first pass to the second (rows of up
 // to 8192 float / 16384 bf16 values are read once; what is longer is read again,
-// from L2).  The kernel is one round trip to memory and two block barriers long:
-// 4096 values 5.9 us with scalar loads in two passes.
+// from L2).  The kernel is one round trip to memory and two block barriers long (one
+// row of 4096: 5.5 us by itself, 320 rows of 8192 6.7); 4096 bf16 rows of 8192, 101 MB, 24 us,
+// are bound by instructions.
 constexpr int Q8_NR = 8;
 LBX_DEV uint32_t q8_abs(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 LBX_DEV uint32_t q8_code(float v, float inv, bool fin) {
@@ -124,6 +125,13 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
 //           32000 channels are 7 units for each of 148 CTAs, nothing is joined.  Joining
 //           cost 10 us there: under a saturated memory a fence, an atomic or a
 //           load takes as long as the queue of loads ahead of it.
+//
+// Bound for few tokens by the weights' stream (1 x 32000 x 4096, 131 MB: 28.5 us with the
+// quantiser, 4.6 TB/s; 8 x 32000 x 8192, 262 MB: 64), for many by the copies from L2 and
+// the clock that the power leaves: a block of 128 x 256 brings 48 KB for 512 cycles of MMA
+// and takes 730 (4096 x 28672 x 8192: 701 us, 2.74 POP/s, tensor pipes busy 70 % of cycles).
+// Two channel tiles at once from one CTA, a token tile loaded once for both, was slower
+// (1020 us for 897 then: half the stages).
 // ---------------------------------------------------------------------------
 constexpr int I8_THREADS = 192;   // warp 0: copies, warp 1: MMA, warps 2-5: results
 constexpr int I8_KB = 128;        // K bytes a block

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 // that showed (4e-5 of the result at 4000 slots, 6e-4 at 130 000), so a sum on them
 // never runs longer than 64 dimensions or 32 slots, small terms first, and the rest is
 // ordinary additions.  float32 calls centre their codes (a pair of codes is two logic
-// operations at most and one exact subtraction): 3e-7 and 5e-6.  bfloat16 calls keep c: in
+// operations at most and one exact subtraction): 3e-7 and 1.2e-6.  bfloat16 calls keep c: in
 // the low bits of a 16-bit lane it IS the fp16 subnormal c * 2^-24, which the tensor cores
 // multiply exactly.  Nibbles 1 and 3 are left at 16 times their value.
 // Codes are the A operand (16 slots x 16 dimensions of the keys, 16 dimensions x 16
@@ -1007,12 +1007,13 @@ static void kv4_cut(Kv4AttnParams &p, int i0, int nt) {
   p.ntile = (p.R + 7) / 8;
   p.nsub = (end + p.ck - 1) / p.ck;
   // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
-  // queries' fragments (1500 instructions) are made once for all of them
+  // queries' fragments (1500 instructions) are made once for all of them (5 tokens of 64
+  // sequences over up to 4000 slots, 64 heads over 8: 370 us, one sub-chunk each 417)
   const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
   p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (48 * device_sm_count())));
-  // Row tiles a block, evenly (5 tiles, 64 sequences over 4000 slots: 469 us sharing the
-  // ring, 506 each with its own); with one sub-chunk a warp a tile has its own ring (5 tiles
-  // over 130 000 slots: 251 us, shared 285).  The warps left take further runs.
+  // Row tiles a block, evenly (5 tiles, 64 sequences over 4000 slots: 370 us sharing the
+  // ring, 398 each with its own); with one sub-chunk a warp a tile has its own ring (5 tiles
+  // over 130 000 slots: 245 us, shared 280).  The warps left take further runs.
   const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
   p.rw = p.cpw == 1 ? 1 : (p.ntile + groups - 1) / groups;
   p.kw = std::min(KA_WARPS / p.rw, (p.nsub + p.cpw - 1) / p.cpw);

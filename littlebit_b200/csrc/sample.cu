@@ -30,8 +30,11 @@ struct AcceptParams {
 // drawing.  All rows are read before the first decision is known: deciding row
 // by row would read fewer of them and wait for the cluster once a draft.
 // Bound by memory for many sequences, by three round trips to it and two cluster barriers
-// for one.
-constexpr int AC_MANY = 16;  // sequences from which blocks have 256 threads (four fill an SM) instead of 1024
+// for one: 64 sequences of up to 8 drafts, 32000 logits, 82 MB: 35 us; 1 of 4: 15.7.
+// Blocks have 1024 threads, or 256 (four fill an SM) from AC_MANY sequences on.  4 drafts, us
+// with 256 and with 1024: 1 sequence 22.6, 20.5; 8: 22.6, 20.5 (of 128256 logits 52, 32);
+// 16: 24.6, 35.8 (57, 59); 64 of 8 drafts: 45, 82.  (These behind a flush of L2.)
+constexpr int AC_MANY = 16;
 constexpr int AC_C = 8;      // blocks a sequence
 constexpr int AC_Q = 4;      // quads of logits a lane loads together
 constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
