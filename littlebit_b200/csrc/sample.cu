@@ -4,6 +4,7 @@
 // max(q_i(d_i), 1e-10)); then argmax_v r_v / e_v with r the positive part of
 // p_a - q_a, or p_k.
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -30,11 +31,13 @@ struct AcceptParams {
 // drawing.  All rows are read before the first decision is known: deciding row
 // by row would read fewer of them and wait for the cluster once a draft.
 // Bound by memory for many sequences, by three round trips to it and two cluster barriers
-// for one: 64 sequences of up to 8 drafts, 32000 logits, 82 MB: 35 us; 1 of 4: 15.7.
-// Blocks have 1024 threads, or 256 (four fill an SM) from AC_MANY sequences on.  4 drafts, us
-// with 256 and with 1024: 1 sequence 22.6, 20.5; 8: 22.6, 20.5 (of 128256 logits 52, 32);
-// 16: 24.6, 35.8 (57, 59); 64 of 8 drafts: 45, 82.  (These behind a flush of L2.)
-constexpr int AC_MANY = 16;
+// for one: 64 sequences of up to 8 drafts, 32000 logits, 82 MB: 32 us; 1 of 4: 15.7 (most of it the host).
+// As many threads as let all blocks be on the GPU at once: 1024 up to AC_ONE sequences, 512 (two
+// blocks an SM) up to AC_TWO, 256 (four) past it.  us with 1024, 512, 256 threads, 4 drafts,
+// behind a flush of L2: 8 sequences of 32000 logits 18, 18, 21, of 128256 29, 35, 47; 12 of 128256
+// 33, 37, 50; 16: 31, 21, 23 and 55, 43, 53; 32: 45, 25, 25 and 82, 54, 66; 64: 70, 41, 33
+// and 129, 96, 84.
+constexpr int AC_ONE = 12, AC_TWO = 32;
 constexpr int AC_C = 8;      // blocks a sequence
 constexpr int AC_Q = 4;      // quads of logits a lane loads together
 constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
@@ -132,24 +135,17 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
   const int nq = (V + 3) / 4, per = (nq + AC_C - 1) / AC_C;
   const int q0 = min(nq, rank * per), q1 = min(nq, q0 + per), nb = (per + BQ - 1) / BQ;
 
-  // what a decision needs besides the rows' statistics, on its way meanwhile
-  int64_t tok = -1;
-  float tl = -INFINITY, dl = -INFINITY, uu = 2.f;
-  if (tid < nd) {
-    tok = __ldg(p.tokens + s * p.tokens_ld + tid);
-    uu = __ldg(p.u + s * p.u_ld + tid);
-    if (tok >= 0 && tok < V) {
-      tl = load_act(row_at(tid), DT, tok);
-      if (has_q) dl = load_act(row_at(nd + 1 + tid), DT, tok);
-    } else if (rank == 0) {
-      atomicCAS(&g_lbx_device_error, 0, 0x811);
-    }
-  }
+  // the random numbers of the drawing, to L2 meanwhile (8 sequences of 128256 logits: 31
+  // to 29 us; many sequences leave memory no idle time, 41 to 43)
+  if (AC_T > 256 && !greedy)
+    for (int v = 4 * q0 + 32 * tid; v < min(4 * q1, V); v += 32 * AC_T)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.e + s * p.e_ld + v));
 
   // ---- statistics of every row's slice: the (row, batch) items dealt evenly to the
   // warps, the next item's loads under way while one is worked on
+  int64_t tok = -1;
+  float tl = -INFINITY, dl = -INFINITY, uu = 2.f;
   for (int i = tid; i < nrow * NWARP; i += AC_T) (&part[0][0])[i] = none;
-  __syncthreads();
   {
     const int items = nrow * nb;
     int it = (int)((int64_t)items * warp / NWARP);
@@ -221,6 +217,18 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
     };
     float4 x[AC_Q], y[AC_Q];
     if (it < end) load(x, r, b);
+    __syncthreads();
+    // what a decision needs besides the rows' statistics, on its way meanwhile
+    if (tid < nd) {
+      tok = __ldg(p.tokens + s * p.tokens_ld + tid);
+      uu = __ldg(p.u + s * p.u_ld + tid);
+      if (tok >= 0 && tok < V) {
+        tl = load_act(row_at(tid), DT, tok);
+        if (has_q) dl = load_act(row_at(nd + 1 + tid), DT, tok);
+      } else if (rank == 0) {
+        atomicCAS(&g_lbx_device_error, 0, 0x811);
+      }
+    }
     while (it < end) {
       work(x, y);
       if (it < end) work(y, x);
@@ -382,8 +390,8 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   LBX_CHECK_SUP((int64_t)a->n_seq * AC_C <= 0x7fffffff, "too many sequences");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a->n_seq * AC_C);
-  const bool many = a->n_seq >= AC_MANY;
-  cfg.blockDim = dim3(many ? 256 : 1024);
+  const int threads = a->n_seq <= AC_ONE ? 1024 : a->n_seq <= AC_TWO ? 512 : 256;
+  cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -394,7 +402,10 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   cfg.attrs = attr;
   cfg.numAttrs = a->use_pdl ? 2 : 1;
   auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, p); };
-  return cuda_status(a->dtype == LBX_F32 ? (many ? go(accept_kernel<LBX_F32, 256>) : go(accept_kernel<LBX_F32, 1024>))
-                                         : (many ? go(accept_kernel<LBX_BF16, 256>) : go(accept_kernel<LBX_BF16, 1024>)),
+  auto pick = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return threads == 1024 ? go(accept_kernel<DT, 1024>) : threads == 512 ? go(accept_kernel<DT, 512>) : go(accept_kernel<DT, 256>);
+  };
+  return cuda_status(a->dtype == LBX_F32 ? pick(std::integral_constant<int, LBX_F32>{}) : pick(std::integral_constant<int, LBX_BF16>{}),
                      "accept_sampled launch");
 }

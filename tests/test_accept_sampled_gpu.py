@@ -66,6 +66,23 @@ def test_ragged_drafts_and_temperatures():
     assert 0 < sum(acc) < int(count.sum())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k,V", [(4, 5003), (64, 130)])
+def test_a_sequence_does_not_depend_on_the_others(k, V, dtype):
+    """From one sequence to many (blocks of other sizes): the same decisions, and again when called again."""
+    from littlebit_b200 import ops
+
+    ins = [x.cuda() for x in _inputs(40, k, V, 7, dtype)]
+    _check(*(x[:12].cpu() for x in ins), 1.0)
+    acc, nxt = ops.accept_sampled(*ins, 1.0)
+    for S in (1, 12, 13, 32, 33, 40):
+        a, b = ops.accept_sampled(*(x[:S] for x in ins), 1.0)
+        same = (a == acc[:S]) & (b == nxt[:S])  # (sums of other orders: an even call may fall either way)
+        assert int(same.sum()) >= 0.9 * S, S
+        a2, b2 = ops.accept_sampled(*(x[:S] for x in ins), 1.0)
+        assert torch.equal(a, a2) and torch.equal(b, b2)
+
+
 def test_greedy_temperature_takes_the_first_maximum():
     tok, t, d, u, e = _inputs(12, 4, 300, 6, T=0.0)
     t[:, :, 17] = t.amax(-1)  # ties with a later or an earlier index
