@@ -1007,7 +1007,7 @@ static void kv4_cut(Kv4AttnParams &p, int i0, int nt) {
   p.ntile = (p.R + 7) / 8;
   p.nsub = (end + p.ck - 1) / p.ck;
   // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
-  // queries' fragments (1500 instructions) are made once for all of them (5 tokens of 64
+  // queries' fragments are made once for all of them (5 tokens of 64
   // sequences over up to 4000 slots, 64 heads over 8: 370 us, one sub-chunk each 417)
   const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
   p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (48 * device_sm_count())));
