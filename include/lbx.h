@@ -453,10 +453,12 @@ typedef struct lbx_int8_args {
   void *y; int64_t y_ld;  /* [m, n]                                            */
 } lbx_int8_args;
 /* The sums are exact, so a token's bits depend neither on the other tokens of
- * the call nor on how the work is split.  The workspace must be zero-filled
- * once when it is allocated (it starts with the tickets of split tiles, which
- * every call leaves at zero); calls sharing one are ordered on one stream.  A
- * bounded wait that runs out records device error 0x821 .. 0x826. */
+ * the call nor on how the work is split.  The workspace's first
+ * LBX_INT8_TICKET_BYTES must be zero-filled once when it is allocated (the
+ * tickets of split tiles, which every call leaves at zero); calls sharing one
+ * are ordered on one stream.  A bounded wait that runs out records device
+ * error 0x821 .. 0x826. */
+#define LBX_INT8_TICKET_BYTES 4096
 size_t lbx_linear_int8_workspace_size(int32_t m, int32_t n, int32_t k);
 int lbx_linear_int8(const lbx_int8_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
 

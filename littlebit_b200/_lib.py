@@ -21,6 +21,7 @@ LBX_EXEC_AUTO, LBX_EXEC_KERNELS, LBX_EXEC_PROGRAM, LBX_EXEC_CLUSTER = 0, 1, 2, 3
 LBX_EXEC_KERNELS_ONE_CTA_V = 4
 LBX_EXEC_TC, LBX_EXEC_NO_TC = 5, 6
 LBX_ACCEPT_MAX_K = 64
+LBX_INT8_TICKET_BYTES = 4096
 
 
 class Branch(ctypes.Structure):

@@ -532,7 +532,8 @@ static I8Plan i8_plan(int m, int n, int k) {
   p.idesc = idesc_i8(p.BN);
   p.tcols = 32;
   while (p.tcols < 2u * p.BN) p.tcols *= 2;
-  w.part = al((size_t)I8_MAXCTA * 4);
+  static_assert(I8_MAXCTA * 4 == LBX_INT8_TICKET_BYTES, "tickets");
+  w.part = LBX_INT8_TICKET_BYTES;
   w.s = w.part + al((size_t)p.Gr * 2 * 128 * p.BN * 4);
   w.q = w.s + al((size_t)m * 4);
   w.q_ld = (k + 15) & ~15;

@@ -545,6 +545,7 @@ _FLOATS = (torch.float32, torch.bfloat16)
 _DTYPE = {torch.float32: L.LBX_F32, torch.bfloat16: L.LBX_BF16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda i: torch.cuda.current_stream(i).cuda_stream)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def _rows(name: str, t: torch.Tensor, dtypes=_FLOATS) -> torch.Tensor:
@@ -595,8 +596,14 @@ class _on:
             torch.cuda.set_device(self.prev)
 
 
-def _stream_ws(index: int, tag: str, stream: int, nbytes: int) -> torch.Tensor:
-    """Scratch of one operator on one stream (calls on different streams never share it)."""
+def _stream_ws(index: int, tag: str, stream: int, nbytes: int, zeros: int = 0) -> torch.Tensor:
+    """Scratch of one operator on one stream (calls on different streams never share it).
+    A captured call has its own, of the graph's memory (it lives as long as the graph,
+    whatever later calls need), its first ``zeros`` bytes set by the graph."""
+    if _capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        buf[:zeros].zero_()
+        return buf
     key = (index, tag, stream)
     ws = _WS.get(key)
     if ws is None:
@@ -650,7 +657,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
                    None if bias is None else _vec("bias", bias, n, torch.float32, dev), out.data_ptr(), _ld(out))
     with _on(dev) as st:
         c = lib()
-        ws = _stream_ws(dev, "int8", st, c.lbx_linear_int8_workspace_size(m, n, k))
+        ws = _stream_ws(dev, "int8", st, c.lbx_linear_int8_workspace_size(m, n, k), L.LBX_INT8_TICKET_BYTES)
         L.check(c.lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
     return out
 

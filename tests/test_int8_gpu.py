@@ -173,6 +173,38 @@ def test_in_a_cuda_graph():
         _check(out, x2, w, ws, None)
 
 
+def test_graphs_keep_their_workspaces():
+    """Graphs captured on one stream, and eager calls there that need more, leave each other's scratch alone."""
+    from littlebit_b200 import ops
+
+    st = torch.cuda.Stream()
+    cases = []
+    for m, k, n in ((1, 20000, 700), (64, 16384, 1000), (130, 512, 2000)):
+        x, w, ws, _ = _case(m, k, n, "f32", False, m)
+        cases.append((x.cuda(), w.cuda()[:, :k], ws.cuda(), torch.empty(m, n, device="cuda")))
+    want = [ops.linear_int8(x, w, s) for x, w, s, _ in cases]
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(st):
+        for x, w, s, out in cases:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):  # (no call before it on this stream)
+                ops.linear_int8(x, w, s, out=out)
+            graphs.append(g)
+        eager = [ops.linear_int8(x, w, s) for x, w, s, _ in cases]
+        junk = [torch.full((1 << 22,), 7, dtype=torch.int32, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for (_, _, _, out), g, y, e in zip(cases, graphs, want, eager):
+            out.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(st):
+                g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, y) and torch.equal(e, y)
+    assert all(int(j.min()) == 7 == int(j.max()) for j in junk)
+
+
 def test_refusals():
     from littlebit_b200 import ops
 
