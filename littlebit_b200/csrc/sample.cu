@@ -26,12 +26,14 @@ struct AcceptParams {
 
 // One cluster of AC_C blocks a sequence, each with a slice of the vocabulary, in one
 // launch: the statistics of all rows at once (a warp takes 512 logits of one
-// row at a time, four 16-byte loads a lane in flight), joined over the cluster's shared
-// memory; every block then makes the same decisions and takes its slice of the
+// row at a time, four 16-byte loads a lane in flight), joined by shuffles and sent to every
+// block's shared memory; every block then makes the same decisions and takes its slice of the
 // drawing.  All rows are read before the first decision is known: deciding row
 // by row would read fewer of them and wait for the cluster once a draft.
 // Bound by memory for many sequences, by three round trips to it and two cluster barriers
-// for one: 64 sequences of up to 8 drafts, 32000 logits, 82 MB: 32 us; 1 of 4: 15.7 (most of it the host).
+// for one: 64 sequences of up to 8 drafts, 32000 logits, 82 MB: 32 us; 1 of 4: 10.3 from the
+// kernel's first instruction to its last (13 with parts joined by one thread a row and
+// read from the blocks that hold them).
 // As many threads as let all blocks be on the GPU at once: 1024 up to AC_ONE sequences, 512 (two
 // blocks an SM) up to AC_TWO, 256 (four) past it.  us with 1024, 512, 256 threads, 4 drafts,
 // behind a flush of L2: 8 sequences of 32000 logits 18, 18, 21, of 128256 29, 35, 47; 12 of 128256
@@ -103,12 +105,13 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
   constexpr int ES = DT == LBX_F32 ? 4 : 2;
   constexpr int NWARP = AC_T / 32;
   __shared__ uint64_t part[AC_ROWS][NWARP];  // each warp's share of a row: (top, sum) pairs, or keys (greedy)
-  __shared__ uint64_t mine[AC_ROWS], tot[AC_ROWS];
-  __shared__ uint64_t best[2][AC_C];          // every block's, in the first block
+  __shared__ uint64_t all[AC_C][AC_ROWS], tot[AC_ROWS];  // every block's share of a row, and the row
+  __shared__ uint64_t best[2][AC_C];          // every block's
   __shared__ uint64_t wbest[AC_T / 32];
   __shared__ int rejected;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int s = blockIdx.x / AC_C, rank = (int)cl.block_rank(), V = p.vocab;
+  cl.barrier_arrive();  // (waited for before the first store to another block's shared memory)
   pdl_trigger();
   pdl_wait();
   const float T = p.temps ? __ldg(p.temps + s) : p.temperature;
@@ -238,21 +241,23 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
     if (greedy) return a > b ? a : b;
     return ac_pack(ac_join(ac_pair(a), ac_pair(b)));
   };
+  // lanes xor o, 2 o, ... joined; every block goes the same way
+  auto reduce = [&](uint64_t v, int o) {
+    for (; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, (unsigned long long)v, o));
+    return v;
+  };
   __syncthreads();
-  for (int r = tid; r < nrow; r += AC_T) {
-    uint64_t a = part[r][0];
-    for (int i = 1; i < NWARP; ++i) a = join(a, part[r][i]);
-    mine[r] = a;
+  cl.barrier_wait();
+  for (int r = warp; r < nrow; r += NWARP) {
+    uint64_t v = reduce(lane < NWARP ? part[r][lane] : none, 16);
+    v = __shfl_sync(0xffffffffu, (unsigned long long)v, 0);
+    if (lane < AC_C) *cl.map_shared_rank(&all[rank][r], lane) = v;
   }
   cl.sync();
-  for (int r = tid; r < nrow; r += AC_T) {
-    uint64_t v[AC_C];
-#pragma unroll
-    for (int i = 0; i < AC_C; ++i) v[i] = *cl.map_shared_rank(&mine[r], i);
-    uint64_t a = v[0];
-#pragma unroll
-    for (int i = 1; i < AC_C; ++i) a = join(a, v[i]);  // (the same order in every block)
-    tot[r] = a;
+  for (int r0 = 4 * warp; r0 < nrow; r0 += 4 * NWARP) {  // eight lanes a row
+    const int r = r0 + lane / AC_C;
+    const uint64_t v = reduce(r < nrow ? all[lane % AC_C][r] : none, AC_C / 2);
+    if (r < nrow && lane % AC_C == 0) tot[r] = v;
   }
   if (tid == 0) rejected = nd;
   __syncthreads();
@@ -297,14 +302,24 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
       constexpr int NB = AC_T == 256 ? 2 : 1;
       for (int b = q0 + tid; b < q1; b += NB * AC_T) {
         float4 x[NB], y[NB], z[NB];
+        const int last = b + (NB - 1) * AC_T;
+        if (pv && qv && ev && last < q1 && 4 * last + 3 < V) {  // (no branch between the loads)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const int k = b + i * AC_T;
-          x[i] = y[i] = z[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-          if (k < q1) {
-            x[i] = ac_quad<DT>(prow, pv, k, V);
-            if (q && less) y[i] = ac_quad<DT>(qrow, qv, k, V);
-            z[i] = ac_quad<LBX_F32>(er, ev, k, V);
+          for (int i = 0; i < NB; ++i) {
+            x[i] = ac_quad_full<DT>(prow, b + i * AC_T);
+            y[i] = ac_quad_full<DT>(qrow, b + i * AC_T);
+            z[i] = ac_quad_full<LBX_F32>(er, b + i * AC_T);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const int k = b + i * AC_T;
+            x[i] = y[i] = z[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (k < q1) {
+              x[i] = ac_quad<DT>(prow, pv, k, V);
+              y[i] = ac_quad<DT>(qrow, qv, k, V);
+              z[i] = ac_quad<LBX_F32>(er, ev, k, V);
+            }
           }
         }
 #pragma unroll
@@ -330,21 +345,18 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
       key = warp_max64(key);
       if (lane == 0) wbest[warp] = key;
       __syncthreads();
-      if (tid == 0) {
-        for (int i = 1; i < AC_T / 32; ++i) key = wbest[i] > key ? wbest[i] : key;
-        *cl.map_shared_rank(&best[pass][rank], 0) = key;
+      if (warp == 0) {
+        key = warp_max64(lane < NWARP ? wbest[lane] : 0ull);
+        if (lane < AC_C) *cl.map_shared_rank(&best[pass][rank], lane) = key;
       }
       cl.sync();
 #pragma unroll
-      for (int i = 0; i < AC_C; ++i) {
-        const uint64_t k = *cl.map_shared_rank(&best[pass][i], 0);
-        got = k > got ? k : got;
-      }
+      for (int i = 0; i < AC_C; ++i) got = best[pass][i] > got ? best[pass][i] : got;
       if (got) break;  // (else p and q are equal, nothing is left over, and the token comes from p)
     }
     next = first_of(got);
   }
-  cl.sync();  // (no block leaves while another reads its shared memory)
+  // (no store to another block's shared memory is later than the last cluster barrier: blocks may leave)
   if (rank == 0 && tid == 0) {
     p.accepted[s] = a;
     p.next[s] = next;
