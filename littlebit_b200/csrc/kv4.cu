@@ -306,6 +306,10 @@ LBX_DEV float ex2(float x) {
   return r;
 }
 
+// Is a group's step or least value (plus 8 steps, where codes are centred) an infinity
+// or a NaN?  Either may be alone: a bfloat16 call's least value says nothing of the step.
+LBX_DEV bool kv4_no_number(float step, float least) { return !(fabsf(step) < INFINITY) || !(fabsf(least) < INFINITY); }
+
 // does query i of its sequence see slot j
 LBX_DEV bool kv4_sees(int j, int prefix, int n, int i, bool tree, uint64_t mask) {
   if (j < prefix) return true;
@@ -632,7 +636,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
               for (int g = 0; g < NG; ++g) {
                 a = fmaxf(a, fabsf(sg[t][g]));
                 // what is not a number reaches the rows that see it, and (below) no other
-                if (!(fabsf(lg[t][g]) < INFINITY)) om[b][g] += __uint_as_float(0x7FC00000u);
+                if (kv4_no_number(sg[t][g], lg[t][g])) om[b][g] += __uint_as_float(0x7FC00000u);
               }
             } else {
               sc[t][b] = -INFINITY;
@@ -644,7 +648,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
         for (int t = 0; t < NK; ++t)
 #pragma unroll
           for (int g = 0; g < NG; ++g)
-            if (!(fabsf(lg[t][g]) < INFINITY)) sg[t][g] = lg[t][g] = 0.f;
+            if (kv4_no_number(sg[t][g], lg[t][g])) sg[t][g] = lg[t][g] = 0.f;
       }
       // ---- references: a row's moves when its maximum is 2^8 above it (or a step is above all before)
       float mx[2];
