@@ -1,0 +1,77 @@
+"""Edges of the low-bit operators: what a mask hides, extreme magnitudes, ties, default bounds, many row tiles."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import lowbit as olow
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _cache(S, H, T, d, seed, scale=1.0):
+    """A 4-bit cache of random rows, filled by the library, and the values it holds (float64)."""
+    from littlebit_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = ops.Kv4Cache.empty(S, H, T, d)
+    T = c.shape[2]
+    loud = 1 + 3 * (torch.arange(H * d, device="cuda") % d % 29 == 3)
+    for s0 in range(0, T, 1024):
+        n = min(1024, T - s0)
+        k, v = (scale * torch.randn(S * n, H * d, generator=g, device="cuda") for _ in range(2))
+        ops.kv4_append(k * loud, v, c, s0)
+    return c
+
+
+def _values(c, s, n):
+    from littlebit_b200 import ops
+
+    one = ops.Kv4Cache(*(t[s:s + 1] for t in (c.k_codes, c.k_params, c.v_codes, c.v_params)))
+    k, v = ops.kv4_read(one, 0, None, n)
+    return k[0].double(), v[0].double()
+
+
+# a step that is not a number beside a least value that is one, and the reverse
+BAD = [(float("nan"), 0.25), (float("inf"), 0.25), (float("-inf"), -1.0), (0.5, float("nan")), (0.5, float("inf")),
+       (float("nan"), float("nan"))]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", BAD)
+def test_stale_params_of_any_kind_reach_no_row(bad, d, dtype):
+    from littlebit_b200 import ops
+
+    heads, kvh, prefix = 8, 2, 70
+    c = _cache(1, kvh, 192, d, 3)
+    q = torch.randn(3, heads * d, generator=torch.Generator().manual_seed(1)).to(DT[dtype]).cuda()
+    masks = torch.tensor([0b001, 0b011, 0b101], dtype=torch.int64, device="cuda")
+    clean = [ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5, tree_mask=m) for m in (None, masks)]
+    for t in (c.k_params, c.v_params):
+        t[:, :, prefix + 3:, :, 0], t[:, :, prefix + 3:, :, 1] = bad
+    for m, want in zip((None, masks), clean):
+        got = ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5, tree_mask=m)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("half", ["k", "v"])
+def test_a_slot_that_is_no_number_reaches_the_rows_that_see_it_alone(half, bad, d, dtype):
+    from littlebit_b200 import ops
+
+    heads, prefix = 3, 40
+    c = _cache(1, 1, 64, d, 5)
+    q = torch.randn(3, heads * d, generator=torch.Generator().manual_seed(2)).to(DT[dtype]).cuda()
+    clean = ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5)
+    p = c.k_params if half == "k" else c.v_params
+    p[0, 0, prefix + 1, :, 0], p[0, 0, prefix + 1, :, 1] = bad  # the second new token's
+    y = ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5)
+    assert torch.equal(y[0], clean[0])
+    if half == "v":
+        assert torch.isnan(y[1:]).all()
+    tree = ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5,
+                             tree_mask=torch.tensor([1, 3, 5], dtype=torch.int64, device="cuda"))
+    assert torch.equal(tree[0], clean[0]) and not torch.isnan(tree[2]).any()
