@@ -530,8 +530,9 @@ typedef struct lbx_kv4_attn_args {
   const uint64_t *tree_mask; /* [n_seq * n] or NULL */
   void *out;
 } lbx_kv4_attn_args;
-/* Workspace: any contents.  A bounded wait that runs out records device error
- * 0x804 .. 0x806. */
+/* Workspace: any contents.  Its size never shrinks as max_prefix or n grow: one
+ * sized for the longest serves every call.  A bounded wait that runs out records
+ * device error 0x804 .. 0x806. */
 size_t lbx_kv4_attn_workspace_size(const lbx_kv4_attn_args *a /* host */);
 int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_bytes, cudaStream_t stream);
 

@@ -1023,16 +1023,20 @@ static void kv4_cut(Kv4AttnParams &p, int i0, int nt) {
   p.kw = std::min(KA_WARPS / p.rw, (p.nsub + p.cpw - 1) / p.cpw);
 }
 
-// tokens a launch (its partial results stay within a gigabyte) and their bytes
+// Tokens a launch (its partial results stay within a gigabyte), and what the call wants
+// of scratch: never less for a longer prefix or for more tokens, so that scratch sized for
+// the longest serves every call (whole tokens times their bytes would not: a shorter
+// prefix may fit one token more into the gigabyte).
 static int kv4_slice(const Kv4AttnParams &p, int D, int64_t &bytes) {
+  constexpr int64_t cap = 1ll << 30;
   const int ck = kv4_sub_chunk(p.c.max_seq), nsub = (p.max_prefix + p.n + ck - 1) / ck;
   if (nsub <= 1) {
     bytes = 0;
     return p.n;
   }
   const int64_t per = (int64_t)p.c.n_seq * p.c.kvh * nsub * p.rep * (D * 4 + 8);
-  const int sl = (int)std::min<int64_t>(p.n, std::max<int64_t>(1, (1ll << 30) / per));
-  bytes = per * sl;
+  const int sl = (int)std::min<int64_t>(p.n, std::max<int64_t>(1, cap / per));
+  bytes = sl == p.n ? per * sl : std::max(cap, per);
   return sl;
 }
 
