@@ -228,7 +228,11 @@ def sampled_speculative_generate(drf: BatchDecoder, tgt: BatchDecoder, prev: tor
     every sequence's tokens are distributed as the target's own samples.  At
     temperature 0 they are the target's greedy tokens.  ``draft_head`` /
     ``target_head``: 8-bit lm_heads used in place of the decoders' bf16 ones.
-    Returns (new tokens [S, max_new], stats)."""
+    A sequence that has its max_new tokens stands still until the others have theirs, so
+    both caches need start + max_new + gamma slots.
+    Returns (new tokens [S, max_new], stats over the steps that sequences needed)."""
+    if gamma < 1 or max_new < 0 or start < 1:
+        raise ValueError("gamma and start must be at least 1, max_new at least 0")
     S, dev, V = tgt.S, tgt.device, tgt.dec.shape.vocab_size
     cap = max_new + gamma + 1
     out = torch.zeros(S, cap, dtype=torch.int64, device=dev)
@@ -244,7 +248,8 @@ def sampled_speculative_generate(drf: BatchDecoder, tgt: BatchDecoder, prev: tor
     def noise():  # exponentially distributed, never 0
         return e.exponential_(generator=generator).clamp_(min=tiny)
 
-    steps = total_acc = done = 0
+    counts = torch.zeros(2, dtype=torch.int64, device=dev)  # accepted drafts, steps of unfinished sequences
+    steps = done = 0
     bound = start
     while done < max_new:
         # draft: [prev, last] at slots pos-1, pos (a sequence whose drafts were all accepted has
@@ -260,19 +265,23 @@ def sampled_speculative_generate(drf: BatchDecoder, tgt: BatchDecoder, prev: tor
         u = torch.rand(S, gamma, generator=generator, device=dev)
         m, nxt = accept_sampled(vtok[:, 1:], tlog, dlog, u, noise(), temperature)
         # this step's tokens: the m accepted drafts, then the drawn one; what lies
-        # past them is rewritten by later steps
+        # past them is rewritten by later steps (a finished sequence's lie past max_new)
         cand = torch.cat([vtok[:, 1:], nxt[:, None]], 1)
         new = torch.where(ar[None] < m[:, None], cand, nxt[:, None])
         out.scatter_(1, (nacc[:, None] + ar[None]).clamp(max=cap - 1), new)
-        prev_t = vtok.gather(1, m[:, None])[:, 0]
-        last_t = nxt
-        nacc += m + 1
-        pos += (m + 1).to(torch.int32)
+        open_ = nacc < max_new
+        counts += torch.stack([torch.where(open_, m, 0).sum(), open_.sum()])
+        nacc = torch.where(open_, nacc + m + 1, nacc)
+        # a sequence that is done feeds the same slots again: its place moves no further
+        go = nacc < max_new
+        prev_t = torch.where(go, vtok.gather(1, m[:, None])[:, 0], prev_t)
+        last_t = torch.where(go, nxt, last_t)
+        pos = torch.where(go, pos + (m + 1).to(torch.int32), pos)
         steps += 1
-        total_acc += int(m.sum())
-        done = int(nacc.min())
-        bound = start + int(nacc.max())
-    stats = {"num_steps": steps, "total_accepted_tokens": total_acc,
-             "acceptance_rate": total_acc / (steps * gamma * S),
-             "mean_acceptance_length": total_acc / (steps * S) + 1.0}
+        done, most = torch.stack([nacc.min(), pos.max()]).tolist()
+        bound = int(most)
+    accepted, needed = counts.tolist()
+    stats = {"num_steps": steps, "total_accepted_tokens": accepted,
+             "acceptance_rate": accepted / max(1, needed * gamma),
+             "mean_acceptance_length": accepted / max(1, needed) + 1.0}
     return out[:, :max_new], stats
