@@ -9,6 +9,7 @@ rejected, and a missing kernel library raises at import of ``_lib``.
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -596,19 +597,35 @@ class _on:
             torch.cuda.set_device(self.prev)
 
 
-def _stream_ws(index: int, tag: str, stream: int, nbytes: int, zeros: int = 0) -> torch.Tensor:
+class _Scratch(Workspace):
     """Scratch of one operator on one stream (calls on different streams never share it).
-    A captured call has its own, of the graph's memory (it lives as long as the graph,
-    whatever later calls need), its first ``zeros`` bytes set by the graph."""
-    if _capturing():
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        buf[:zeros].zero_()
-        return buf
+    Its lock is held from :meth:`take` until the call's launches are in the stream: a call
+    is several launches that pass results through the scratch, and another thread's on the
+    same stream must not come between them (the C call lets other threads run)."""
+
+    def __init__(self, device: torch.device):
+        super().__init__(device)
+        self.lock = threading.RLock()  # (a finaliser that calls the operator finds its own thread's)
+
+    def take(self, nbytes: int, zeros: int = 0) -> torch.Tensor:
+        """The scratch, for the holder of the lock.  A captured call has its own, of the
+        graph's memory (it lives as long as the graph, whatever later calls need), its
+        first ``zeros`` bytes set by the graph."""
+        if _capturing():
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            buf[:zeros].zero_()
+            return buf
+        buf = self.buf
+        return buf if buf.numel() >= nbytes else self.get(nbytes)
+
+
+_SCRATCH: dict = {}
+
+
+def _stream_ws(index: int, tag: str, stream: int) -> _Scratch:
     key = (index, tag, stream)
-    ws = _WS.get(key)
-    if ws is None:
-        ws = _WS[key] = Workspace(torch.device("cuda", index))
-    return ws.get(nbytes)
+    # (of two threads that come first, both get the one that is kept)
+    return _SCRATCH.get(key) or _SCRATCH.setdefault(key, _Scratch(torch.device("cuda", index)))
 
 
 def quantize_tokens(x: torch.Tensor):
@@ -656,9 +673,10 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
                    _ld(weight), _vec("weight_scale", weight_scale, n, torch.float32, dev),
                    None if bias is None else _vec("bias", bias, n, torch.float32, dev), out.data_ptr(), _ld(out))
     with _on(dev) as st:
-        c = lib()
-        ws = _stream_ws(dev, "int8", st, c.lbx_linear_int8_workspace_size(m, n, k), L.LBX_INT8_TICKET_BYTES)
-        L.check(c.lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
+        c, sc = lib(), _stream_ws(dev, "int8", st)
+        with sc.lock:
+            ws = sc.take(c.lbx_linear_int8_workspace_size(m, n, k), L.LBX_INT8_TICKET_BYTES)
+            L.check(c.lbx_linear_int8(ctypes.byref(a), ws.data_ptr(), ws.numel(), st), "linear_int8")
     return out
 
 
@@ -816,10 +834,11 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional
     a = L.Kv4AttnArgs(c, rows // c.n_seq, heads, bound, _DTYPE[q.dtype], 1, scale, pp, q.data_ptr(), _ld(q), rope, tm,
                       out.data_ptr())
     with _on(dev) as st:
-        cl = lib()
+        cl, sc = lib(), _stream_ws(dev, "kv4", st)
         ref = ctypes.byref(a)
-        ws = _stream_ws(dev, "kv4", st, cl.lbx_kv4_attn_workspace_size(ref) or 1)
-        L.check(cl.lbx_kv4_attn(ref, ws.data_ptr(), ws.numel(), st), "attention_kv4")
+        with sc.lock:
+            ws = sc.take(cl.lbx_kv4_attn_workspace_size(ref) or 1)
+            L.check(cl.lbx_kv4_attn(ref, ws.data_ptr(), ws.numel(), st), "attention_kv4")
     return out
 
 

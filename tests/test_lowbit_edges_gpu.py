@@ -75,3 +75,35 @@ def test_a_slot_that_is_no_number_reaches_the_rows_that_see_it_alone(half, bad, 
     tree = ops.attention_kv4(q, c, prefix, None, heads, d ** -0.5,
                              tree_mask=torch.tensor([1, 3, 5], dtype=torch.int64, device="cuda"))
     assert torch.equal(tree[0], clean[0]) and not torch.isnan(tree[2]).any()
+
+
+def test_threads_on_one_stream_keep_their_results():
+    import threading
+
+    from littlebit_b200 import ops
+
+    d, heads = 128, 8
+    g = torch.Generator().manual_seed(11)
+    c = _cache(1, 2, 1024, d, 4)
+    w = torch.randint(-127, 128, (700, 512), generator=g, dtype=torch.int32).to(torch.int8).cuda()
+    ws = torch.rand(700, generator=g).cuda()
+    xs = [torch.randn(m, 512, generator=g).cuda() for m in (1, 7, 33, 64)]
+    qs = [torch.randn(n, heads * d, generator=g).cuda() for n in (1, 2, 5, 9)]
+    want = [(ops.linear_int8(x, w, ws), ops.attention_kv4(q, c, 900, None, heads, 0.1)) for x, q in zip(xs, qs)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            for _ in range(150):
+                y = ops.linear_int8(xs[i], w, ws)
+                o = ops.attention_kv4(qs[i], c, 900, None, heads, 0.1)
+                if not (torch.equal(y, want[i][0]) and torch.equal(o, want[i][1])):
+                    bad.append(i)
+        except BaseException as e:  # noqa: BLE001 (told below, from the main thread)
+            bad.append(repr(e))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad and ops.device_error() == 0

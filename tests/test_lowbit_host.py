@@ -114,3 +114,139 @@ def test_sampled_loop_refusals():
         a = dict(start=4, max_new=3, gamma=2) | kw
         with pytest.raises(ValueError):
             bd.sampled_speculative_generate(m, m, prompt[:, 2], prompt[:, 3], a["start"], a["max_new"], gamma=a["gamma"])
+
+
+def _scratch_on_the_cpu(monkeypatch):
+    import torch
+
+    from littlebit_b200 import ops
+
+    plain = ops.Workspace.__init__
+    monkeypatch.setattr(ops.Workspace, "__init__", lambda self, device: plain(self, torch.device("cpu")))
+    monkeypatch.setattr(ops, "_SCRATCH", {})
+    monkeypatch.setattr(ops, "_capturing", lambda: False)
+    return ops
+
+
+def test_threads_on_one_stream_take_turns_at_its_scratch(monkeypatch):
+    """A call's launches stay together: while one thread has the scratch no other thread's call of the operator on
+    that stream may enqueue; calls on other streams, and other operators', may."""
+    import threading
+    import time
+
+    ops = _scratch_on_the_cpu(monkeypatch)
+    inside, most, bufs = {}, {}, {}
+    note = threading.Lock()
+
+    def call(tag, stream, nbytes):
+        for i in range(20):
+            sc = ops._stream_ws(0, tag, stream)
+            with sc.lock:
+                assert sc.take(nbytes + i).numel() >= nbytes + i
+                with note:
+                    inside[tag, stream] = inside.get((tag, stream), 0) + 1
+                    most[tag, stream] = max(most.get((tag, stream), 0), inside[tag, stream])
+                    most["all"] = max(most.get("all", 0), sum(inside.values()))
+                    bufs.setdefault((tag, stream), set()).add(id(sc))
+                time.sleep(0.0005)  # (the C call: other threads run)
+                with note:
+                    inside[tag, stream] -= 1
+
+    ts = [threading.Thread(target=call, args=a) for a in (("int8", 7, 64), ("int8", 7, 64), ("int8", 7, 640),
+                                                          ("int8", 8, 64), ("kv4", 7, 64))]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert most["int8", 7] == 1 and most["all"] > 1
+    assert len(bufs["int8", 7]) == 1 and len(set.union(*bufs.values())) == 3
+    assert all(v == 0 for v in inside.values())
+
+
+class _Watch:
+    """Stands in for the C library: notes calls that overlap in one scratch."""
+
+    def __init__(self):
+        import threading
+
+        self.note, self.now, self.clash = threading.Lock(), {}, 0
+
+    def lbx_linear_int8_workspace_size(self, m, n, k):
+        return 8192
+
+    def lbx_kv4_attn_workspace_size(self, a):
+        return 8192
+
+    def _call(self, ws):
+        import time
+
+        with self.note:
+            self.clash += self.now.get(ws, 0) > 0
+            self.now[ws] = self.now.get(ws, 0) + 1
+        time.sleep(0.001)
+        with self.note:
+            self.now[ws] -= 1
+        return 0
+
+    def lbx_linear_int8(self, a, ws, nbytes, stream):
+        return self._call(ws)
+
+    def lbx_kv4_attn(self, a, ws, nbytes, stream):
+        return self._call(ws)
+
+
+@pytest.mark.parametrize("op", ["linear_int8", "attention_kv4"])
+def test_calls_of_two_threads_do_not_overlap_in_their_scratch(monkeypatch, op):
+    """The public entries, their library and device replaced, on tensors of the CPU that pass for the GPU's."""
+    import threading
+    import types
+
+    import torch
+
+    ops = _scratch_on_the_cpu(monkeypatch)
+    watch = _Watch()
+    monkeypatch.setattr(ops, "lib", lambda: watch)
+    monkeypatch.setattr(ops, "_rows", lambda name, t, dtypes=None: t)
+    scratch = ops._stream_ws
+    monkeypatch.setattr(ops, "_stream_ws", lambda index, *a: scratch(0, *a))  # (a tensor of the CPU is on device -1)
+
+    class On:
+        def __init__(self, index):
+            pass
+
+        def __enter__(self):
+            return 7
+
+        def __exit__(self, *exc):
+            pass
+
+    monkeypatch.setattr(ops, "_on", On)
+    cache = types.SimpleNamespace(struct=lambda: L.Kv4Cache(256, 256, 256, 256, 1, 1, 64, 64), index=-1)
+    x, w, s = torch.zeros(2, 64), torch.zeros(16, 64, dtype=torch.int8), torch.ones(16)
+
+    def work():
+        for _ in range(20):
+            if op == "linear_int8":
+                ops.linear_int8(x, w, s)
+            else:
+                ops.attention_kv4(x, cache, 0, None, 1, 0.1)
+
+    ts = [threading.Thread(target=work) for _ in range(3)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert watch.clash == 0 and sum(watch.now.values()) == 0 and len(watch.now) == 1
+
+
+def test_scratch_is_given_up_after_an_error(monkeypatch):
+    import threading
+
+    ops = _scratch_on_the_cpu(monkeypatch)
+    for _ in range(2):
+        sc = ops._stream_ws(0, "int8", 1)
+        with pytest.raises(RuntimeError, match="invalid argument"):
+            with sc.lock:
+                sc.take(64)
+                L.check(L.load().lbx_linear_int8(None, None, 0, None), "linear_int8")
+    got = []
+    t = threading.Thread(target=lambda: got.append(sc.lock.acquire(blocking=False)))
+    t.start()
+    t.join()
+    assert got == [True] and sc.get(64).numel() >= 64
