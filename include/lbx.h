@@ -433,8 +433,9 @@ int lbx_kv_move(uint16_t *const *k_caches, uint16_t *const *v_caches, int32_t n_
  *
  * lbx_quant_tokens: for each of m rows of x [m, k] (fp32 or bf16, row stride
  * x_ld elements) a = max |x|, scale = a * (1/127 in fp32) and
- * q = rint(x * i), i = 127 / a (0 where a = 0), each operation rounded to
- * fp32, ties to even; |q| <= 127.  A row holding a NaN or an infinity gets
+ * q = rint(x * i), i = 127 / a (0 where a = 0 and where fp32 does not hold 127 / a,
+ * a < 3.74e-37: such a row's codes are 0), each operation rounded to fp32, ties to
+ * even; |q| <= 127.  A row holding a NaN or an infinity gets
  * scale NaN and codes 0.  q rows are q_ld bytes apart (q_ld >= k).  The same
  * call quantises a weight matrix, its rows being the output channels. */
 int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, int32_t m, int32_t k, int8_t *q,

@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
   for (int i = 0; i < Q8_THREADS / 32; ++i) m = max(m, red[i]);
   const bool fin = m < 0x7F800000u;
   const float a = __uint_as_float(m);
-  const float inv = fin && a > 0.f ? __fdiv_rn(127.0f, a) : 0.f;
+  float inv = fin && a > 0.f ? __fdiv_rn(127.0f, a) : 0.f;
+  if (!(inv < INFINITY)) inv = 0.f;  // (a below 127 / FLT_MAX: the row is 0, as a 4-bit group with so small a step)
   if (tid == 0) scale[row] = fin ? __fmul_rn(a, 1.0f / 127.0f) : __uint_as_float(0x7FC00000u);
   auto put = [&](int e, const uint4 &w) {
     q8_unpack<XDT>(w, v);

@@ -30,6 +30,7 @@ def quantize_tokens(x):
     fin = np.isfinite(a)
     with np.errstate(all="ignore"):
         inv = np.where(fin & (a > 0), np.float32(127) / a, np.float32(0)).astype(np.float32)
+        inv = np.where(np.isfinite(inv), inv, np.float32(0))
         q = np.where(fin[:, None], np.rint(x * inv[:, None]), 0)
         scale = np.where(fin, a * np.float32(1 / 127), np.float32(np.nan)).astype(np.float32)
     return q.astype(np.int8), scale

@@ -107,3 +107,28 @@ def test_threads_on_one_stream_keep_their_results():
     [t.start() for t in ts]
     [t.join() for t in ts]
     assert not bad and ops.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1e-45, 1e-40, 1.1754943508222875e-38, 1e-37, 3.7e-37, 3.8e-37, 1e-36, 1e-30, 1e30, 3.3e38])
+def test_eight_bit_codes_of_rows_of_any_magnitude(top, dtype):
+    """Codes are 127 x / a wherever float32 holds 127 / a (from a = 3.74e-37 on), and 0 below: never a
+    sign or a size that the row does not have."""
+    from littlebit_b200 import ops
+
+    x = torch.linspace(-1, 1, 200, dtype=torch.float64)
+    rows = torch.stack([x, x.flip(0) * 0.5, -x.abs()]) * top
+    rows = rows.float().to(DT[dtype])
+    q, s = ops.quantize_tokens(rows.cuda())
+    rq, rs = olow.quantize_tokens(rows.float().numpy())
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
+    np.testing.assert_array_equal(s.cpu().numpy(), rs)
+    f = rows.double()
+    assert (q.cpu().double() * f >= 0).all()
+    a = f.abs().amax(1, keepdim=True)
+    held = (a > 3.75e-37) if top > 1e-38 else torch.zeros_like(a, dtype=torch.bool)
+    want = torch.where(held, f / a.clamp_min(1e-300) * 127, torch.zeros_like(f))
+    assert ((q.cpu().double() - want).abs() <= 0.5 + 1e-4).all()
+    w = torch.ones(16, 208, dtype=torch.int8, device="cuda")[:, :200]
+    y = ops.linear_int8(rows.cuda(), w, torch.ones(16, device="cuda"), out_dtype=torch.float32)
+    assert (y[:, 0].cpu().double().numpy() * rq.astype(np.float64).sum(1) >= 0).all()

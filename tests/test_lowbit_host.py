@@ -250,3 +250,15 @@ def test_scratch_is_given_up_after_an_error(monkeypatch):
     t.start()
     t.join()
     assert got == [True] and sc.get(64).numel() >= 64
+
+
+def test_eight_bit_codes_of_rows_that_nearly_vanish():
+    """127 / a is no float32 below a = 3.74e-37: codes 0, never another sign."""
+    import numpy as np
+
+    from oracle import lowbit as olow
+
+    x = np.array([[1, -1, 0.5]], np.float32)
+    for top, want in ((1e-45, 0), (1e-38, 0), (3.7e-37, 0), (3.8e-37, 127), (1e-30, 127)):
+        q, s = olow.quantize_tokens((x * np.float32(top)).astype(np.float32))
+        assert q[0, :2].tolist() == [want, -want] and 0 <= s[0] < 1e-32
