@@ -548,7 +548,8 @@ int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_byte
  * target_0: the sampler of the drafts themselves.  draft == NULL: the drafts
  * were not sampled (greedy or looked up), q_i is 1 at d_i.  T = 0 (up to 1e-30): p
  * and q are 1 at their first maximum.  A logit of -inf or NaN has probability 0; +inf
- * counts as the maximum, shared equally.  A row without any probability
+ * counts as the largest float.  A mask of the type's lowest number is a number: a row
+ * of nothing else has equal probabilities.  A row without any probability
  * rejects its draft, and gives the next token -1.  A draft outside the
  * vocabulary is rejected (device error 0x811), q_i then taken as it is.
  * n_draft[s] outside [0, k] is clamped (device error 0x812). */

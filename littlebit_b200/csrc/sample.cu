@@ -43,10 +43,12 @@ constexpr int AC_ONE = 12, AC_TWO = 32;
 constexpr int AC_C = 8;      // blocks a sequence
 constexpr int AC_Q = 4;      // quads of logits a lane loads together
 constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
-// Scaled logits y = x * log2(e) / T stay within +-AC_TOP, NaN at the bottom: weights
-// 2^(y - top) then need no case of their own for infinities, and 36 instructions a
-// logit (selects turned into branches) became 7.
-constexpr float AC_TOP = 3e38f;
+// Logits are kept within [-inf, AC_TOP], NaN as -inf, and a row's top starts at -AC_TOP:
+// weights 2^((x - top) log2(e) / T) then need no case of their own for infinities, and 36
+// instructions a logit (selects turned into branches) became 7.  -inf has the weight 0 against
+// any top; a mask of the type's lowest number is a number, and a row of nothing else has
+// equal probabilities.  (Scaled before the subtraction, such numbers overflowed.)
+constexpr float AC_TOP = 3.402823466e38f;  // the largest float
 constexpr float AC_COLD = 1e-30f;  // temperatures up to here take the maximum
 
 // does a row start on 16 (fp32) or 8 (bf16) bytes
@@ -71,7 +73,7 @@ LBX_DEV float4 ac_quad(const void *row, bool vec, int q, int V) {
   for (int i = 0; i < 4; ++i) v[i] = 4 * q + i < V ? load_act(row, DT, 4 * (int64_t)q + i) : -INFINITY;
   return make_float4(v[0], v[1], v[2], v[3]);
 }
-LBX_DEV float ac_scaled(float x, float c) { return fminf(fmaxf(x * c, -AC_TOP), AC_TOP); }
+LBX_DEV float ac_held(float x) { return fminf(fmaxf(x, -INFINITY), AC_TOP); }
 LBX_DEV float ac_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -90,10 +92,12 @@ LBX_DEV uint64_t warp_max64(uint64_t v) {
   }
   return v;
 }
+// the weight of x against a top, c = log2(e) / T
+LBX_DEV float ac_weight(float x, float top, float c) { return ac_ex2((x - top) * c); }
 // (top, sum of weights against it) of two parts of a row; a part of nothing: (-AC_TOP, 0)
-LBX_DEV float2 ac_join(float2 a, float2 b) {
+LBX_DEV float2 ac_join(float2 a, float2 b, float c) {
   const float m = fmaxf(a.x, b.x);
-  return make_float2(m, a.y * ac_ex2(a.x - m) + b.y * ac_ex2(b.x - m));
+  return make_float2(m, a.y * ac_weight(a.x, m, c) + b.y * ac_weight(b.x, m, c));
 }
 LBX_DEV uint64_t ac_pack(float2 v) { return (uint64_t)__float_as_uint(v.x) << 32 | __float_as_uint(v.y); }
 LBX_DEV float2 ac_pair(uint64_t v) { return make_float2(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v)); }
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
   pdl_wait();
   const float T = p.temps ? __ldg(p.temps + s) : p.temperature;
   const bool greedy = !(T > AC_COLD);
-  const float c = 1.4426950408889634f / T;
+  const float c = fmaxf(1.4426950408889634f / T, 1e-30f);  // (an infinite T: -inf times 0 would be no number)
   const uint64_t none = greedy ? 0ull : ac_pack(make_float2(-AC_TOP, 0.f));
   int nd = p.k;
   if (p.n_draft) {
@@ -189,24 +193,23 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
         float mn = m;
 #pragma unroll
         for (int i = 0; i < AC_Q; ++i) {
-          x[i] = make_float4(ac_scaled(x[i].x, c), ac_scaled(x[i].y, c), ac_scaled(x[i].z, c), ac_scaled(x[i].w, c));
+          x[i] = make_float4(ac_held(x[i].x), ac_held(x[i].y), ac_held(x[i].z), ac_held(x[i].w));
           mn = fmaxf(mn, fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w)));
         }
-        l *= ac_ex2(m - mn);
+        l *= ac_weight(m, mn, c);
         m = mn;
-        // (a top still at the bottom: nothing but -inf so far, whose weights of 1 the rows' totals drop)
 #pragma unroll
         for (int i = 0; i < AC_Q; ++i)
-          l += (ac_ex2(x[i].x - m) + ac_ex2(x[i].y - m)) + (ac_ex2(x[i].z - m) + ac_ex2(x[i].w - m));
+          l += (ac_weight(x[i].x, m, c) + ac_weight(x[i].y, m, c)) + (ac_weight(x[i].z, m, c) + ac_weight(x[i].w, m, c));
       }
       if (r2 != r || it + 1 >= end) {
         if (greedy) {
           key = warp_max64(key);
         } else {
-          float2 ml = make_float2(m, m > -AC_TOP ? l : 0.f);
+          float2 ml = make_float2(m, l);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1)
-            ml = ac_join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o)));
+            ml = ac_join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, o), __shfl_xor_sync(0xffffffffu, ml.y, o)), c);
           key = ac_pack(ml);
         }
         if (lane == 0) part[r][warp] = key;
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
   }
   auto join = [&](uint64_t a, uint64_t b) {
     if (greedy) return a > b ? a : b;
-    return ac_pack(ac_join(ac_pair(a), ac_pair(b)));
+    return ac_pack(ac_join(ac_pair(a), ac_pair(b), c));
   };
   // lanes xor o, 2 o, ... joined; every block goes the same way
   auto reduce = [&](uint64_t v, int o) {
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
   auto first_of = [](uint64_t k) { return k ? (int64_t)(0xFFFFFFFFu - (uint32_t)k) : -1; };
   auto prob = [&](float x, int r) {
     const float2 ml = ac_pair(tot[r]);
-    return ml.y > 0.f ? ac_ex2(ac_scaled(x, c) - ml.x) / ml.y : 0.f;
+    return ml.y > 0.f ? ac_weight(ac_held(x), ml.x, c) / ml.y : 0.f;
   };
   if (tid < nd) {
     bool ok;
@@ -330,9 +333,9 @@ __global__ void __launch_bounds__(AC_T, 1024 / AC_T) accept_kernel(const __grid_
           for (int e = 0; e < 4; ++e) {
             const int v = 4 * (b + i * AC_T) + e;
             // (products rounded on their own: equal rows leave exactly nothing)
-            float r = __fmul_rn(ac_ex2(ac_scaled(xs[e], c) - pm.x), pi);
+            float r = __fmul_rn(ac_weight(ac_held(xs[e]), pm.x, c), pi);
             if (less) {
-              if (q) r = __fsub_rn(r, __fmul_rn(ac_ex2(ac_scaled(ys[e], c) - qm.x), qi));
+              if (q) r = __fsub_rn(r, __fmul_rn(ac_weight(ac_held(ys[e]), qm.x, c), qi));
               else if (v == dtok) r -= 1.f;
             }
             if (r > 0.f) {

@@ -132,3 +132,50 @@ def test_eight_bit_codes_of_rows_of_any_magnitude(top, dtype):
     w = torch.ones(16, 208, dtype=torch.int8, device="cuda")[:, :200]
     y = ops.linear_int8(rows.cuda(), w, torch.ones(16, device="cuda"), out_dtype=torch.float32)
     assert (y[:, 0].cpu().double().numpy() * rq.astype(np.float64).sum(1) >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("S", [1, 20, 40])
+@pytest.mark.parametrize("T", [0.4, 1.0, 2.0])
+def test_rows_of_the_lowest_number_are_uniform(T, S, dtype):
+    """A row whose every logit is the type's lowest number has equal probabilities; only -inf and NaN have none."""
+    from littlebit_b200 import ops
+
+    V = 1003
+    low = torch.finfo(DT[dtype]).min
+    g = torch.Generator().manual_seed(S)
+    e = -torch.log(torch.rand(S, V, generator=g).clamp_min(1e-30)) + 1e-30
+    t = torch.full((S, 1, V), low, dtype=DT[dtype])
+    _, nxt = ops.accept_sampled(None, t.cuda(), None, None, e.cuda(), T)
+    assert torch.equal(nxt.cpu(), e.argmin(-1))
+    # with some of them masked by -inf and NaN, among the others
+    t[:, :, ::2] = float("-inf")
+    t[:, :, 1::10] = float("nan")
+    _, nxt = ops.accept_sampled(None, t.cuda(), None, None, e.cuda(), T)
+    left = e.clone()
+    left[:, ::2] = left[:, 1::10] = float("inf")
+    assert torch.equal(nxt.cpu(), left.argmin(-1))
+    # beside an ordinary logit they have no probability
+    t[:, :, 5] = -40.0
+    _, nxt = ops.accept_sampled(None, t.cuda(), None, None, e.cuda(), T)
+    assert (nxt == 5).all()
+    # nothing but -inf and NaN
+    t[:] = float("-inf")
+    t[:, :, 7] = float("nan")
+    _, nxt = ops.accept_sampled(None, t.cuda(), None, None, e.cuda(), T)
+    assert (nxt == -1).all()
+
+
+def test_a_draft_from_a_row_of_the_lowest_number():
+    """p and q uniform: the ratio is 1 and every draft is accepted; p against a q elsewhere: refused by q's excess alone."""
+    from littlebit_b200 import ops
+
+    V, low = 64, torch.finfo(torch.float32).min
+    t = torch.full((2, 2, V), low)
+    d = torch.full((2, 1, V), low)
+    d[1, 0, 9] = 0.0                       # q is 1 at 9, p is 1/64
+    u = torch.tensor([[0.999], [0.02]])    # above 1/64
+    e = torch.rand(2, V, generator=torch.Generator().manual_seed(1)) + 0.1
+    acc, nxt = ops.accept_sampled(torch.tensor([[3], [9]]).cuda(), t.cuda(), d.cuda(), u.cuda(), e.cuda())
+    e[1, 9] = 9.0
+    assert acc.tolist() == [1, 0] and nxt.cpu().tolist() == e.argmin(-1).tolist()
