@@ -81,7 +81,7 @@ LBX_DEV float ac_ex2(float x) {
 }
 // the larger value first, then the lower index; 0 for -inf and NaN
 LBX_DEV uint64_t ac_key(float x, uint32_t i) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(__fadd_rn(x, 0.f));  // (-0 becomes 0: the two are equal)
   return x > -INFINITY ? (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i) : 0ull;
 }
 LBX_DEV uint64_t warp_max64(uint64_t v) {

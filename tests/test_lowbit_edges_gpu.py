@@ -179,3 +179,16 @@ def test_a_draft_from_a_row_of_the_lowest_number():
     acc, nxt = ops.accept_sampled(torch.tensor([[3], [9]]).cuda(), t.cuda(), d.cuda(), u.cuda(), e.cuda())
     e[1, 9] = 9.0
     assert acc.tolist() == [1, 0] and nxt.cpu().tolist() == e.argmin(-1).tolist()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("at", [(3, 4), (0, 999), (500, 501), (31, 512)])
+def test_zeros_of_either_sign_are_a_tie(at, dtype):
+    from littlebit_b200 import ops
+
+    t = torch.full((3, 1, 1000), -1.0, dtype=DT[dtype])
+    t[0, 0, at[0]], t[0, 0, at[1]] = -0.0, 0.0
+    t[1, 0, at[0]], t[1, 0, at[1]] = 0.0, -0.0
+    t[2, 0, at[0]], t[2, 0, at[1]] = -0.0, -0.0
+    _, nxt = ops.accept_sampled(None, t.cuda(), None, None, torch.ones(3, 1000, device="cuda"), 0.0)
+    assert nxt.tolist() == [at[0]] * 3
