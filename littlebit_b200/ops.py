@@ -759,11 +759,12 @@ class Kv4Cache:
         return self._struct
 
 
-def _start_arg(name: str, start, n_seq: int, bound: Optional[int], max_seq: int, index: int):
+def _start_arg(name: str, start, n_seq: int, bound: Optional[int], last: int, index: int):
     """(device address or None, host bound) of per-sequence slot counts: an int for all,
-    or a device int32 [n_seq] with its host-side upper bound."""
+    or a device int32 [n_seq] with its host-side upper bound (``last``, the last slot that
+    the call's tokens fit at, where the caller names none)."""
     if isinstance(start, torch.Tensor):
-        return _vec(name, start, n_seq, torch.int32, index), max_seq if bound is None else int(bound)
+        return _vec(name, start, n_seq, torch.int32, index), last if bound is None else int(bound)
     return None, int(start)
 
 
@@ -774,7 +775,7 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start,
 
     k_new / v_new [S * n, kv_heads * head_dim], float32 or bfloat16, sequence by
     sequence.  ``start``: first slot, an int for every sequence, or a device int32
-    [S] bounded by ``max_start``."""
+    [S] bounded by ``max_start`` (None: the last slot that the tokens fit at)."""
     c, dev = cache.struct(), cache.index
     _rows("k_new", k_new)
     _rows("v_new", v_new, (k_new.dtype,))
@@ -787,7 +788,7 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start,
     ld = _ld(k_new)
     if rows > 1 and _ld(v_new) != ld:
         raise RuntimeError("k_new and v_new must have one row stride")
-    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq, dev)
+    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq - rows // c.n_seq, dev)
     rope = None if rope_cs is None else _vec("rope_cs", rope_cs, rows * c.head_dim, torch.float32, dev)
     a = L.Kv4AppendArgs(c, rows // c.n_seq, bound, _DTYPE[k_new.dtype], 1, sp, k_new.data_ptr(), v_new.data_ptr(), ld,
                         rope)
@@ -796,9 +797,10 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, cache: Kv4Cache, start,
 
 
 def kv4_read(cache: Kv4Cache, start, max_start: Optional[int], n: int):
-    """The values of n slots of every sequence: (k, v) float32 [S, kv_heads, n, head_dim]."""
+    """The values of n slots of every sequence: (k, v) float32 [S, kv_heads, n, head_dim].
+    ``start`` and ``max_start`` as of :func:`kv4_append`."""
     c, dev = cache.struct(), cache.index
-    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq, dev)
+    sp, bound = _start_arg("start", start, c.n_seq, max_start, c.max_seq - n, dev)
     kv = torch.empty(2, c.n_seq, c.kv_heads, n, c.head_dim, dtype=torch.float32, device=cache.k_codes.device)
     k, v = kv.unbind(0)
     with _on(dev) as st:
@@ -814,7 +816,8 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional
 
     q [S * n, heads * head_dim], float32 or bfloat16, is rotated by ``rope_cs``.
     ``prefix``: cached slots before the new tokens, an int, or a device int32 [S]
-    bounded by ``max_prefix``.  A query sees its sequence's cached slots and the
+    bounded by ``max_prefix`` (None: as many as leave room for the new tokens; a near bound
+    makes a smaller grid).  A query sees its sequence's cached slots and the
     new ones up to itself, or those of its ``tree_mask`` bits (int64 [S * n], n <= 64).
     A query that sees nothing gives zeros.  Result: q's shape and type."""
     c, dev = cache.struct(), cache.index
@@ -824,7 +827,7 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, prefix, max_prefix: Optional
         raise RuntimeError("q and the cache must be on one device")
     if rows == 0 or rows % c.n_seq or width != heads * c.head_dim:
         raise RuntimeError(f"q must be [{c.n_seq} * n, {heads * c.head_dim}], got {tuple(q.shape)}")
-    pp, bound = _start_arg("prefix", prefix, c.n_seq, max_prefix, c.max_seq, dev)
+    pp, bound = _start_arg("prefix", prefix, c.n_seq, max_prefix, c.max_seq - rows // c.n_seq, dev)
     rope = None if rope_cs is None else _vec("rope_cs", rope_cs, rows * c.head_dim, torch.float32, dev)
     tm = None if tree_mask is None else _vec("tree_mask", tree_mask, rows, torch.int64, dev)
     if out is None:

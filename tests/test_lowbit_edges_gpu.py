@@ -192,3 +192,24 @@ def test_zeros_of_either_sign_are_a_tie(at, dtype):
     t[2, 0, at[0]], t[2, 0, at[1]] = -0.0, -0.0
     _, nxt = ops.accept_sampled(None, t.cuda(), None, None, torch.ones(3, 1000, device="cuda"), 0.0)
     assert nxt.tolist() == [at[0]] * 3
+
+
+def test_a_device_start_without_a_bound_reaches_the_whole_cache():
+    from littlebit_b200 import ops
+
+    c = ops.Kv4Cache.empty(2, 1, 64, 64)
+    x = torch.randn(2 * 3, 64, device="cuda")
+    at = torch.tensor([0, 61], dtype=torch.int32, device="cuda")  # the last start that three tokens fit at
+    ops.clear_device_error()
+    ops.kv4_append(x, x, c, at)
+    k, v = ops.kv4_read(c, at, None, 3)
+    y = ops.attention_kv4(x, c, at, None, 1, 0.125)
+    assert ops.device_error() == 0
+    w, p = olow.kv4_quantize(x.cpu().numpy().reshape(2, 3, 64))
+    np.testing.assert_allclose(v[:, 0].cpu().numpy(), olow.kv4_values(w, p), rtol=2 ** -23, atol=1e-6)
+    assert torch.equal(k, v)
+    assert torch.equal(y, ops.attention_kv4(x, c, at, 61, 1, 0.125))
+    # past the last start: told, as with a bound of the caller's
+    ops.kv4_append(x, x, c, at + 1)
+    assert ops.device_error() == 0x801
+    ops.clear_device_error()
