@@ -32,7 +32,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import _lib as L
-from .model import LittleBitDecoder
+from .model import LittleBitDecoder, cache_slots
 from .ops import Int8Linear, Kv4Cache, _p, _stream, accept_sampled, kv4_append, lib
 
 
@@ -46,9 +46,7 @@ class BatchDecoder:
             raise ValueError("1..64 sequences per batch decoder")
         if kv_bits not in (4, 16):
             raise ValueError("kv_bits must be 4 or 16")
-        self.dec, self.S, self.max_seq, self.kv_bits = dec, int(n_seq), int(max_seq), kv_bits
-        if kv_bits == 4:
-            self.max_seq = -(-self.max_seq // 64) * 64
+        self.dec, self.S, self.max_seq, self.kv_bits = dec, int(n_seq), cache_slots(max_seq, kv_bits), kv_bits
         s = dec.shape
         dev = dec.device
         self.device = dev

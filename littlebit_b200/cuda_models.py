@@ -30,7 +30,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib as L
-from .model import DecoderShape, LittleBitDecoder, load_runtime
+from .model import DecoderShape, LittleBitDecoder, cache_slots, load_runtime
 from .ops import PackedLinear, _p, _stream, accept_greedy_chain, lib, lmhead_argmax
 
 PREFILL_CHUNK = 16  # tokens per decoder step while prefilling
@@ -62,9 +62,10 @@ def _embed_and_head(state, base_model_id):
 
 def _branch0_view(dec: LittleBitDecoder, max_seq: int) -> LittleBitDecoder:
     """A decoder over branch 0 of every projection of ``dec`` (same device tensors,
-    its own KV cache and workspace)."""
+    its own KV cache, of ``dec``'s bits, and workspace)."""
     v = LittleBitDecoder.__new__(LittleBitDecoder)
-    v.shape, v.device, v.max_seq, v.use_pdl = dec.shape, dec.device, max_seq, dec.use_pdl
+    v.shape, v.device, v.use_pdl, v.kv_bits = dec.shape, dec.device, dec.use_pdl, dec.kv_bits
+    v.max_seq = cache_slots(max_seq, dec.kv_bits)
     v.exec_mode = getattr(dec, "exec_mode", L.LBX_EXEC_AUTO)
     v.embed, v.lm_head, v.final_norm = dec.embed, dec.lm_head, dec.final_norm
     v.layers = []
@@ -72,7 +73,6 @@ def _branch0_view(dec: LittleBitDecoder, max_seq: int) -> LittleBitDecoder:
         v.layers.append({"ln1": ly["ln1"], "ln2": ly["ln2"],
                          "projs": [PackedLinear(p.in_features, p.out_features, p.branches[:1], p.bias)
                                    for p in ly["projs"]]})
-    v.kv_bits = dec.kv_bits
     v._alloc_cache()
     v._build_struct()
     v._ws = torch.zeros(0, dtype=torch.uint8, device=dec.device)

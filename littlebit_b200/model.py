@@ -99,6 +99,11 @@ def branches_from_runtime(state: Dict[str, torch.Tensor], prefix: str, device,
     return br
 
 
+def cache_slots(max_seq: int, kv_bits: int) -> int:
+    """Slots of a cache asked to hold max_seq: a 4-bit one has a multiple of 64."""
+    return -(-int(max_seq) // 64) * 64 if kv_bits == 4 else int(max_seq)
+
+
 class LittleBitDecoder:
     """A LittleBit Llama decoder resident on one GPU, with its own KV cache."""
 
@@ -116,7 +121,7 @@ class LittleBitDecoder:
         self.shape = shape
         self.device = torch.device(device)
         self.kv_bits = kv_bits
-        self.max_seq = -(-int(max_seq) // 64) * 64 if kv_bits == 4 else int(max_seq)
+        self.max_seq = cache_slots(max_seq, kv_bits)
         self.use_pdl = use_pdl
         self.exec_mode = exec_mode
         dev = self.device

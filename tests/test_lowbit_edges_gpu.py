@@ -213,3 +213,22 @@ def test_a_device_start_without_a_bound_reaches_the_whole_cache():
     ops.kv4_append(x, x, c, at + 1)
     assert ops.device_error() == 0x801
     ops.clear_device_error()
+
+
+@pytest.mark.parametrize("max_seq", [1, 64, 100])
+def test_a_draft_view_of_a_four_bit_decoder_steps_by_itself(max_seq):
+    from littlebit_b200.cuda_models import _branch0_view
+    from littlebit_b200.model import DecoderShape, LittleBitDecoder, synthetic_runtime_state
+
+    shape = DecoderShape(num_hidden_layers=2, hidden_size=256, intermediate_size=512, num_attention_heads=4,
+                         num_key_value_heads=2, vocab_size=512)
+    ranks = {"q_proj": [64, 32], "k_proj": [32, 16], "v_proj": [32, 16], "o_proj": [64, 32],
+             "gate_proj": [96, 40], "up_proj": [96, 40], "down_proj": [96, 40]}
+    st = synthetic_runtime_state(shape, ranks, seed=21, unit_gain=True)
+    dec = LittleBitDecoder(shape, st, device="cuda", max_seq=128, kv_bits=4)
+    view = _branch0_view(dec, max_seq)
+    assert view.max_seq == -(-max_seq // 64) * 64 == view.kv4[0].shape[2]
+    wide = _branch0_view(dec, 128)
+    ids = [5, 9, 2, 77][:max_seq]
+    got, want = (x.forward_tokens(ids, 0)["logits"] for x in (view, wide))
+    assert torch.equal(got, want)
