@@ -515,7 +515,8 @@ int lbx_kv4_read(const lbx_kv4_cache *c /* host */, const int32_t *start, int32_
  * apart) is rotated by rope_cs (NULL: not); query i of a sequence sees slots
  * [0, prefix[s]) and the new slots prefix[s] + j with bit j of its tree mask
  * set, or j <= i without one.  A query that sees nothing gives zeros.  Stale
- * slots are never used, whatever they hold.  Query head h reads kv head
+ * slots are never used, whatever they hold; a slot whose step or least value is
+ * no number makes the rows that see it NaN, and no other.  Query head h reads kv head
  * h / (heads / kv_heads).  n <= 64 with a tree mask, any n without.  out
  * [n_seq * n, heads * head_dim] has q's type.  A query's bits depend neither on
  * the other queries and sequences of the call nor on max_prefix, so a causal

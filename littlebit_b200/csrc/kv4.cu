@@ -252,8 +252,9 @@ LBX_DEV uint32_t f16x2_rest(uint32_t r, float lo, float hi) {
   const __half2 h = *reinterpret_cast<const __half2 *>(&r);
   return f16x2(lo - __low2float(h), hi - __high2float(h));
 }
-// exponent of |x| <- its bits, within what the power-of-two factors reach
-LBX_DEV int kv4_exp(uint32_t bits) { return min(max((int)(bits >> 23) - 127, -112), 100); }
+// exponent of |x| <- its bits, within what the power-of-two factors reach: steps up to 2^100
+// (past it the sums of the weighted values overflow anyway), queries up to top
+LBX_DEV int kv4_exp(uint32_t bits, int top = 100) { return min(max((int)(bits >> 23) - 127, -112), top); }
 LBX_DEV float kv4_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The masks of the unpacking, in registers: with both a mask and bits to set,
 // immediates would make two instructions of each.
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
     float mq = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) mq = fmaxf(mq, fabsf(x[i]));
-    const int e = kv4_exp(__float_as_uint(quad_max(mq)));
+    const int e = kv4_exp(__float_as_uint(quad_max(mq)), SPLIT ? 127 : 117);  // (unit stays a float)
     const float up = kv4_pow2(14 - e), unit = kv4_pow2(e - 14) * (SPLIT ? 1.f : 16777216.f);
     float sum[NG];
 #pragma unroll

@@ -232,3 +232,60 @@ def test_a_draft_view_of_a_four_bit_decoder_steps_by_itself(max_seq):
     ids = [5, 9, 2, 77][:max_seq]
     got, want = (x.forward_tokens(ids, 0)["logits"] for x in (view, wide))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("exp", [-120, -60, 60, 99, 101, 110, 120])
+def test_float32_queries_of_any_magnitude(exp, d):
+    """Scores that far apart leave the largest one's value (or, for tiny queries, the mean), whatever the
+    queries' exponent."""
+    from littlebit_b200 import ops
+
+    c = _cache(1, 1, 64, d, 9)
+    kv, vv = _values(c, 0, 50)
+    q = torch.randn(1, d, generator=torch.Generator().manual_seed(4)) * 2.0 ** exp
+    y = ops.attention_kv4(q.cuda(), c, 49, None, 1, d ** -0.5).double()[0]
+    s = (kv[0] @ q.cuda().double()[0]) * d ** -0.5
+    want = torch.softmax(s, 0) @ vv[0]
+    # (the two largest scores differ by far more than their rounding, 2^-18 of the largest)
+    top = s.topk(2).values
+    assert exp < 0 or top[0] - top[1] > 2.0 ** -12 * s.abs().max()
+    assert (y - want).norm() <= 2.0 ** -18 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("exp", [-120, -60, 60, 95, 100])
+def test_values_of_any_magnitude(exp, dtype):
+    """Values up to 2^100 and down to the least normal step."""
+    from littlebit_b200 import ops
+
+    d = 64
+    c = ops.Kv4Cache.empty(1, 1, 64, d)
+    g = torch.Generator().manual_seed(6)
+    k = torch.randn(50, d, generator=g).to(DT[dtype])
+    v = (torch.randn(50, d, generator=g) * 2.0 ** exp).to(DT[dtype])
+    ops.kv4_append(k.cuda(), v.cuda(), c, 0)
+    kv, vv = _values(c, 0, 50)
+    q = torch.randn(1, d, generator=g).to(DT[dtype])
+    y = ops.attention_kv4(q.cuda(), c, 49, None, 1, d ** -0.5).double()[0]
+    want = torch.softmax((kv[0] @ q.cuda().double()[0]) * d ** -0.5, 0) @ vv[0]
+    tol = 2.0 ** -18 if dtype == "f32" else 2.0 ** -8
+    assert (y - want).norm() <= tol * want.norm()
+
+
+@pytest.mark.parametrize("exp", [-120, -60, 60, 100, 105, 110, 114])
+def test_bfloat16_queries_of_any_magnitude(exp):
+    """As in float32, with the rounding of the result to bfloat16 (2^-8) and of the queries to 11 bits, which for
+    tiny queries is nothing and for huge ones leaves the largest score the largest."""
+    from littlebit_b200 import ops
+
+    d = 64
+    c = _cache(1, 1, 64, d, 9)
+    kv, vv = _values(c, 0, 50)
+    q = (torch.randn(1, d, generator=torch.Generator().manual_seed(4)) * 2.0 ** exp).bfloat16()
+    y = ops.attention_kv4(q.cuda(), c, 49, None, 1, d ** -0.5).double()[0]
+    s = (kv[0] @ q.cuda().double()[0]) * d ** -0.5
+    want = torch.softmax(s, 0) @ vv[0]
+    top = s.topk(2).values
+    assert exp < 0 or top[0] - top[1] > 2.0 ** -7 * s.abs().max()
+    assert (y - want).norm() <= 2.0 ** -8 * want.norm()
