@@ -437,13 +437,13 @@ int lbx_kv_move(uint16_t *const *k_caches, uint16_t *const *v_caches, int32_t n_
  * a < 3.74e-37: such a row's codes are 0), each operation rounded to fp32, ties to
  * even; |q| <= 127.  A row holding a NaN or an infinity gets
  * scale NaN and codes 0.  q rows are q_ld bytes apart (q_ld >= k).  The same
- * call quantises a weight matrix, its rows being the output channels. */
+ * call quantises a weight matrix, its rows being the output channels.  k <= 2^30. */
 int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, int32_t m, int32_t k, int8_t *q,
                      int64_t q_ld, float *scale, cudaStream_t stream);
 
 typedef struct lbx_int8_args {
-  int32_t m, n, k;        /* tokens, output channels, input features (<= 131072:
-                             127 * 128 * k then fits the int32 sums)           */
+  int32_t m, n, k;        /* tokens and output channels (<= 2^30), input features
+                             (<= 131072: 127 * 128 * k then fits the int32 sums) */
   int32_t x_dtype, y_dtype;
   int32_t use_pdl;
   const void *x; int64_t x_ld;        /* [m, k]                                */
@@ -473,7 +473,7 @@ int lbx_linear_int8(const lbx_int8_args *a /* host */, void *ws, size_t ws_bytes
  *     keys:   (r % 4) * (head_dim / 32) + 2 * g + r / 4
  *     values: r * (head_dim / 64) + g
  * of its row (the orders in which the attention kernel's lanes read them).
- * head_dim is 64 or 128; max_seq a multiple of 64.  Arrays are
+ * head_dim is 64 or 128; max_seq a multiple of 64, up to 2^30.  Arrays are
  * [n_seq, kv_heads, max_seq, head_dim/2] bytes and
  * [n_seq, kv_heads, max_seq, head_dim/64, 2] bf16, 16-byte aligned. */
 typedef struct lbx_kv4_cache {
@@ -555,7 +555,8 @@ int lbx_kv4_attn(const lbx_kv4_attn_args *a /* host */, void *ws, size_t ws_byte
  * vocabulary is rejected (device error 0x811), q_i then taken as it is.
  * n_draft[s] outside [0, k] is clamped (device error 0x812). */
 typedef struct lbx_accept_args {
-  int32_t n_seq, k, vocab, dtype;      /* dtype: of both logits; k <= LBX_ACCEPT_MAX_K */
+  int32_t n_seq, k, vocab, dtype;      /* dtype: of both logits; k <= LBX_ACCEPT_MAX_K,
+                                        * vocab <= 2^30 */
   int32_t use_pdl;
   float temperature;                   /* >= 0; of every sequence when temps == NULL */
   const float *temps;                  /* device [n_seq] or NULL */

@@ -14,6 +14,7 @@ namespace lbx {
 
 constexpr int Q8_THREADS = 256;
 constexpr int Q8_MAXK = 131072;
+constexpr int Q8_MAXDIM = 1 << 30;  // tokens, channels, features of a row: indexes past the end stay 32-bit numbers
 
 // One CTA a row: the absolute maximum, then the codes.  VEC: 16-byte loads, up to
 // Q8_NR of them held in registers from the first pass to the second (rows of up
@@ -588,6 +589,7 @@ extern "C" int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, in
   using namespace lbx;
   LBX_CHECK_ARG(m >= 0 && k >= 1, "bad shape");
   LBX_CHECK_ARG(x_dtype == LBX_F32 || x_dtype == LBX_BF16, "bad dtype");
+  LBX_CHECK_SUP(k <= Q8_MAXDIM, "k must be <= %d", Q8_MAXDIM);
   LBX_CHECK_ARG(x_ld >= k && q_ld >= k, "row strides must be at least k");
   if (m == 0) return LBX_OK;
   LBX_CHECK_ARG(x && q && scale, "NULL pointer");
@@ -595,8 +597,9 @@ extern "C" int lbx_quant_tokens(const void *x, int32_t x_dtype, int64_t x_ld, in
 }
 
 extern "C" size_t lbx_linear_int8_workspace_size(int32_t m, int32_t n, int32_t k) {
-  if (m < 1 || n < 1 || k < 1) return 0;
-  return lbx::i8_plan(m, n, k).total;
+  if (m < 1 || n < 1 || k < 1 || m > lbx::Q8_MAXDIM || n > lbx::Q8_MAXDIM || k > lbx::Q8_MAXK) return 0;
+  const lbx::I8Plan w = lbx::i8_plan(m, n, k);
+  return w.p.BN > 0 ? w.total : 0;
 }
 
 extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
@@ -604,6 +607,7 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   LBX_CHECK_ARG(a, "args is NULL");
   LBX_CHECK_ARG(a->m >= 0 && a->n >= 1 && a->k >= 1, "bad shape");
   LBX_CHECK_SUP(a->k <= Q8_MAXK, "k must be <= %d", Q8_MAXK);
+  LBX_CHECK_SUP(a->m <= Q8_MAXDIM && a->n <= Q8_MAXDIM, "m and n must be <= %d", Q8_MAXDIM);
   LBX_CHECK_ARG((a->x_dtype == LBX_F32 || a->x_dtype == LBX_BF16) && (a->y_dtype == LBX_F32 || a->y_dtype == LBX_BF16),
                 "bad dtype");
   if (a->m == 0) return LBX_OK;

@@ -12,6 +12,7 @@ namespace lbx {
 
 constexpr int KV4_G = 64;       // dimensions a group
 constexpr uint16_t KV4_NAN = 0x7FC0u;
+constexpr int KV4_MAXSEQ = 1 << 30;  // slots of a sequence: those past the end stay 32-bit numbers
 
 // word index, in its row, of block b (dimensions 8b .. 8b+7)
 template <int D, bool VALUE>
@@ -895,6 +896,7 @@ static int kv4_view(const lbx_kv4_cache &c, Kv4View &v) {
   LBX_CHECK_ARG(c.n_seq >= 1 && c.kv_heads >= 1 && c.max_seq >= 1, "bad cache shape");
   LBX_CHECK_SUP(c.head_dim == 64 || c.head_dim == 128, "head_dim must be 64 or 128");
   LBX_CHECK_ARG(c.max_seq % 64 == 0, "max_seq must be a multiple of 64");
+  LBX_CHECK_SUP(c.max_seq <= KV4_MAXSEQ, "max_seq must be <= %d", KV4_MAXSEQ);
   LBX_CHECK_ARG(c.k_codes && c.k_params && c.v_codes && c.v_params, "NULL pointer");
   LBX_CHECK_ARG(aligned16(c.k_codes) && aligned16(c.k_params) && aligned16(c.v_codes) && aligned16(c.v_params),
                 "cache arrays must be 16-byte aligned");

@@ -49,6 +49,7 @@ constexpr int AC_ROWS = 2 * LBX_ACCEPT_MAX_K + 1;
 // any top; a mask of the type's lowest number is a number, and a row of nothing else has
 // equal probabilities.  (Scaled before the subtraction, such numbers overflowed.)
 constexpr float AC_TOP = 3.402823466e38f;  // the largest float
+constexpr int AC_MAXV = 1 << 30;   // logits a row: indexes past the end stay 32-bit numbers
 constexpr float AC_COLD = 1e-30f;  // temperatures up to here take the maximum
 
 // does a row start on 16 (fp32) or 8 (bf16) bytes
@@ -373,6 +374,7 @@ extern "C" int lbx_accept_sampled(const lbx_accept_args *a, cudaStream_t stream)
   LBX_CHECK_ARG(a, "args is NULL");
   LBX_CHECK_ARG(a->n_seq >= 0 && a->k >= 0 && a->vocab >= 1, "bad shape");
   LBX_CHECK_SUP(a->k <= LBX_ACCEPT_MAX_K, "k must be <= %d", LBX_ACCEPT_MAX_K);
+  LBX_CHECK_SUP(a->vocab <= AC_MAXV, "vocab must be <= %d", AC_MAXV);
   LBX_CHECK_ARG(a->dtype == LBX_F32 || a->dtype == LBX_BF16, "bad dtype");
   LBX_CHECK_ARG(a->temps || (a->temperature >= 0.f && a->temperature < INFINITY), "temperature must be >= 0");
   if (a->n_seq == 0) return LBX_OK;

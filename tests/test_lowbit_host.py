@@ -262,3 +262,22 @@ def test_eight_bit_codes_of_rows_that_nearly_vanish():
     for top, want in ((1e-45, 0), (1e-38, 0), (3.7e-37, 0), (3.8e-37, 127), (1e-30, 127)):
         q, s = olow.quantize_tokens((x * np.float32(top)).astype(np.float32))
         assert q[0, :2].tolist() == [want, -want] and 0 <= s[0] < 1e-32
+
+
+def test_sizes_that_32_bits_do_not_hold_are_refused():
+    """Indexes of the kernels are 32-bit within a row, a tile or a cache's slots: sizes so near 2^31 that a
+    step past the end would wrap are refused by the host."""
+    lib, top = L.load(), (1 << 31) - 1
+    for m, n, k in ((top, 1, 16), (1, top, 16), (top - 300, 64, 64), (1, 64, top)):
+        assert lib.lbx_linear_int8_workspace_size(m, n, k) == 0, (m, n, k)
+        a = L.Int8Args(m, n, k, 0, 0, 0, 256, k, 256, -(-k // 16) * 16, 256, None, 256, n)
+        assert lib.lbx_linear_int8(ctypes.byref(a), 256, 1 << 62, None) == L.LBX_EUNSUPPORTED
+    assert lib.lbx_linear_int8_workspace_size((1 << 30), 1, 16) > 1 << 34
+    assert lib.lbx_quant_tokens(256, 0, top, 1, top, 256, top, 256, None) == L.LBX_EUNSUPPORTED
+    s = L.AcceptArgs(n_seq=1, k=0, vocab=top, temperature=1.0, target=256, target_seq=0, target_row=0, e=256, accepted=256,
+                     next=256)
+    assert lib.lbx_accept_sampled(ctypes.byref(s), None) == L.LBX_EUNSUPPORTED
+    c = L.Kv4Cache(256, 256, 256, 256, 1, 1, (1 << 31) - 64, 64)
+    t = L.Kv4AttnArgs(cache=c, n=1, heads=1, max_prefix=0, q=256, q_ld=64, out=256, scale=1.0)
+    assert lib.lbx_kv4_attn_workspace_size(ctypes.byref(t)) == 0
+    assert lib.lbx_kv4_attn(ctypes.byref(t), 256, 1 << 62, None) == L.LBX_EUNSUPPORTED
