@@ -180,7 +180,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 // ordinary additions.  float32 calls centre their codes (a pair of codes is two logic
 // operations at most and one exact subtraction): 3e-7 and 1.2e-6.  bfloat16 calls keep c: in
 // the low bits of a 16-bit lane it IS the fp16 subnormal c * 2^-24, which the tensor cores
-// multiply exactly.  Nibbles 1 and 3 are left at 16 times their value.
+// multiply exactly.  Nibbles 1 and 3 are left at 16 times their value.  Their sums are centred
+// all the same: they begin at 8 times what rounding took from the queries' sum, and at -8
+// times the sum of the rounded weights, so that what a rounding leaves is multiplied by
+// c - 8 and not by c (left out, errors of a head over 2046 slots were 3.1e-3 where the result's
+// own rounding makes 1.7e-3).
 // Codes are the A operand (16 slots x 16 dimensions of the keys, 16 dimensions x 16
 // slots of the values) and query rows the columns of B, eight to a column tile, so that
 // a decode step's few rows waste half a tile at most and the running sums take 4
@@ -233,6 +237,13 @@ LBX_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// (from sums of its own, not d's)
+LBX_DEV void mma_f16_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                          uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 LBX_DEV void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -248,10 +259,18 @@ LBX_DEV uint32_t f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// what the fp16 rounding of (lo, hi) in r left over, as fp16
-LBX_DEV uint32_t f16x2_rest(uint32_t r, float lo, float hi) {
+// what the fp16 rounding of (lo, hi) in r left over; as fp16; its sum
+LBX_DEV float2 f16x2_left(uint32_t r, float lo, float hi) {
   const __half2 h = *reinterpret_cast<const __half2 *>(&r);
-  return f16x2(lo - __low2float(h), hi - __high2float(h));
+  return make_float2(lo - __low2float(h), hi - __high2float(h));
+}
+LBX_DEV uint32_t f16x2_rest(uint32_t r, float lo, float hi) {
+  const float2 v = f16x2_left(r, lo, hi);
+  return f16x2(v.x, v.y);
+}
+LBX_DEV float f16x2_lost(uint32_t r, float lo, float hi) {
+  const float2 v = f16x2_left(r, lo, hi);
+  return v.x + v.y;
 }
 // exponent of |x| <- its bits, within what the power-of-two factors reach: steps up to 2^100
 // (past it the sums of the weighted values overflow anyway), queries up to top
@@ -308,9 +327,9 @@ LBX_DEV float ex2(float x) {
   return r;
 }
 
-// Is a group's step or least value (plus 8 steps, where codes are centred) an infinity
-// or a NaN?  Either may be alone: a bfloat16 call's least value says nothing of the step.
-LBX_DEV bool kv4_no_number(float step, float least) { return !(fabsf(step) < INFINITY) || !(fabsf(least) < INFINITY); }
+// Is a group's step or least value an infinity or a NaN?  Either may be alone; least + 8 step
+// is then one too.
+LBX_DEV bool kv4_no_number(float least8) { return !(fabsf(least8) < INFINITY); }
 
 // does query i of its sequence see slot j
 LBX_DEV bool kv4_sees(int j, int prefix, int n, int i, bool tree, uint64_t mask) {
@@ -468,6 +487,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
   // accumulator columns it owns rows 2 j and 2 j + 1
   uint32_t qb[NS][2 * NW][2];
   float fq[2], qs[2][NG];  // the queries' unit, and their sums in it
+  float ql[NG][4];         // bfloat16 calls: 8 times what the rounding took from the sums, as accumulators
   int qi[2];               // token index of the rows
   bool rok[2];
   const bool tree = p.tree != nullptr;
@@ -503,6 +523,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
       qi[b] = p.i0 + (rok[b] ? R / p.rep : 0);
       mask[b] = tree && rok[b] ? __ldg(p.tree + (int64_t)s * p.n + qi[b]) : 0ull;
     }
+    float lost[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) lost[g] = 0.f;
 #pragma unroll
     for (int t = 0; t < NW; ++t) {
       float y[8];
@@ -516,7 +539,17 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
         if constexpr (SPLIT) {
           qb[1][2 * t + k][0] = f16x2_rest(b0, y[2 * k], y[2 * k + 4]);
           qb[1][2 * t + k][1] = f16x2_rest(b1, y[2 * k + 1], y[2 * k + 5]);
+        } else {
+          lost[t * NG / NW] += f16x2_lost(b0, y[2 * k], y[2 * k + 4]) + 16.f * f16x2_lost(b1, y[2 * k + 1], y[2 * k + 5]);
         }
+      }
+    }
+    if constexpr (!SPLIT) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float a = quad_sum(lost[g]) * (8.f * 5.9604644775390625e-8f);
+        ql[g][0] = ql[g][2] = __shfl_sync(0xffffffffu, a, 8 * j);
+        ql[g][1] = ql[g][3] = __shfl_sync(0xffffffffu, a, 8 * j + 4);
       }
     }
   }
@@ -592,7 +625,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
 #pragma unroll
             for (int q = 0; q < KS; ++q) {
               const uint32_t(&b)[2] = qb[e][g * KS + q];
-              if (e == NS - 1 && q == 0) mma_f16_first(acc[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
+              if (!SPLIT && q == 0) mma_f16_from(acc[g], ql[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
+              else if (e == NS - 1 && q == 0) mma_f16_first(acc[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
               else mma_f16(acc[g], f[q][0], f[q][1], f[q][2], f[q][3], b[0], b[1]);
             }
         }
@@ -622,7 +656,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           sg[t][g] = kv4_step(pp[g]);
-          lg[t][g] = SPLIT ? fmaf(8.f, sg[t][g], kv4_least(pp[g])) : kv4_least(pp[g]);
+          lg[t][g] = fmaf(8.f, sg[t][g], kv4_least(pp[g]));
           sx[0] = fmaxf(sx[0], fabsf(sg[t][g]));  // (a NaN is passed over)
         }
       }
@@ -638,7 +672,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
               for (int g = 0; g < NG; ++g) {
                 a = fmaxf(a, fabsf(sg[t][g]));
                 // what is not a number reaches the rows that see it, and (below) no other
-                if (kv4_no_number(sg[t][g], lg[t][g])) om[b][g] += __uint_as_float(0x7FC00000u);
+                if (kv4_no_number(lg[t][g])) om[b][g] += __uint_as_float(0x7FC00000u);
               }
             } else {
               sc[t][b] = -INFINITY;
@@ -650,7 +684,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
         for (int t = 0; t < NK; ++t)
 #pragma unroll
           for (int g = 0; g < NG; ++g)
-            if (kv4_no_number(sg[t][g], lg[t][g])) sg[t][g] = lg[t][g] = 0.f;
+            if (kv4_no_number(lg[t][g])) sg[t][g] = lg[t][g] = 0.f;
       }
       // ---- references: a row's moves when its maximum is 2^8 above it (or a step is above all before)
       float mx[2];
@@ -720,6 +754,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
             vw[a][k] = *reinterpret_cast<const uint32_t *>(
                 sv + (16 * a + 8 * (k >> 1) + kv4_key(2 * j + (k & 1))) * (D / 2) + r * (D / 16) + 4 * g);
         }
+        float c8[4];  // bfloat16 calls: -8 times the sum of the rounded weights, where their sums of codes begin
+        if constexpr (!SPLIT) {
+          mma_f16_first(c8, 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pb[0][0][0], pb[0][0][1]);
+#pragma unroll
+          for (int a = 1; a < NK / 2; ++a)
+            mma_f16(c8, 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pb[a][0][0], pb[a][0][1]);
+        }
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {  // nibbles 0-3, 4-7 of the word
           uint32_t v[NK / 2][2];
@@ -744,7 +785,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv4_attn_kernel(const __grid
             for (int e = NS - 1; e >= 0; --e)
 #pragma unroll
               for (int a = 0; a < NK / 2; ++a) {
-                if (e == NS - 1 && a == 0) mma_f16_first(t, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
+                if (!SPLIT && a == 0) mma_f16_from(t, c8, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
+                else if (e == NS - 1 && a == 0) mma_f16_first(t, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
                 else mma_f16(t, f[a][0], f[a][1], f[a][2], f[a][3], pb[a][e][0], pb[a][e][1]);
               }
 #pragma unroll
