@@ -123,3 +123,31 @@ FEW = [(1, 1, 4, 4, 128, 64, 0, False), (1, 1, 32, 32, 128, 4096, 4000, False), 
 @pytest.mark.parametrize("S,n,heads,kvh,d,T,prefix,tree", FEW)
 def test_few_sequences(S, n, heads, kvh, d, T, prefix, tree, dtype):
     _run(S, n, heads, kvh, d, T, [prefix] * S, tree, dtype, range(S))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("small", [0, 1])
+@pytest.mark.parametrize("ratio", [2.0 ** -4, 2.0 ** -8, 2.0 ** -40])
+def test_groups_of_other_magnitudes(ratio, small, dtype):
+    """A weight times a group's step is held relative to the largest step that the row has seen: a group of values
+    2^-8 of its neighbour keeps its own accuracy, and one far below is off by no more than the head's."""
+    from littlebit_b200 import ops
+
+    n, T, d, prefix = 3, 640, 128, 600
+    c = _filled(1, 1, T, d, 5)
+    size = c.v_params.float()
+    size[:, :, :, small] *= ratio
+    c.v_params.copy_(size)
+    q = torch.randn(n, 4 * d, generator=torch.Generator().manual_seed(6)).to(DT[dtype]).cuda()
+    out = ops.attention_kv4(q, c, prefix, None, 4, d ** -0.5).double().reshape(n, 4, 2, 64)
+    k, v = (_values(x[0, :, :prefix + n], p[0, :, :prefix + n], val)[0]
+            for x, p, val in ((c.k_codes, c.k_params, False), (c.v_codes, c.v_params, True)))
+    x = q.double().reshape(n, 4, d)
+    sc = torch.einsum("nhd,td->nht", x, k) * d ** -0.5
+    sc[:, :, prefix:].masked_fill_(~torch.tril(torch.ones(n, n, dtype=torch.bool, device="cuda"))[:, None], -torch.inf)
+    ref = torch.einsum("nht,td->nhd", torch.softmax(sc, -1), v).reshape(n, 4, 2, 64)
+    sigma = float(torch.einsum("nhd,td->", x ** 2, k ** 2) / (4 * n * (prefix + n))) ** 0.5 * d ** -0.5
+    tol = 2.0 ** -20 * (1 + sigma) if dtype == "f32" else (2.0 ** -8 + 2.0 ** -11 * (1 + sigma)) / 3 ** 0.5
+    err, norm = ((out - ref) ** 2).sum((0, 1, 3)).sqrt(), (ref ** 2).sum((0, 1, 3)).sqrt()
+    assert err[1 - small] <= tol * norm[1 - small]
+    assert err[small] <= tol * (norm[small] if ratio >= 2.0 ** -8 else norm[1 - small])
