@@ -521,7 +521,12 @@ int lbx_kv4_read(const lbx_kv4_cache *c /* host */, const int32_t *start, int32_
  * [n_seq * n, heads * head_dim] has q's type.  A query's bits depend neither on
  * the other queries and sequences of the call nor on max_prefix, so a causal
  * run in one call equals its tokens one at a time.  A prefix outside
- * [0, max_prefix] gives NaN rows and records device error 0x803. */
+ * [0, max_prefix] gives NaN rows and records device error 0x803.
+ * Sums and the softmax are held in fp32.  The queries, and the weights times
+ * their group's step, enter the products in 22 bits (LBX_F32) or 11 (LBX_BF16,
+ * whose result has 8); the latter relative to the largest step of the head that the
+ * row has seen, so a group of steps 2^-16 (LBX_BF16: 2^-20) of that and less
+ * loses bits of its own.  Values past 2^100 may overflow on the way. */
 typedef struct lbx_kv4_attn_args {
   lbx_kv4_cache cache;
   int32_t n, heads, max_prefix, dtype, use_pdl;

@@ -128,10 +128,12 @@ __global__ void __launch_bounds__(Q8_THREADS) quant_tokens_kernel(const void *__
 //           cost 10 us there: under a saturated memory a fence, an atomic or a
 //           load takes as long as the queue of loads ahead of it.
 //
-// Bound for few tokens by the weights' stream (1 x 32000 x 4096, 131 MB: 28.5 us with the
-// quantiser, 4.6 TB/s; 8 x 32000 x 8192, 262 MB: 64), for many by the copies from L2 and
-// the clock that the power leaves: a block of 128 x 256 brings 48 KB for 512 cycles of MMA
-// and takes 730 (4096 x 28672 x 8192: 701 us, 2.74 POP/s, tensor pipes busy 70 % of cycles).
+// Bound for few tokens by the weights' stream and what comes before it: 1 x 32000 x 4096, 131 MB,
+// 28.4 us with the quantiser; twice and four times the bytes (8 x 32000 x 8192, x 16384) 50.7 and
+// 94.3: 6.0 TB/s for what is added, and 6.6 us for the quantiser, the first loads and the last results.
+// For many by the copies from L2 and the clock that the power leaves: a block of 128 x 256 brings
+// 48 KB for 512 cycles of MMA and takes 730 (4096 x 28672 x 8192: 701 us by itself, 793 to 833 in a row of
+// calls, 2.74 POP/s, tensor pipes busy 70 % of cycles).
 // Two channel tiles at once from one CTA, a token tile loaded once for both, was slower
 // (1020 us for 897 then: half the stages).
 // ---------------------------------------------------------------------------
@@ -634,8 +636,9 @@ extern "C" int lbx_linear_int8(const lbx_int8_args *a, void *ws, size_t ws_bytes
   if (rc) return rc;
   const int blk = (128 + p.BN) * I8_KB;
   // The even deal is a stream from memory: up to 4 K blocks a stage, so that 512
-  // consecutive bytes of a row are asked for together (262 MB for 8 tokens: 72.7 us with
-  // one block a stage, 66.6 with two, 64.5 with four), with three stages at least.
+  // consecutive bytes of a row are asked for together (262 MB for 8 tokens, behind a flush
+  // whose lines L2 has yet to write back: 72.7 us with one block a stage, 66.6 with two,
+  // 64.5 with four), with three stages at least.
   const int st_max = (int)((smax - 1024) / blk);
   p.KS = !p.units ? 1 : st_max >= 12 ? 4 : st_max >= 6 ? 2 : 1;
   p.ST = std::min(I8_MAXST, st_max / p.KS);

@@ -190,13 +190,15 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 // a decode step's few rows waste half a tile at most and the running sums take 4
 // registers for 16 dimensions.  The weights reach B's layout by one 8 x 8 transposition
 // (movmatrix) a tile.  (Rows as A measured 500 instructions per 16 slots, half of them moves
-// and masks, and 206 us where this form takes 161; two column tiles a warp share the
-// unpacked codes but halve the warps: 341 us against 285 for five tiles.)
+// and masks, and 1.28 times this form's time when it was taken; two column tiles a warp share the
+// unpacked codes but halve the warps: 1.2 times, for five tiles.)
 //
-// What bounds it is issue: 330 (bf16) to 450 (float32) instructions per 16 slots and warp at
+// What bounds it is issue: 340 (bf16) to 450 (float32) instructions per 16 slots and warp at
 // half an instruction a cycle, where 6.5 TB/s would be 400 cycles per 16 slots of
-// 128-wide keys and values.  Neither more warps (queries' fragments in shared memory, 16
-// a multiprocessor: 193 us for 161) nor longer steps (64 slots, 255 registers: 163) change that.
+// 128-wide keys and values: 64 sequences of up to 8100 slots, 64 heads over 8, one token each
+// 126 to 133 us in bf16 and 172 in float32, five tokens 613 and 825.  Neither more warps
+// (queries' fragments in shared memory, 16 a multiprocessor: 1.2 times) nor longer steps
+// (64 slots, 255 registers: equal) changed that.
 //
 // float32 calls (SPLIT) take each query and weight in two fp16 terms, 22 bits;
 // bfloat16 ones in one, 11 bits against the result's 8.
@@ -1056,11 +1058,11 @@ static void kv4_cut(Kv4AttnParams &p, int i0, int nt) {
   p.ntile = (p.R + 7) / 8;
   p.nsub = (end + p.ck - 1) / p.ck;
   // sub-chunks a warp takes on end: a few rounds of warps are enough, and the
-  // queries' fragments are made once for all of them (5 tokens of 64
+  // queries' fragments are made once for all of them (bf16, 5 tokens of 64
   // sequences over up to 4000 slots, 64 heads over 8: 370 us, one sub-chunk each 417)
   const int64_t units = (int64_t)p.c.n_seq * p.c.kvh * p.ntile * p.nsub;
   p.cpw = (int)std::min<int64_t>(8, std::max<int64_t>(1, units / (48 * device_sm_count())));
-  // Row tiles a block, evenly (5 tiles, 64 sequences over 4000 slots: 370 us sharing the
+  // Row tiles a block, evenly (the same 5 tiles: 370 us sharing the
   // ring, 398 each with its own); with one sub-chunk a warp a tile has its own ring (5 tiles
   // over 130 000 slots: 245 us, shared 280).  The warps left take further runs.
   const int groups = (p.ntile + KA_WARPS - 1) / KA_WARPS;
